@@ -35,6 +35,7 @@ extern "C" {
 #endif
 #define PKV_NOALLOC_MAX_PARTS 320     /* pkv_decode_attn_noalloc: upper bound on batch * n_split */
 #define PKV_SMALL_WRITE_TOKENS 64    /* pkv_cache_write spreads the projection over the GPU up to this n */
+#define PKV_TREE_MAX 64              /* drafted tokens of one sequence in a tree (bits of a mask word) */
 #define PKV_VQ_TILE_BYTES 8448       /* quantised V: bytes per (page, kv head): 128 tokens x 64 bytes of codes + 128 bf16 scales */
 
 enum pkv_status {
@@ -417,6 +418,59 @@ int pkv_merge_exchange(const pkv_exchange_t* x, const float* parts_dev, int64_t 
 int pkv_decode_attn_noalloc(const pkv_layer_t* layer, const pkv_cache_t* cache, const void* qop_dev,
                             const int32_t* page_table_dev, int32_t max_pages, const int32_t* seqlens_dev,
                             int32_t batch, int32_t n_split, float* out_dev, int32_t* status_dev, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------------------
+ * A speculative step: every sequence of a batch gets a few drafted tokens, a chain or a tree, that are written behind its
+ * cached tokens, attend to them and to one another, and of which a path is kept (no counterpart in the reference, which
+ * decodes token by token and has no pages).  Ragged: the tokens of sequence b are the rows cu[b] .. cu[b+1]-1 of every
+ * per-token array.  All lengths live on the device, so that a step can be captured in a CUDA graph and replayed.
+ * status_dev words of these calls besides 1 and 2 above: 4 = a length, a parent or an index out of range (word 1: the
+ * sequence), 5 = the page pool has too few pages (word 1: how many are missing) or would get back more than it has. */
+
+/* The page table of a batch.  free_dev: optional page pool, int32 [n_pages + 1]: the number of free pages, then the free
+ * pages as a stack (the next page is free_dev[free_dev[0]]).  NULL: every table row is filled for good. */
+typedef struct pkv_pages {
+    int32_t* page_table_dev;         /* [batch, max_pages] */
+    int32_t* seqlens_dev;            /* [batch] tokens stored */
+    int32_t* free_dev;
+    int32_t  batch, max_pages, n_pages;
+} pkv_pages_t;
+
+/* What pkv_plan_step fills.  Buffers are the caller's; ticket_dev is one uint32, zero before its first use. */
+typedef struct pkv_plan {
+    int32_t* cu_dev;                 /* [batch + 1] first row of each sequence */
+    int32_t* seq_dev;                /* [capacity] sequence of each token */
+    int32_t* positions_dev;          /* [capacity] position: the place in the sequence, or in a tree length + depth */
+    int32_t* slots_dev;              /* [capacity] page * 128 + row; -1 behind the last token (the writers skip it) */
+    int64_t* mask_dev;               /* [capacity] ancestors of a drafted token and itself, bit = row in its sequence; may be NULL without parents */
+    uint32_t* ticket_dev;
+    int32_t* status_dev;             /* optional int32[4] */
+    int32_t  capacity;
+} pkv_plan_t;
+
+/* Room for n_new_dev[b] >= 0 more tokens in every sequence: pages from the pool (in the order of the sequences), table
+ * entries, slots and positions, and seqlens += n_new.  parents_dev (optional, [capacity], ragged like the rest): row of
+ * each token's parent within its sequence, before the token itself, or -1 for a child of the last cached token; then
+ * n_new <= PKV_TREE_MAX, and masks are filled too.  The other arrays behind the last token are left as they were.
+ * When a length, a parent or the pool does not allow the step, the call changes no table and no length, cu is all zero,
+ * every slot is -1 and the status says why.  batch <= 4096. */
+int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev, const int32_t* parents_dev, const pkv_plan_t* plan,
+                  void* stream);
+
+/* seqlens[b] = min(seqlens[b], lengths_dev[b]); pages that hold no token any more go back to the pool, their table entries
+ * become -1.  A step that is planned and dropped leaves the pool as it was.  lengths_dev must not be seqlens_dev. */
+int pkv_truncate(const pkv_pages_t* pages, const int32_t* lengths_dev, int32_t* status_dev, void* stream);
+
+/* The accepted path: keep_dev [capacity] (ragged by cu_dev: the first n_keep_dev[b] <= PKV_TREE_MAX entries of a sequence's
+ * rows count) names rows of the step's tokens in ascending order; row base + keep[j] moves to base + j, base = seqlens -
+ * (cu[b+1] - cu[b]), in the latent and value pages of every layer (layers: host array of n_layers caches that are addressed
+ * by the same table; no cache twice).  Only bytes move: a token keeps its rotation, so a kept path's positions must
+ * be base, base + 1, ... (in a tree, depths 0, 1, ...).  lengths_out_dev (optional, [batch], not seqlens_dev): base + n_keep,
+ * for pkv_truncate.  Lengths and tables stay as they are.  A sequence whose indices do not ascend or are out of range is
+ * left alone (status 4, lengths_out = its length). */
+int pkv_keep_rows(const pkv_cache_t* const* layers, int32_t n_layers, const pkv_pages_t* pages, const int32_t* cu_dev,
+                  int32_t capacity, const int32_t* keep_dev, const int32_t* n_keep_dev, int32_t* lengths_out_dev,
+                  int32_t* status_dev, void* stream);
 
 /* Measurement aid (no counterpart in the reference): reads `bytes` (16-byte aligned buffer) once with plain
  * 16-byte loads from every SM and discards them; sink_dev is one uint32 the kernel may add to.  Timed by

@@ -15,6 +15,7 @@ PAGE_TOKENS = 128
 MAX_WIDTH = 256
 QUERY_TERMS = 4
 NOALLOC_MAX_PARTS = 320
+TREE_MAX = 64
 F32, BF16, F64 = 0, 1, 2
 ATTN_SCORES_ONLY, ATTN_SIMT, ATTN_PACKED_OUT, ATTN_EARLY_STREAM, ATTN_TAIL_WRITTEN, ATTN_QUERY_READY = 1, 2, 4, 8, 16, 32
 EXCHANGE_PUSH, EXCHANGE_MERGE = 1, 2
@@ -49,6 +50,18 @@ class LayerHost(ctypes.Structure):
 class Cache(ctypes.Structure):
     _fields_ = [("latent_dev", c_void_p), ("v_dev", c_void_p), ("n_pages", c_int32), ("W", c_int32),
                 ("n_kv", c_int32), ("head_dim", c_int32), ("vq_dev", c_void_p), ("v_bits", c_int32)]
+
+
+class Pages(ctypes.Structure):
+    """struct pkv_pages"""
+    _fields_ = [("page_table_dev", c_void_p), ("seqlens_dev", c_void_p), ("free_dev", c_void_p), ("batch", c_int32),
+                ("max_pages", c_int32), ("n_pages", c_int32)]
+
+
+class Plan(ctypes.Structure):
+    """struct pkv_plan"""
+    _fields_ = [("cu_dev", c_void_p), ("seq_dev", c_void_p), ("positions_dev", c_void_p), ("slots_dev", c_void_p),
+                ("mask_dev", c_void_p), ("ticket_dev", c_void_p), ("status_dev", c_void_p), ("capacity", c_int32)]
 
 
 #: name -> (restype, argtypes); the complete exported surface of include/phasorkv_b200.h
@@ -104,6 +117,10 @@ SIGNATURES = {
     "pkv_vq_page_bytes": (c_int64, [c_int32, c_int32]),
     "pkv_vq_write": (c_int32, [POINTER(Cache), c_void_p, c_void_p, c_int32, c_void_p]),
     "pkv_vq_read": (c_int32, [POINTER(Cache), c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pkv_plan_step": (c_int32, [POINTER(Pages), c_void_p, c_void_p, POINTER(Plan), c_void_p]),
+    "pkv_truncate": (c_int32, [POINTER(Pages), c_void_p, c_void_p, c_void_p]),
+    "pkv_keep_rows": (c_int32, [POINTER(POINTER(Cache)), c_int32, POINTER(Pages), c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+                                c_void_p, c_void_p]),
     "pkv_read_probe": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p]),
     "pkv_merge": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                             c_void_p]),
@@ -142,3 +159,21 @@ def ptr(t) -> c_void_p:
 def current_stream() -> c_void_p:
     import torch
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def need(t, dtype, shape, device, what: str) -> None:
+    """Refuses a tensor that a kernel would misread: another type, shape, device or order."""
+    if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device.type != device.type or \
+            (device.index is not None and t.device.index != device.index):
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
+                         f"got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def on_device(device):
+    """Context in which `device` is the current one (nothing to do when it is already)."""
+    import contextlib
+
+    import torch
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)

@@ -68,6 +68,8 @@ class PagedLatentCache:
         pt = torch.arange(batch * self.max_pages, dtype=torch.int32).reshape(batch, self.max_pages)
         self.page_table = (pt % self.n_pages).to(self.device)
         self.seqlens = torch.zeros(batch, dtype=torch.int32, device=self.device)
+        self.free = None                                    # page pool, see use_page_pool()
+        self.status = None                                  # status words of truncate / keep_rows, made with the first plan
         self.c = _lib.Cache(self.latent.data_ptr(), 0 if self.v is None else self.v.data_ptr(), self.n_pages, W,
                             n_kv, head_dim, 0 if self.vq is None else self.vq.data_ptr(), self.v_bits)
 
@@ -75,6 +77,82 @@ class PagedLatentCache:
         """Slot (page * 128 + row) of token `local_pos` of sequence `seq`; int32 tensors on the device."""
         page = self.page_table[seq.long(), (local_pos // PAGE_TOKENS).long()]
         return (page * PAGE_TOKENS + (local_pos % PAGE_TOKENS).to(torch.int32)).to(torch.int32)
+
+    # ------------------------------------------------------------------ pages of a step
+    def use_page_pool(self) -> None:
+        """Pages are handed out by `plan_step` and come back with `truncate` from here on, instead of every sequence owning a
+        fixed row of them. Forgets what is cached. ``free[0]`` counts the free pages, ``free[free[0]]`` is the next."""
+        self.free = torch.cat([torch.tensor([self.n_pages], dtype=torch.int32),
+                               torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32)]).to(self.device)
+        self.page_table.fill_(-1)
+        self.seqlens.zero_()
+
+    def share_pages(self, owner: "PagedLatentCache") -> None:
+        """Address this layer's pools by `owner`'s page table, lengths and pool (one plan then serves all layers)."""
+        mine, theirs = ((c.batch, c.max_pages, c.n_pages, c.latent.device) for c in (self, owner))
+        if mine != theirs:
+            raise ValueError("caches that share pages have the same batch, pages per sequence, pool size and device")
+        self.page_table, self.seqlens, self.free = owner.page_table, owner.seqlens, owner.free
+
+    def _pages(self) -> _lib.Pages:
+        return _lib.Pages(self.page_table.data_ptr(), self.seqlens.data_ptr(), 0 if self.free is None else self.free.data_ptr(),
+                          self.batch, self.max_pages, self.n_pages)
+
+    def _status(self) -> torch.Tensor:
+        if self.status is None:
+            self.status = torch.zeros(4, dtype=torch.int32, device=self.device)
+        return self.status
+
+    def step_plan(self, capacity: int, tree: bool = False) -> "StepPlan":
+        """Buffers for `plan_step`: up to `capacity` tokens over all sequences; `tree`: with ancestor masks."""
+        self._status()
+        return StepPlan(self.batch, int(capacity), tree, self.latent.device)
+
+    def plan_step(self, plan: "StepPlan", n_new: torch.Tensor, parents: Optional[torch.Tensor] = None) -> None:
+        """Room for ``n_new[b]`` (int32 [batch], on the device) more tokens in every sequence: pages from the pool, `seqlens`,
+        and the tokens' sequence, position, slot and, with `parents` (int32 [capacity]), ancestor mask into `plan`.
+        ``parents[i]`` is the row of token i's parent among its sequence's new tokens, before i, or -1; positions are then
+        length + depth. A step that does not fit changes nothing: ``plan.cu`` is zero, every slot -1, ``plan.status`` says why."""
+        _lib.need(n_new, torch.int32, (self.batch,), self.latent.device, "n_new")
+        if parents is not None:
+            _lib.need(parents, torch.int32, (plan.capacity,), self.latent.device, "parents")
+            if plan.mask is None:
+                raise ValueError("parents need a plan with masks: step_plan(capacity, tree=True)")
+        plan._match(self)
+        pg = self._pages()
+        with _lib.on_device(self.latent.device):
+            _lib.check(_lib.load().pkv_plan_step(ctypes.byref(pg), _lib.ptr(n_new), _lib.ptr(parents), ctypes.byref(plan.c),
+                                                 _lib.current_stream()), "pkv_plan_step")
+
+    def truncate(self, lengths: torch.Tensor) -> None:
+        """At most ``lengths[b]`` (int32 [batch], on the device) tokens of every sequence stay; whole pages behind them go back
+        to the pool. Negative lengths are refused (nothing changes, ``status[0]`` = 4)."""
+        _lib.need(lengths, torch.int32, (self.batch,), self.latent.device, "lengths")
+        pg = self._pages()
+        with _lib.on_device(self.latent.device):
+            _lib.check(_lib.load().pkv_truncate(ctypes.byref(pg), _lib.ptr(lengths), _lib.ptr(self._status()), _lib.current_stream()),
+                       "pkv_truncate")
+
+    def keep_rows(self, plan: "StepPlan", keep: torch.Tensor, n_keep: torch.Tensor, lengths: Optional[torch.Tensor] = None,
+                  layers: Optional[Sequence["PagedLatentCache"]] = None) -> None:
+        """Move the rows of an accepted path behind the cached tokens. The first ``n_keep[b]`` of ``keep[plan.cu[b]:]``
+        name rows of the planned step's tokens of sequence b, ascending, whose positions follow one another; they become
+        its tokens base, base + 1, ... in every cache of `layers` (default: this one; others share its table).
+        `lengths` (int32 [batch]) receives base + n_keep, ready for `truncate`, which has to follow."""
+        _lib.need(keep, torch.int32, (plan.capacity,), self.latent.device, "keep")
+        _lib.need(n_keep, torch.int32, (self.batch,), self.latent.device, "n_keep")
+        if lengths is not None:
+            _lib.need(lengths, torch.int32, (self.batch,), self.latent.device, "lengths")
+        plan._match(self)
+        layers = [self] if layers is None else list(layers)
+        if any(c.page_table.data_ptr() != self.page_table.data_ptr() for c in layers):
+            raise ValueError("layers must share this cache's page table (share_pages)")
+        pg = self._pages()
+        arr = (ctypes.POINTER(_lib.Cache) * len(layers))(*[ctypes.pointer(c.c) for c in layers])
+        with _lib.on_device(self.latent.device):
+            _lib.check(_lib.load().pkv_keep_rows(arr, len(layers), ctypes.byref(pg), _lib.ptr(plan.cu), plan.capacity, _lib.ptr(keep),
+                                                 _lib.ptr(n_keep), _lib.ptr(lengths), _lib.ptr(self._status()), _lib.current_stream()),
+                       "pkv_keep_rows")
 
     def v_rows(self, slots: torch.Tensor) -> torch.Tensor:
         """Value rows [n, n_kv, head_dim] stored at `slots` (page * 128 + row); quantised pages: dequantised fp32."""
@@ -139,6 +217,28 @@ class PagedLatentCache:
                                               _lib.ptr(r), _lib.ptr(c), _lib.ptr(s), _lib.current_stream()),
                    "pkv_cache_read")
         return r, c, s
+
+
+class StepPlan:
+    """What `PagedLatentCache.plan_step` fills, for the step's other calls: ``cu`` [batch + 1] first row of every sequence,
+    and for each of up to `capacity` tokens its sequence ``seq``, ``positions``, ``slots`` (-1 behind the last token) and, in
+    a tree, the 64-bit word ``mask`` of the drafted tokens it attends to (its ancestors and itself)."""
+
+    def __init__(self, batch: int, capacity: int, tree: bool, device):
+        if capacity < 0:
+            raise ValueError("capacity must not be negative")
+        self.batch, self.capacity, self.device = batch, capacity, torch.device(device)
+        z = lambda n, dt: torch.zeros(n, dtype=dt, device=device)
+        self.cu = z(batch + 1, torch.int32)
+        self.seq, self.positions, self.slots = z(capacity, torch.int32), z(capacity, torch.int32), z(capacity, torch.int32)
+        self.mask = z(capacity, torch.int64) if tree else None
+        self.ticket, self.status = z(1, torch.int32), z(4, torch.int32)
+        self.c = _lib.Plan(self.cu.data_ptr(), self.seq.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(),
+                           0 if self.mask is None else self.mask.data_ptr(), self.ticket.data_ptr(), self.status.data_ptr(), capacity)
+
+    def _match(self, cache: "PagedLatentCache") -> None:
+        if self.batch != cache.batch or self.device != cache.latent.device:
+            raise ValueError("the plan was made for another batch or device")
 
 
 class DecodeWorkspace:
