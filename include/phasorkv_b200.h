@@ -461,6 +461,23 @@ int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev, const int3
  * become -1.  A step that is planned and dropped leaves the pool as it was.  lengths_dev must not be seqlens_dev. */
 int pkv_truncate(const pkv_pages_t* pages, const int32_t* lengths_dev, int32_t* status_dev, void* stream);
 
+/* Attention of drafted tokens: row i of sequence b's rows cu_dev[b] .. cu_dev[b+1]-1 attends to the sequence's cached tokens
+ * (places 0 .. base-1, base = seqlens - rows) and to those of its drafted tokens (places base + j, written before) whose
+ * bit j is set in mask_dev[i]; bits past the sequence's rows are ignored, mask_dev NULL: bits 0 .. i.  A row that sees
+ * nothing gets zeros.
+ *   q_dev [n_tokens, n_q, 128] pre-RoPE, fp32 or bf16 (q_dtype), absorbed at positions_dev [n_tokens]
+ *   out_dev [n_tokens, n_q, 128] bf16; rows behind cu_dev[batch] are left as they were
+ *   max_draft <= PKV_TREE_MAX: most rows of one sequence
+ *   workspace_dev: pkv_tree_workspace_bytes(layer, batch, max_draft, max_pages) bytes, 1024-byte aligned
+ * Any n_q / n_kv up to 64, head_dim 128, bf16 or quantised value pages.  Rows that a token does not see may hold anything
+ * (infinities and NaN in their values too).  A drafted value row with an infinity or NaN makes the outputs that see it
+ * NaN.  A sequence with more rows than max_draft, n_tokens or its length allow is left out (status 4). */
+int64_t pkv_tree_workspace_bytes(const pkv_layer_t* layer, int32_t batch, int32_t max_draft, int32_t max_pages);
+int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache, const pkv_pages_t* pages, const void* q_dev,
+                  int32_t q_dtype, const int32_t* positions_dev, const int64_t* mask_dev, const int32_t* cu_dev,
+                  int32_t n_tokens, int32_t max_draft, void* workspace_dev, int64_t workspace_bytes, void* out_dev,
+                  int32_t* status_dev, void* stream);
+
 /* The accepted path: keep_dev [capacity] (ragged by cu_dev: the first n_keep_dev[b] <= PKV_TREE_MAX entries of a sequence's
  * rows count) names rows of the step's tokens in ascending order; row base + keep[j] moves to base + j, base = seqlens -
  * (cu[b+1] - cu[b]), in the latent and value pages of every layer (layers: host array of n_layers caches that are addressed

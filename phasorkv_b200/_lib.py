@@ -121,6 +121,9 @@ SIGNATURES = {
     "pkv_truncate": (c_int32, [POINTER(Pages), c_void_p, c_void_p, c_void_p]),
     "pkv_keep_rows": (c_int32, [POINTER(POINTER(Cache)), c_int32, POINTER(Pages), c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p]),
+    "pkv_tree_workspace_bytes": (c_int64, [POINTER(Layer), c_int32, c_int32, c_int32]),
+    "pkv_tree_attn": (c_int32, [POINTER(Layer), POINTER(Cache), POINTER(Pages), c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+                                c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]),
     "pkv_read_probe": (c_int32, [c_void_p, c_int64, c_void_p, c_void_p]),
     "pkv_merge": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p,
                             c_void_p]),

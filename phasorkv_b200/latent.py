@@ -262,6 +262,24 @@ class DecodeWorkspace:
         self.exact = None                                                     # exact-token partial, see exact_step()
 
 
+class TreeWorkspace:
+    """Scratch of `PhasorKey.tree_step` (the absorbed queries in operand form, partial results), reused by every layer of
+    one shape and every step; ``status`` holds the kernels' status words."""
+
+    def __init__(self, pk: "PhasorKey", batch: int, capacity: int, max_draft: int, max_tokens: int):
+        if not 1 <= max_draft <= _lib.TREE_MAX:
+            raise ValueError(f"a tree has 1 .. {_lib.TREE_MAX} drafted tokens per sequence, not {max_draft}")
+        if batch < 0 or capacity < 0 or max_tokens <= 0:
+            raise ValueError("batch, capacity and max_tokens must not be negative")
+        self.batch, self.capacity, self.max_draft, self.key = batch, capacity, max_draft, pk._tree_key()
+        self.max_pages = (max_tokens + PAGE_TOKENS - 1) // PAGE_TOKENS
+        n = int(_lib.load().pkv_tree_workspace_bytes(ctypes.byref(pk._layer()), batch, max_draft, self.max_pages))
+        if n < 0:
+            _lib.check(n, "pkv_tree_workspace_bytes")
+        self.buffer = _aligned_bytes(n, pk.device)
+        self.status = torch.zeros(4, dtype=torch.int32, device=pk.device)
+
+
 class PhasorKey:
     """The phasor key cache of one layer.
 
@@ -660,6 +678,41 @@ class PhasorKey:
         self.absorb_step(q, positions, ws, operand=not simt)
         self.attend_step(cache, ws, simt=simt, scores_only=scores_only, out=ws.out, after_absorb=True)
         return ws.out
+
+    def tree_workspace(self, batch: int, capacity: int, max_draft: int, max_tokens: int) -> TreeWorkspace:
+        """Scratch of `tree_step` for up to `capacity` drafted tokens, `max_draft` (<= 64) a sequence, on caches of up to
+        `max_tokens` tokens a sequence. Calls that may run at the same time need one each."""
+        return TreeWorkspace(self, int(batch), int(capacity), int(max_draft), int(max_tokens))
+
+    def tree_step(self, cache: PagedLatentCache, q: torch.Tensor, plan: StepPlan, ws: TreeWorkspace,
+                  out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Attention of the step's drafted tokens, which are written already: q [n, H, d] pre-RoPE (bf16 or fp32), ragged by
+        ``plan.cu``, at ``plan.positions`` -> out [n, H, d] bf16. Row i attends to all tokens cached before the step and to the
+        drafted tokens of its sequence named by ``plan.mask[i]`` (a plan without masks: to those up to itself). A row
+        that sees nothing gets zeros, rows behind ``plan.cu[-1]`` are left as they were."""
+        self._need_inv_freq("tree_step")
+        n, dev = q.shape[0], cache.latent.device
+        if q.dtype not in (torch.bfloat16, torch.float32):
+            raise ValueError(f"q must be bfloat16 or float32, got {q.dtype}")
+        _lib.need(q, q.dtype, (n, self.n_q, self.head_dim), dev, "q")
+        if out is None:
+            out = torch.zeros(q.shape, dtype=torch.bfloat16, device=dev)
+        else:
+            _lib.need(out, torch.bfloat16, q.shape, dev, "out")
+        plan._match(cache)
+        if n > plan.capacity or n > ws.capacity or ws.batch != cache.batch or ws.max_pages < cache.max_pages or ws.key != self._tree_key():
+            raise ValueError("q has more rows than the plan or the workspace, or the workspace was made for another layer shape or cache")
+        pg = cache._pages()
+        L = self._layer()
+        with _lib.on_device(dev):
+            _lib.check(_lib.load().pkv_tree_attn(ctypes.byref(L), ctypes.byref(cache.c), ctypes.byref(pg), _lib.ptr(q), self._xdt(q),
+                                                 _lib.ptr(plan.positions), _lib.ptr(plan.mask), _lib.ptr(plan.cu), n, ws.max_draft,
+                                                 _lib.ptr(ws.buffer), ws.buffer.numel(), _lib.ptr(out), _lib.ptr(ws.status),
+                                                 _lib.current_stream()), "pkv_tree_attn")
+        return out
+
+    def _tree_key(self):
+        return self.n_q, self.n_kv, self.cache_width
 
     # ------------------------------------------------------------------ plumbing
     def _layer(self) -> _lib.Layer:
