@@ -3,161 +3,985 @@
 //   S[i, h, t] = q'_{i,h} . c_t,   O[i, h] = softmax_t(S d^-1/2) V_{g(h)}   over t < base and t = base + j, bit j of mask_i
 //
 // with q' the absorbed query of drafted token i (conj(A) zq e^{i theta pos}; slow dims unrotated) and c_t the NVFP4 rows.
-// First form, on the CUDA cores: a CTA takes one drafted token, one kv head and up to eight of its query heads and
-// walks the sequence page by page, a token per thread for the scores, a dim per thread for P.V.
+//
+// The latent of a token serves all heads, so the rows of a score tile may be any mix of (kv head, drafted token, query
+// head): a tile has 128 rows, `rph` for each of its G kv heads, and every CTA walks the pages of a sequence for one
+// tile. Per page and tile:
+//   S  [128 rows x 128 tokens]  = Q' . C^T     block-scaled NVFP4 tcgen05.mma, the four residual terms of the query added up
+//                                              in tensor memory; a page is the B operand as it is stored
+//   P  = 2^(S - m)              one row per thread: maximum, sum and mask need no other thread
+//   O^T[128 dims x rph] += V_g^T . P_g^T       bf16 tcgen05.mma, a kv head at a time, V as stored
+// With few drafted tokens the V pages bound it (HBM), with many the score MMAs and the softmax.
+//
+// Three launches: the operand (absorbed queries), the attention, the merge of what several CTAs did of one tile.
+#include "pkv_absorb.cuh"
 #include "pkv_common.cuh"
+#include "pkv_tcgen05.cuh"
+
+#include <cudaTypedefs.h>
+#include <cstring>
 
 int pkv_check_layer(const pkv_layer_t* L);
 int pkv_check_cache(const pkv_cache_t* c);
 
 namespace {
 
-constexpr int DH = 128, NT = 128, RC = 8;
+using namespace pkv;
 
-struct Args {
+constexpr int DH = 128, ROWS = 128;                  // head dim; rows of a tile
+constexpr int HALF = 64;                             // tokens per V stage: half a page of one kv head
+constexpr int MAX_G = 8;                             // kv heads of a tile (16 rows at least each)
+constexpr float RESCALE_THRESHOLD = 8.0f;            // in base-2 logits
+constexpr uint32_t WAIT_LIMIT = 1u << 19;            // probes of a bounded wait
+
+// ------------------------------------------------------------------------------------------------ tiles and their pages
+// A tile index z = blk * groups + group: `qpb` drafted tokens from blk * qpb on, kv heads group * G .. . Row r of the tile:
+// kv head r / rph, drafted token (r % rph) / rep, query head (r % rph) % rep of the kv head.
+struct Tiles {
+    int rep, qpb, rph, G, groups, Z;
+    int gang, passes, gangs;                         // CTAs that walk the same pages side by side; rounds over the tiles
+};
+
+struct Batch {
+    const int32_t *cu, *seqlens;
+    int batch, max_pages, n_tokens, max_draft;
+    // pages of sequence b, 0 when it has no drafted token or its numbers do not fit
+    __device__ __forceinline__ int pages(int b, int& lo, int& n, int& T) const {
+        lo = cu[b];
+        n = cu[b + 1] - lo;
+        T = seqlens[b];
+        const bool ok = n > 0 && n <= max_draft && lo >= 0 && lo <= n_tokens - n && T >= n && T <= max_pages * PKV_PAGE_TOKENS;
+        return ok ? (T + PKV_PAGE_TOKENS - 1) / PKV_PAGE_TOKENS : 0;
+    }
+};
+
+// Work is a list of pages: sequence by sequence, `passes` times over its pages. Gang x of X takes the pages
+// [x U / X, (x + 1) U / X) of the U on the list, its CTA zi the tile pass * gang + zi: the tiles of a sequence read a page
+// at about the same time (from L2 all but the first), and every CTA streams as many pages whatever the lengths are.
+__device__ __forceinline__ long gang_start(long U, int gangs, int x) { return U * x / gangs; }
+__device__ __forceinline__ int gang_of(long U, int gangs, long u) { return (int)(((u + 1) * gangs - 1) / U); }
+
+struct Part {                                        // a stretch of pages of one tile
+    int b, z, p_lo, p_hi, pages, lo, n, T;
+};
+
+struct Walk {
+    int b, pass, p, left;
+    __device__ __forceinline__ bool next(const Batch& B, const Tiles& X, int zi, Part& s) {
+        while (left > 0 && b < B.batch) {
+            s.pages = B.pages(b, s.lo, s.n, s.T);
+            if (s.pages == 0) { ++b; continue; }
+            const int take = min(left, s.pages - p);
+            s.b = b; s.z = pass * X.gang + zi; s.p_lo = p; s.p_hi = p + take;
+            left -= take;
+            p += take;
+            if (p == s.pages) { p = 0; if (++pass == X.passes) { pass = 0; ++b; } }
+            if (s.z < X.Z && s.z / X.groups * X.qpb < s.n) return true;      // else: no row of this tile in this sequence
+        }
+        return false;
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ operand
+// Tile operand of a (sequence, tile): four residual terms, each a 128-row tile laid out like a cache page (swizzled codes,
+// then the block scales), and 128 fp32 row scales.
+__host__ __device__ constexpr int page_bytes(int WP) { return PKV_PAGE_TOKENS * WP / 2 + WP / 64 * 512; }
+__host__ __device__ constexpr int blob_bytes(int WP) { return PKV_QUERY_TERMS * page_bytes(WP) + ROWS * 4; }
+
+struct AbsorbArgs {
     pkv_layer_t L;
-    pkv_cache_t C;
-    pkv_pages_t pg;
+    Batch B;
+    Tiles X;
     const void* q;
-    int q_bf16, n_tokens, max_draft;
-    const int32_t *positions, *cu;
+    int q_bf16;
+    const int32_t* positions;
+    uint8_t* blobs;
+    int32_t* status;
+};
+
+constexpr int AR = 16;                               // rows per CTA
+
+// CTA (16 rows of a tile, tile, sequence); WP / 16 threads per row, each with one 16-column block in registers. Rows that
+// no drafted token has are not written: a row of garbage only reaches its own column of the result, which nobody reads.
+template <int WP>
+__global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const AbsorbArgs A) {
+    constexpr int NB = WP / 16, NT = AR * NB, RB = WP / 2;
+    __shared__ float2 zq[AR][DH / 2];
+    __shared__ float2 ph[AR][DH / 2];
+    __shared__ float raw[AR][DH];
+    const pkv_layer_t& L = A.L;
+    const int tid = threadIdx.x, z = blockIdx.y, b = blockIdx.z, r0 = blockIdx.x * AR;
+    pkv_grid_wait();                                 // everything before this launch is done ..
+    pkv_grid_launch_dependents();                    // .. so the attention behind it may stream pages while this one still runs
+    int lo, n, T;
+    const int pages = A.B.pages(b, lo, n, T);
+    if (pages == 0) {
+        if (n != 0 && A.status && tid == 0 && blockIdx.x == 0 && z == 0) { atomicExch(&A.status[0], 4); atomicExch(&A.status[1], b); }
+        return;
+    }
+    const int rep = A.X.rep, blk = z / A.X.groups, first = blk * A.X.qpb, nq = min(A.X.qpb, n - first);
+    const int g = (z % A.X.groups) * A.X.G + r0 / A.X.rph, rr0 = r0 % A.X.rph;      // rph is a multiple of 16: one kv head per CTA
+    const int rows = min(AR, nq * rep - rr0);
+    if (nq <= 0 || r0 / A.X.rph >= A.X.G || g >= L.n_kv || rows <= 0) return;
+    // this CTA's rows belong to the drafted tokens q_lo .. q_hi
+    const int q_lo = rr0 / rep, q_hi = (rr0 + rows - 1) / rep;
+    for (int k = tid; k < rows * (DH / 4); k += NT) {
+        const int r = k / (DH / 4), c = k % (DH / 4) * 4, rr = rr0 + r;
+        const size_t o = ((size_t)(lo + first + rr / rep) * L.n_q + g * rep + rr % rep) * DH + c;
+        float4 v;
+        if (A.q_bf16) {
+            const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)A.q + o);
+            v = make_float4(pkv_bf16_bits_to_float(u.x & 0xffffu), pkv_bf16_bits_to_float(u.x >> 16), pkv_bf16_bits_to_float(u.y & 0xffffu),
+                            pkv_bf16_bits_to_float(u.y >> 16));
+        } else {
+            v = *reinterpret_cast<const float4*>((const float*)A.q + o);
+        }
+        *reinterpret_cast<float4*>(&raw[r][c]) = v;
+    }
+    for (int k = tid; k < (q_hi - q_lo + 1) * (DH / 2); k += NT) {       // phasors: the angle in 64 bits
+        const int j = k % (DH / 2);
+        double sn, cs;
+        sincos((double)A.positions[lo + first + q_lo + k / (DH / 2)] * L.inv_freq_dev[j], &sn, &cs);
+        ph[k / (DH / 2)][j] = make_float2((float)((double)L.attn_scale * cs), (float)((double)L.attn_scale * sn));
+    }
+    __syncthreads();
+    for (int k = tid; k < rows * (DH / 2); k += NT) {
+        const int r = k / (DH / 2), j = k % (DH / 2);
+        const float2 p = ph[(rr0 + r) / rep - q_lo][j];
+        const float x = raw[r][j], y = raw[r][j + DH / 2];
+        zq[r][j] = make_float2(x * p.x - y * p.y, x * p.y + y * p.x);
+    }
+    __syncthreads();
+    const int r = tid / NB, j = tid % NB, R = L.R, W = 2 * R + L.R_s;
+    const bool live = r < rows;
+    float res[16], am = 0.0f;
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int c = j * 16 + i;
+        float v = 0.0f;
+        if (live && c < 2 * R) {                     // conj(A) zq
+            const int k = c < R ? c : c - R;
+            const float2 w = zq[r][L.freq_dev[k]];
+            const float ar = L.A_re_dev[g * R + k], ai = L.A_im_dev[g * R + k];
+            v = c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x;
+        } else if (live && c < W) {                  // slow dims: the raw query
+            for (int s = 0; s < 2 * L.n_slow; ++s)
+                v = fmaf(raw[r][s < L.n_slow ? L.slow_dev[s] : L.slow_dev[s - L.n_slow] + DH / 2],
+                         L.A_s_dev[((size_t)g * 2 * L.n_slow + s) * L.R_s + c - 2 * R], v);
+        }
+        // tiers: the cache's block is in units of its own scale while the attention applies the layer's one
+        if (L.second_blocks_dev && c < W) v *= L.second_blocks_dev[c >> 4] / L.second;
+        res[i] = v;
+        am = fmaxf(am, fabsf(v));
+        fine = fine && fabsf(v) < INFINITY;
+    }
+#pragma unroll
+    for (int o = NB / 2; o; o >>= 1) {
+        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+        fine = __shfl_xor_sync(0xffffffffu, fine ? 1 : 0, o) && fine;
+    }
+    if (!live) return;
+    const float second = fmaxf(am, 1e-30f) * (1.0f / (448.0f * 6.0f)), inv = __frcp_rn(second);
+    uint8_t* blob = A.blobs + ((size_t)b * A.X.Z + z) * blob_bytes(WP);
+    const uint32_t row = r0 + r;
+#pragma unroll 1
+    for (int t = 0; t < PKV_QUERY_TERMS; ++t) {
+        uint8_t sb;
+        const uint2 packed = pkv_absorb_impl::quantize_query_block16(res, second, inv, sb);
+        uint8_t* tile = blob + t * page_bytes(WP);
+        *reinterpret_cast<uint2*>(tile + pkv_code_offset(row, j * 8, RB)) = packed;
+        tile[PKV_PAGE_TOKENS * RB + pkv_scale_offset(row, j)] = sb;
+    }
+    // a query that is not finite makes its whole row NaN
+    if (j == 0) reinterpret_cast<float*>(blob + PKV_QUERY_TERMS * page_bytes(WP))[row] = fine ? second : __int_as_float(0x7fc00000);
+}
+
+// ------------------------------------------------------------------------------------------------ attention
+// tensor memory columns
+constexpr uint32_t TM_S = 0;          // 2 x 128: scores of a page, rows x tokens
+constexpr uint32_t TM_O = 256;        // 128: O^T, dims x rows
+constexpr uint32_t TM_SFA = 384;      // 4 per (term, K step): scales of the query
+constexpr uint32_t TM_SFB = 448;      // 2 x 16: scales of the page
+constexpr uint32_t TM_COLS = 512;
+
+template <int WP, bool VQ>
+struct Cfg {
+    static constexpr int RB = WP / 2, KB = WP / 64, PAGE = page_bytes(WP), CODES = PKV_PAGE_TOKENS * RB;
+    static constexpr int NK = WP == 256 ? 2 : 4;                                  // latent pages in flight
+    static constexpr int NV = VQ ? (WP == 256 ? 3 : 4) : (WP == 256 ? 5 : 7);     // V operand stages (64 tokens of a kv head, bf16)
+    static constexpr int NR = VQ ? (WP == 256 ? 6 : 8) : 0;                       // raw stages of quantised V
+    static constexpr int V_BYTES = HALF * DH * 2, RAW_BYTES = HALF * DH / 2, P_BYTES = ROWS * PKV_PAGE_TOKENS * 2;
+    static constexpr int SC_BYTES = MAX_G * PKV_PAGE_TOKENS * 2;                  // token scales of a page
+    static constexpr int Q_OFF = 0;
+    static constexpr int K_OFF = (blob_bytes(WP) + 1023) / 1024 * 1024;
+    static constexpr int V_OFF = K_OFF + NK * PAGE;
+    static constexpr int P_OFF = V_OFF + NV * V_BYTES;
+    static constexpr int R_OFF = P_OFF + P_BYTES;
+    static constexpr int SC_OFF = R_OFF + NR * RAW_BYTES;
+    static constexpr int X_OFF = SC_OFF + (VQ ? 2 * SC_BYTES : 0);
+    static constexpr int SMEM = X_OFF + 2048;
+    static constexpr int NTHREADS = VQ ? 384 : 256;
+    static constexpr uint64_t SWZ = RB == 128 ? SWZ_128B : SWZ_64B;
+    static_assert(SMEM <= 232448 && V_OFF % 1024 == 0 && P_OFF % 1024 == 0, "shared memory of a CTA");
+};
+
+struct Shared {                       // at X_OFF
+    uint64_t q_full, q_empty, p_full, pv_done, o_empty;
+    uint64_t k_full[4], k_empty[4], v_full[7], v_empty[7], v_clean[7], s_full[2], s_empty[2];
+    uint64_t r_full[8], r_empty[8], sc_full[2], sc_empty[2];
+    uint32_t tmem_base;
+    volatile int abort_flag;
+    Walk start;
+    float row_f[ROWS];                // rescale factors, then 1 / sum
+    uint32_t bad[MAX_G][2];           // drafted tokens whose value row of a kv head is not finite
+    long scan[12];
+};
+static_assert(sizeof(Shared) <= 2048, "behind the stages");
+
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
+    for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 1023u) == 1023u && X->abort_flag) return false;
+    }
+    X->abort_flag = 1;
+    if (status) { atomicExch(&status[0], 1); atomicExch(&status[1], where); }
+    return false;
+}
+
+// the 128 softmax threads meet (named barrier 1) and learn whether the predicate held in any of them
+__device__ __forceinline__ bool softmax_any(bool pred) {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(pred ? 1 : 0) : "memory");
+    return r != 0;
+}
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2_fast(float x) {     // 2 ulp, results below 2^-126 become 0: a weight needs no more
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+struct AttnArgs {
+    Batch B;
+    Tiles X;
+    const int32_t* page_table;
     const int64_t* mask;
+    const uint8_t* blobs;
+    const uint8_t* vq;
+    int n_pages, n_kv, n_q;
+    float col_scale;                  // tensor scale of the latent x log2(e) / sqrt(d)
+    float* part_o;                    // [2 per CTA][128 rows][128 dims]
+    float2* part_ml;                  // [2 per CTA][128 rows]
     __nv_bfloat16* out;
     int32_t* status;
 };
 
-__global__ void __launch_bounds__(NT) pkv_tree_attn_kernel(const Args A) {
-    __shared__ float qa[RC][PKV_MAX_WIDTH];
-    __shared__ float qs[RC][DH];
-    __shared__ float2 ph[DH / 2];
-    __shared__ float ps[RC][NT];
-    __shared__ float red[RC][4];
-    const pkv_layer_t& L = A.L;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.y;
-    const int rep = L.n_q / L.n_kv, r0 = blockIdx.z * RC, nr = min(RC, rep - r0), W = A.C.W;
+template <int WP, bool VQ>
+__global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel(const __grid_constant__ CUtensorMap kmap,
+                                                                                 const __grid_constant__ CUtensorMap qmap,
+                                                                                 const __grid_constant__ CUtensorMap vmap, const AttnArgs A) {
+    using C = Cfg<WP, VQ>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    Shared* X = reinterpret_cast<Shared*>(smem + C::X_OFF);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const Tiles& tl = A.X;
+    const int gang = blockIdx.x / tl.gang, zi = blockIdx.x % tl.gang;
     pkv_grid_launch_dependents();
-    pkv_grid_wait();
-    const int i = blockIdx.x;
-    int b = 0;
-    while (b < A.pg.batch && A.cu[b + 1] <= i) ++b;
-    if (b == A.pg.batch) return;
-    const int lo = A.cu[b], n = A.cu[b + 1] - lo, T = A.pg.seqlens_dev[b], base = T - n, row = i - lo;
-    if (lo < 0 || row < 0 || A.cu[b + 1] > A.n_tokens || n > A.max_draft || base < 0 || T > A.pg.max_pages * PKV_PAGE_TOKENS) {
-        if (A.status && tid == 0) { atomicExch(&A.status[0], 4); atomicExch(&A.status[1], b); }
-        return;
+
+    // ---- barriers, tensor memory, and where on the list of pages this CTA starts. Page table, lengths, masks and pages are
+    // final: the operand launch in front of this one has started, so everything before that is done.
+    if (tid == 0) {
+        mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 129); mbar_init(&X->p_full, 128); mbar_init(&X->pv_done, 1);
+        mbar_init(&X->o_empty, 128);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&X->s_full[i], 1); mbar_init(&X->s_empty[i], 128);
+            mbar_init(&X->sc_full[i], 1); mbar_init(&X->sc_empty[i], 128);
+        }
+        for (int i = 0; i < C::NK; ++i) { mbar_init(&X->k_full[i], 1); mbar_init(&X->k_empty[i], 1); }
+        for (int i = 0; i < C::NV; ++i) { mbar_init(&X->v_full[i], VQ ? 128 : 1); mbar_init(&X->v_empty[i], 1); mbar_init(&X->v_clean[i], 128); }
+        for (int i = 0; i < C::NR; ++i) { mbar_init(&X->r_full[i], 1); mbar_init(&X->r_empty[i], 128); }
+        X->abort_flag = 0;
+        X->start = Walk{0, 0, 0, 0};
+        fence_barrier_init();
     }
-    const unsigned long long word = A.mask ? (unsigned long long)A.mask[i] : (row >= 63 ? ~0ull : (2ull << row) - 1);
-    for (int k = tid; k < nr * DH; k += NT) {
-        const size_t o = ((size_t)i * L.n_q + g * rep + r0 + k / DH) * DH + k % DH;
-        qs[k / DH][k % DH] = A.q_bf16 ? __bfloat162float(((const __nv_bfloat16*)A.q)[o]) : ((const float*)A.q)[o];
-    }
-    for (int j = tid; j < DH / 2; j += NT) {
-        double sn, cs;
-        sincos((double)A.positions[i] * L.inv_freq_dev[j], &sn, &cs);
-        ph[j] = make_float2((float)(L.attn_scale * cs), (float)(L.attn_scale * sn));
+    if (tid < MAX_G * 2) X->bad[tid >> 1][tid & 1] = 0u;
+    if (warp == 3) tmem_alloc(&X->tmem_base, TM_COLS);
+    tc_fence_before_sync();
+    {
+        const int per = (A.B.batch + C::NTHREADS - 1) / C::NTHREADS, b_lo = min(tid * per, A.B.batch), b_hi = min(b_lo + per, A.B.batch);
+        long mine = 0;
+        int lo, n, T;
+        for (int b = b_lo; b < b_hi; ++b) mine += A.B.pages(b, lo, n, T);
+        long incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long y = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += y;
+        }
+        if (lane == 31) X->scan[warp] = incl;
+        __syncthreads();
+        long before = incl - mine, U = 0;
+        for (int w = 0; w < C::NTHREADS / 32; ++w) {
+            if (w < warp) before += X->scan[w];
+            U += X->scan[w];
+        }
+        U *= tl.passes;
+        const int gangs = (int)min((long)tl.gangs, U);
+        if (gang < gangs) {
+            const long u0 = gang_start(U, gangs, gang), u1 = gang_start(U, gangs, gang + 1);
+            if (mine > 0 && before * tl.passes <= u0 && u0 < (before + mine) * tl.passes) {
+                long u = u0 - before * tl.passes;
+                for (int b = b_lo; b < b_hi; ++b) {
+                    const int pages = A.B.pages(b, lo, n, T);
+                    if (u < (long)pages * tl.passes) {
+                        X->start = Walk{b, (int)(u / pages), (int)(u % pages), (int)(u1 - u0)};
+                        break;
+                    }
+                    u -= (long)pages * tl.passes;
+                }
+            }
+        }
     }
     __syncthreads();
-    for (int k = tid; k < nr * W; k += NT) {
-        const int r = k / W, c = k % W;
-        float v = 0.0f;
-        if (c < 2 * L.R) {
-            const int d = c < L.R ? c : c - L.R, f = L.freq_dev[d];
-            const float zr = qs[r][f] * ph[f].x - qs[r][f + DH / 2] * ph[f].y, zi = qs[r][f] * ph[f].y + qs[r][f + DH / 2] * ph[f].x;
-            const float ar = L.A_re_dev[g * L.R + d], ai = L.A_im_dev[g * L.R + d];
-            v = c < L.R ? ar * zr + ai * zi : ar * zi - ai * zr;
-        } else {
-            for (int s = 0; s < 2 * L.n_slow; ++s)
-                v = fmaf(qs[r][s < L.n_slow ? L.slow_dev[s] : L.slow_dev[s - L.n_slow] + DH / 2],
-                         L.A_s_dev[((size_t)g * 2 * L.n_slow + s) * L.R_s + c - 2 * L.R], v);
-        }
-        qa[r][c] = v * (PKV_LOG2E * rsqrtf((float)DH)) * (L.second_blocks_dev ? L.second_blocks_dev[c >> 4] : L.second);
-    }
-    float m[RC], l[RC], acc[RC];
-    for (int r = 0; r < RC; ++r) { m[r] = -INFINITY; l[r] = acc[r] = 0.0f; }
-    const int RB = pkv_row_bytes(W), pb = pkv_page_bytes(W);
-    for (int p = 0; p * PKV_PAGE_TOKENS < T; ++p) {
-        const int page = A.pg.page_table_dev[(size_t)b * A.pg.max_pages + p];
-        if (page < 0 || page >= A.C.n_pages) {
-            if (A.status && tid == 0) { atomicExch(&A.status[0], 2); atomicExch(&A.status[1], p); }
-            return;
-        }
-        const int t = p * PKV_PAGE_TOKENS + tid;
-        const bool see = t < base || (t < T && (word >> (t - base) & 1));
-        float s[RC] = {};
-        const uint8_t* pg = A.C.latent_dev + (size_t)page * pb;
-        __syncthreads();
-        for (int j = 0; j < W / 16; ++j) {
-            const uint2 w = *reinterpret_cast<const uint2*>(pg + pkv_code_offset(tid, j * 8, RB));
-            const float sc = pkv_e4m3_to_float(pg[PKV_PAGE_TOKENS * RB + pkv_scale_offset(tid, j)]);
-            for (int e = 0; e < 16; ++e) {
-                const float c = pkv_e2m1_value(((e < 8 ? w.x : w.y) >> (4 * (e & 7))) & 15u) * sc;
-#pragma unroll
-                for (int r = 0; r < RC; ++r) s[r] = fmaf(qa[r < nr ? r : 0][j * 16 + e], c, s[r]);
+    tc_fence_after_sync();
+    const uint32_t tb = X->tmem_base, sbase = smem_u32(smem);
+    Walk walk = X->start;
+    Part s;
+    auto heads = [&](const Part& p) { return min(tl.G, A.n_kv - p.z % tl.groups * tl.G); };      // kv heads of the tile
+
+    if (warp == 0) {
+        // ================================================================== latent pages and query operand
+        if (lane == 0) {
+            tma_prefetch_desc(&kmap); tma_prefetch_desc(&qmap);
+            int k = 0, seg = 0;
+            bool ok = true, waited = false;
+            while (ok && walk.next(A.B, tl, zi, s)) {
+                for (int p = s.p_lo; p < s.p_hi && ok; ++p, ++k) {
+                    const int st = k % C::NK, page = A.page_table[(size_t)s.b * A.B.max_pages + p];
+                    if (page < 0 || page >= A.n_pages) {               // never dereferenced
+                        X->abort_flag = 1;
+                        if (A.status) { atomicExch(&A.status[0], 2); atomicExch(&A.status[1], p); }
+                        ok = false;
+                        break;
+                    }
+                    if (k >= C::NK) ok = wait_or_abort(&X->k_empty[st], (k / C::NK - 1) & 1, X, A.status, 10);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&X->k_full[st], C::PAGE);
+                    tma_load_2d(smem + C::K_OFF + st * C::PAGE, &kmap, 0, page * (C::PAGE / 128), &X->k_full[st]);
+                    if (p == s.p_lo) {                                  // the tile's operand, behind its first page
+                        if (seg > 0) ok = wait_or_abort(&X->q_empty, (seg - 1) & 1, X, A.status, 11);
+                        if (!ok) { ++k; break; }
+                        if (!waited) { pkv_grid_wait(); waited = true; }
+                        asm volatile("fence.proxy.async;" ::: "memory");   // written by ordinary stores, read by the copy engine
+                        const long blob = (long)s.b * tl.Z + s.z;
+                        mbar_arrive_expect_tx(&X->q_full, blob_bytes(WP));
+                        for (int t = 0; t < PKV_QUERY_TERMS; ++t)
+                            tma_load_2d(smem + C::Q_OFF + t * C::PAGE, &qmap, 0, (int)(blob * (blob_bytes(WP) / 128) + t * (C::PAGE / 128)), &X->q_full);
+                        bulk_g2s(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE, A.blobs + blob * blob_bytes(WP) + PKV_QUERY_TERMS * C::PAGE, ROWS * 4, &X->q_full);
+                        ++seg;
+                    }
+                }
+            }
+            if (!waited) pkv_grid_wait();
+            if (X->abort_flag) {                                        // copies in flight land before anyone leaves
+                if (seg > 0) mbar_wait(&X->q_full, (seg - 1) & 1, 1u << 16);
+                for (int j = max(0, k - C::NK); j < k; ++j) mbar_wait(&X->k_full[j % C::NK], (j / C::NK) & 1, 1u << 16);
             }
         }
-#pragma unroll
-        for (int r = 0; r < RC; ++r) {
-            float x = see ? s[r] : -INFINITY;
-            s[r] = x;
-            for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(~0u, x, o));
-            if (lane == 0) red[r][warp] = x;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < RC; ++r) {
-            const float mn = fmaxf(m[r], fmaxf(fmaxf(red[r][0], red[r][1]), fmaxf(red[r][2], red[r][3])));
-            const float f = m[r] > -INFINITY ? exp2f(m[r] - mn) : 1.0f;
-            m[r] = mn; l[r] *= f; acc[r] *= f;
-            ps[r][tid] = see ? exp2f(s[r] - mn) : 0.0f;
-        }
-        __syncthreads();
-        const uint8_t* vq = (const uint8_t*)A.C.vq_dev + (size_t)page * L.n_kv * PKV_VQ_TILE_BYTES;
-        const __nv_bfloat16* v = (const __nv_bfloat16*)A.C.v_dev + ((size_t)page * L.n_kv + g) * PKV_PAGE_TOKENS * DH;
-        for (int k = 0; k < PKV_PAGE_TOKENS && p * PKV_PAGE_TOKENS + k < T; ++k) {
-            const int tt = p * PKV_PAGE_TOKENS + k;
-            if (tt >= base && !(word >> (tt - base) & 1)) continue;              // a masked row's values are never read
-            float x;
-            if (A.C.v_bits) {
-                const uint8_t byte = vq[g * 8192 + k * 64 + ((((tid >> 1) >> 4) ^ ((k >> 1) & 3)) << 4) + ((tid >> 1) & 15)];
-                x = pkv_e2m1_value(tid & 1 ? byte >> 4 : byte & 15u) *
-                    __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(vq + L.n_kv * 8192 + g * 256 + k * 2));
-            } else {
-                x = __bfloat162float(v[k * DH + tid]);
+    } else if (warp == 1) {
+        // ================================================================== values
+        if (lane == 0) {
+            tma_prefetch_desc(&vmap);
+            int k = 0, pg = 0;
+            bool ok = true;
+            while (ok && walk.next(A.B, tl, zi, s)) {
+                const int g0 = s.z % tl.groups * tl.G, ng = heads(s);
+                for (int p = s.p_lo; p < s.p_hi && ok; ++p, ++pg) {
+                    const int page = A.page_table[(size_t)s.b * A.B.max_pages + p];
+                    if (page < 0 || page >= A.n_pages) { ok = false; break; }      // (reported by warp 0)
+                    if constexpr (VQ) {                                 // the token scales of the page's kv heads
+                        if (pg >= 2) ok = wait_or_abort(&X->sc_empty[pg & 1], ((pg >> 1) - 1) & 1, X, A.status, 22);
+                        if (!ok) break;
+                        mbar_arrive_expect_tx(&X->sc_full[pg & 1], ng * PKV_PAGE_TOKENS * 2);
+                        bulk_g2s(smem + C::SC_OFF + (pg & 1) * C::SC_BYTES,
+                                 A.vq + (size_t)page * A.n_kv * PKV_VQ_TILE_BYTES + (size_t)A.n_kv * 8192 + g0 * 256, ng * PKV_PAGE_TOKENS * 2, &X->sc_full[pg & 1]);
+                    }
+                    for (int j = 0; j < 2 * ng && ok; ++j, ++k) {
+                        if constexpr (VQ) {
+                            const int st = k % (C::NR ? C::NR : 1);
+                            if (k >= C::NR) ok = wait_or_abort(&X->r_empty[st], (k / C::NR - 1) & 1, X, A.status, 21);
+                            if (!ok) break;
+                            mbar_arrive_expect_tx(&X->r_full[st], C::RAW_BYTES);
+                            tma_load_2d(smem + C::R_OFF + st * C::RAW_BYTES, &vmap, 0, page * A.n_kv * (PKV_VQ_TILE_BYTES / 128) + (g0 + (j >> 1)) * 64 + (j & 1) * 32,
+                                        &X->r_full[st]);
+                        } else {
+                            const int st = k % C::NV, y = (page * A.n_kv + g0 + (j >> 1)) * PKV_PAGE_TOKENS + (j & 1) * HALF;
+                            if (k >= C::NV) ok = wait_or_abort(&X->v_empty[st], (k / C::NV - 1) & 1, X, A.status, 20);
+                            if (!ok) break;
+                            uint8_t* dst = smem + C::V_OFF + st * C::V_BYTES;
+                            mbar_arrive_expect_tx(&X->v_full[st], C::V_BYTES);
+                            tma_load_2d(dst, &vmap, 0, y, &X->v_full[st]);
+                            tma_load_2d(dst + C::V_BYTES / 2, &vmap, 64, y, &X->v_full[st]);
+                        }
+                    }
+                }
             }
+            if (X->abort_flag) {
+                if constexpr (VQ) {
+                    for (int j = max(0, k - C::NR); j < k; ++j) mbar_wait(&X->r_full[j % (C::NR ? C::NR : 1)], (j / (C::NR ? C::NR : 1)) & 1, 1u << 16);
+                    for (int j = max(0, pg - 1); j <= pg; ++j) mbar_wait(&X->sc_full[j & 1], (j >> 1) & 1, 1u << 10);
+                } else {
+                    for (int j = max(0, k - C::NV); j < k; ++j) mbar_wait(&X->v_full[j % C::NV], (j / C::NV) & 1, 1u << 16);
+                }
+            }
+        }
+    } else if (warp == 2) {
+        // ================================================================== MMAs, all from one thread
+        if (lane == 0) {
+            constexpr uint32_t idesc_s = idesc_nvfp4(ROWS, PKV_PAGE_TOKENS);
+            const uint32_t idesc_o = idesc_bf16(DH, tl.rph, true, false);
+            const uint64_t q_desc = smem_desc(sbase + C::Q_OFF, 0, 8 * C::RB, C::SWZ);
+            const uint64_t p_desc = smem_desc(sbase + C::P_OFF, 0, 1024, SWZ_128B);
+            int k = 0, kv = 0, seg = 0;
+            uint32_t cleaned = 0;                      // phase bit of every stage's v_clean
+            bool ok = true;
+            while (ok && walk.next(A.B, tl, zi, s)) {
+                const int ng = heads(s), base = s.T - s.n;
+                ok = wait_or_abort(&X->q_full, seg & 1, X, A.status, 30);
+                if (!ok) break;
+                tc_fence_after_sync();
+                for (int t = 0; t < PKV_QUERY_TERMS; ++t)
+                    for (int c = 0; c < C::KB; ++c)
+                        tmem_cp_32x128b_warpx4(tb + TM_SFA + (t * C::KB + c) * 4, smem_desc(sbase + C::Q_OFF + t * C::PAGE + C::CODES + c * 512, 0, 128, SWZ_NONE));
+                // O^T += V^T P^T of page p (the page before the one whose scores were just issued)
+                auto values = [&](int p, int kk) -> bool {
+                    if (!wait_or_abort(&X->p_full, kk & 1, X, A.status, 31)) return false;
+                    if (p == s.p_lo && seg > 0 && !wait_or_abort(&X->o_empty, (seg - 1) & 1, X, A.status, 35)) return false;
+                    tc_fence_after_sync();
+                    const bool tail = !VQ && base < (p + 1) * PKV_PAGE_TOKENS;     // rows that are no cached tokens: looked over first
+                    for (int g = 0; g < ng; ++g) {
+                        for (int h = 0; h < 2; ++h, ++kv) {
+                            const int st = kv % C::NV;
+                            if (!wait_or_abort(&X->v_full[st], (kv / C::NV) & 1, X, A.status, 32)) return false;
+                            if (tail) {
+                                if (!wait_or_abort(&X->v_clean[st], cleaned >> st & 1, X, A.status, 36)) return false;
+                                cleaned ^= 1u << st;
+                            }
+                            tc_fence_after_sync();
+                            const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
+                            const uint64_t pg_desc = p_desc + (uint64_t)((h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
 #pragma unroll
-            for (int r = 0; r < RC; ++r) { acc[r] = fmaf(ps[r][k], x, acc[r]); l[r] += ps[r][k]; }
+                            for (int c = 0; c < HALF / 16; ++c)
+                                mma_bf16(tb + TM_O + g * tl.rph, v_desc + (uint64_t)(c * 16 * 128 / 16), pg_desc + (uint64_t)(c * 32 / 16), idesc_o,
+                                         !(p == s.p_lo && h == 0 && c == 0));
+                            tc_commit(&X->v_empty[st]);
+                        }
+                    }
+                    tc_commit(&X->pv_done);
+                    return true;
+                };
+                for (int p = s.p_lo; p < s.p_hi && ok; ++p, ++k) {
+                    const int st = k % C::NK, sb = k & 1;
+                    ok = wait_or_abort(&X->k_full[st], (k / C::NK) & 1, X, A.status, 33);
+                    if (ok && k >= 2) ok = wait_or_abort(&X->s_empty[sb], ((k >> 1) - 1) & 1, X, A.status, 34);
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint32_t ka = sbase + C::K_OFF + st * C::PAGE, sfb = tb + TM_SFB + 16 * sb;
+                    const uint64_t k_desc = smem_desc(ka, 0, 8 * C::RB, C::SWZ), sf_desc = smem_desc(ka + C::CODES, 0, 128, SWZ_NONE);
+#pragma unroll
+                    for (int c = 0; c < C::KB; ++c) tmem_cp_32x128b_warpx4(sfb + 4 * c, sf_desc + (uint64_t)(c * 512 / 16));
+#pragma unroll
+                    for (int t = 0; t < PKV_QUERY_TERMS; ++t)
+#pragma unroll
+                        for (int c = 0; c < C::KB; ++c)
+                            mma_nvfp4(tb + TM_S + 128 * sb, q_desc + (uint64_t)((t * C::PAGE + c * 32) / 16), k_desc + (uint64_t)(c * 32 / 16), idesc_s,
+                                      tb + TM_SFA + (t * C::KB + c) * 4, sfb + 4 * c, t != 0 || c != 0);
+                    tc_commit(&X->k_empty[st]);
+                    tc_commit(&X->s_full[sb]);
+                    if (p + 1 == s.p_hi) tc_commit(&X->q_empty);
+                    if (p > s.p_lo) ok = values(p - 1, k - 1);
+                }
+                if (ok) ok = values(s.p_hi - 1, k - 1);
+                ++seg;
+            }
+        }
+    } else if (VQ && warp >= 8) {
+        // ================================================================== quantised values -> bf16 operand tiles
+        // Every E2M1 level is a bf16 number; the token's scale goes into the softmax weight. 128 threads, two per token.
+        const int r = (tid - 256) >> 1, part = tid & 1;
+        auto prmt = [](uint32_t a, uint32_t b, uint32_t c) -> uint32_t {
+            uint32_t d;
+            asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+            return d;
+        };
+        // bf16 of 0 .5 1 1.5 2 3 4 6: high bytes 00 3F 3F 3F 40 40 40 40, low bytes 00 00 80 C0 00 40 80 C0
+        constexpr uint32_t HI_A = 0x3F3F3F00u, HI_B = 0x40404040u, LO_A = 0xC0800000u, LO_B = 0xC0804000u;
+        int k = 0;
+        bool ok = true;
+        while (ok && walk.next(A.B, tl, zi, s)) {
+            const int tiles = 2 * heads(s) * (s.p_hi - s.p_lo);
+            for (int j = 0; j < tiles && ok; ++j, ++k) {
+                const int rs = k % (C::NR ? C::NR : 1), st = k % C::NV;
+                ok = wait_or_abort(&X->r_full[rs], (k / (C::NR ? C::NR : 1)) & 1, X, A.status, 50);
+                if (ok && k >= C::NV) ok = wait_or_abort(&X->v_empty[st], (k / C::NV - 1) & 1, X, A.status, 51);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint8_t* raw = smem + C::R_OFF + rs * C::RAW_BYTES + r * 64;
+                uint8_t* row = smem + C::V_OFF + st * C::V_BYTES + part * (C::V_BYTES / 2) + r * 128;      // 64 dims of the token
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {                           // 32 codes -> 64 bytes
+                    const uint4 w4 = *reinterpret_cast<const uint4*>(raw + (((part * 2 + c) ^ ((r >> 1) & 3)) << 4));
+                    const uint32_t wv[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const uint32_t w = wv[u], mag = w & 0x77777777u, up = w << 4;
+                        const uint32_t h0 = prmt(HI_A, HI_B, mag) | (prmt(up, w, 0x5140u) & 0x80808080u);
+                        const uint32_t h1 = prmt(HI_A, HI_B, mag >> 16) | (prmt(up, w, 0x7362u) & 0x80808080u);
+                        const uint32_t l0 = prmt(LO_A, LO_B, mag), l1 = prmt(LO_A, LO_B, mag >> 16);
+                        const uint4 o = make_uint4(prmt(l0, h0, 0x5140u), prmt(l0, h0, 0x7362u), prmt(l1, h1, 0x5140u), prmt(l1, h1, 0x7362u));
+                        *reinterpret_cast<uint4*>(row + (((c * 4 + u) ^ (r & 7)) << 4)) = o;
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&X->v_full[st]);
+                mbar_arrive(&X->r_empty[rs]);
+            }
+        }
+    } else if (warp >= 4) {
+        // ================================================================== softmax: a row per thread
+        const int quad = warp & 3, r = quad * 32 + lane;
+        const uint32_t tl_s = tb + ((uint32_t)(quad * 32) << 16);
+        const float* row_scale = reinterpret_cast<const float*>(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE);
+        uint8_t* p_row = smem + C::P_OFF + r * 128;
+        int k = 0, kv = 0, seg = 0;
+        bool ok = true;                              // false once any wait of this warp gave up; the loops end for all four together
+        auto wait_all = [&](uint64_t* bar, uint32_t parity, int where) {
+            ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
+        };
+        bool go = true;
+        while (go && walk.next(A.B, tl, zi, s)) {
+            const int ng = heads(s), base = s.T - s.n, first = s.z / tl.groups * tl.qpb, nq = min(tl.qpb, s.n - first);
+            const int gl = r / tl.rph, rr = r % tl.rph;
+            const bool mine = gl < ng && rr < nq * tl.rep;              // a drafted token's row
+            unsigned long long word = 0;
+            if (mine) {
+                const int i = first + rr / tl.rep;
+                word = A.mask ? (unsigned long long)A.mask[s.lo + i] : (i >= 63 ? ~0ull : (2ull << i) - 1);
+                if (s.n < 64) word &= (1ull << s.n) - 1;
+            }
+            wait_all(&X->q_full, seg & 1, 40);
+            float cs = ok ? row_scale[r] * A.col_scale : 0.0f;
+            if (cs < 1e-37f) cs = 1e-37f;                               // (keeps NaN; a masked score -inf x cs stays -inf)
+            mbar_arrive(&X->q_empty);
+            float m = -INFINITY, l = 0.0f;
+            for (int p = s.p_lo; p < s.p_hi; ++p, ++k, kv += 2 * ng) {
+                const int sb = k & 1, drafts = base - p * PKV_PAGE_TOKENS;
+                wait_all(&X->s_full[sb], (k >> 1) & 1, 41);
+                float x[128];
+                if (ok) {
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(tl_s + TM_S + 128 * sb + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
+                    tmem_ld_wait();
+                    tc_fence_before_sync();
+                    mbar_arrive(&X->s_empty[sb]);
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) x[c] = 0.0f;
+                }
+                if (drafts < PKV_PAGE_TOKENS || !mine) {                // tokens the row does not see
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int j0 = 32 * c - drafts;                 // drafted token of the chunk's first column (negative: cached)
+                        uint32_t see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
+                        if (!mine) see = 0u;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (!(see >> e & 1)) x[32 * c + e] = -INFINITY;
+                    }
+                }
+                float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+                for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cs;
+                const bool need = top > m + RESCALE_THRESHOLD;
+                // the reference maximum of a row only moves when a page exceeds it by 2^8: then its column of O^T is rescaled
+                if (softmax_any(need || !ok)) {
+                    float f = 1.0f;
+                    if (need) {
+                        if (m > -INFINITY) { f = exp2f(m - top); l *= f; }
+                        m = top;
+                    }
+                    X->row_f[r] = f;
+                    if (p > s.p_lo) wait_all(&X->pv_done, (k - 1) & 1, 42);        // the accumulators are at rest
+                    if (softmax_any(!ok)) { go = false; break; }                   // (the same answer in all four warps)
+                    if (p > s.p_lo) {
+                        tc_fence_after_sync();
+                        for (int c0 = 0; c0 < ng * tl.rph; c0 += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(tl_s + TM_O + c0, o);
+                            tmem_ld_wait();
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * X->row_f[c0 + c]);
+                            tmem_st16(tl_s + TM_O + c0, o);
+                        }
+                        tmem_st_wait();
+                        tc_fence_before_sync();
+                    }
+                    softmax_sync();                                     // row_f has been read
+                }
+                const float mu = m > -INFINITY ? m : 0.0f;              // nothing seen yet: every weight is 2^-inf
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t w[64];
+                if constexpr (VQ) {
+                    // the weight of a token carries its value scale of this row's kv head (a masked one's may be anything)
+                    wait_all(&X->sc_full[k & 1], (k >> 1) & 1, 46);
+                    const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + (k & 1) * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2);
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const uint4 q4 = sc[c];
+                        const uint32_t qs[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float p0 = ex2_fast(fmaf(x[8 * c + 2 * e], cs, -mu)), p1 = ex2_fast(fmaf(x[8 * c + 2 * e + 1], cs, -mu));
+                            sum[e] += p0 + p1;
+                            w[4 * c + e] = pack_bf16(p0 == 0.0f ? 0.0f : p0 * __uint_as_float(qs[e] << 16), p1 == 0.0f ? 0.0f : p1 * __uint_as_float(qs[e] & 0xffff0000u));
+                        }
+                    }
+                    mbar_arrive(&X->sc_empty[k & 1]);
+                } else {
+                    // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so that
+                    // numerator and denominator agree
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) {
+                        w[c] = pack_bf16(ex2_fast(fmaf(x[2 * c], cs, -mu)), ex2_fast(fmaf(x[2 * c + 1], cs, -mu)));
+                        sum[c & 3] += __uint_as_float(w[c] << 16) + __uint_as_float(w[c] & 0xffff0000u);
+                    }
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (k > 0) wait_all(&X->pv_done, (k - 1) & 1, 43);      // the weights of the page before have been read
+                // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, two blocks
+#pragma unroll
+                for (int c = 0; c < 16; ++c)
+                    *reinterpret_cast<uint4*>(p_row + (c >> 3) * (C::P_BYTES / 2) + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                fence_proxy_async_smem();
+                mbar_arrive(&X->p_full);
+                if constexpr (!VQ) {
+                    // Values behind the cached tokens: rows past the sequence become zero, and so does what is not finite in a
+                    // drafted row (0 x inf would reach rows that do not see it); who does see it gets NaN at the end.
+                    if (drafts < PKV_PAGE_TOKENS && ok) {
+                        // (Every tile of such a page is handed over, also one with cached rows only: the page before is known to be
+                        // consumed, and within this one the stages then advance in step with these waits.)
+                        for (int j = 0; j < 2 * ng; ++j) {
+                            const int h = j & 1, st = (kv + j) % C::NV;
+                            wait_all(&X->v_full[st], ((kv + j) / C::NV) & 1, 47);
+                            if (!ok) break;
+                            uint8_t* tile = smem + C::V_OFF + st * C::V_BYTES;
+#pragma unroll 4
+                            for (int it = 0; it < C::V_BYTES / 16 / 128 && drafts < (h + 1) * HALF; ++it) {
+                                const int id = it * 128 + r, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
+                                if (d < 0) continue;
+                                uint4* at = reinterpret_cast<uint4*>(tile) + id;
+                                if (d >= s.n) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
+                                uint4 v = *at;
+                                uint32_t* e = reinterpret_cast<uint32_t*>(&v);
+                                bool hit = false;
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    if ((e[q] & 0x7f80u) == 0x7f80u) { e[q] &= 0xffff0000u; hit = true; }
+                                    if ((e[q] & 0x7f800000u) == 0x7f800000u) { e[q] &= 0xffffu; hit = true; }
+                                }
+                                if (hit) { *at = v; atomicOr(&X->bad[j >> 1][d >> 5], 1u << (d & 31)); }
+                            }
+                            fence_proxy_async_smem();
+                            mbar_arrive(&X->v_clean[st]);
+                        }
+                    }
+                }
+            }
+            if (!go) break;
+            // ---- the tile's stretch is done: O^T out of tensor memory
+            wait_all(&X->pv_done, (k - 1) & 1, 44);
+            if (softmax_any(!ok)) { go = false; break; }
+            tc_fence_after_sync();
+            if (!VQ && mine && ((word & 0xffffffffu & X->bad[gl][0]) | ((word >> 32) & X->bad[gl][1]))) l = __int_as_float(0x7fc00000);
+            const bool whole = s.p_lo == 0 && s.p_hi == s.pages;
+            const size_t slot = (size_t)blockIdx.x * 2 + (s.p_lo == 0);
+            if (whole) X->row_f[r] = l == 0.0f ? 0.0f : 1.0f / l;       // a row that sees nothing: zeros
+            else if (mine) A.part_ml[slot * ROWS + r] = make_float2(m, l);
+            softmax_sync();
+            if (r < MAX_G * 2) X->bad[r >> 1][r & 1] = 0u;
+            for (int g = 0; g < ng; ++g) {
+                for (int c0 = 0; c0 < nq * tl.rep; c0 += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(tl_s + TM_O + g * tl.rph + c0, o);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int c = 0; c < 16; ++c) {
+                        const int q = c0 + c;                           // row of the kv head; this thread's dim is r
+                        if (q >= nq * tl.rep) break;
+                        if (whole) {
+                            const size_t row = (size_t)(s.lo + first + q / tl.rep) * A.n_q + (s.z % tl.groups * tl.G + g) * tl.rep + q % tl.rep;
+                            A.out[row * DH + r] = __float2bfloat16(__uint_as_float(o[c]) * X->row_f[g * tl.rph + q]);
+                        } else {
+                            A.part_o[(slot * ROWS + g * tl.rph + q) * DH + r] = __uint_as_float(o[c]);
+                        }
+                    }
+                }
+            }
+            tc_fence_before_sync();
+            mbar_arrive(&X->o_empty);
+            softmax_sync();                                             // row_f and bad are free again
+            ++seg;
         }
     }
-    for (int r = 0; r < nr; ++r)
-        A.out[((size_t)i * L.n_q + g * rep + r0 + r) * DH + tid] = __float2bfloat16(m[r] > -INFINITY || l[r] != 0.0f ? acc[r] / l[r] : 0.0f);
+    // ---- everyone meets, tensor memory goes back
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 3) tmem_dealloc(tb, TM_COLS);
+    if (X->abort_flag) {                             // a stretch that was not finished counts for nothing in the merge
+        for (int i = tid; i < 2 * ROWS; i += C::NTHREADS) A.part_ml[(size_t)blockIdx.x * 2 * ROWS + i] = make_float2(-INFINITY, 0.0f);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ merge
+// O = sum 2^(m - M) o / sum 2^(m - M) l over the stretches of a tile that several CTAs did. CTA: 8 / WPR rows of a tile,
+// WPR warps per row; a lane holds four dims.
+struct MergeArgs {
+    Batch B;
+    Tiles X;
+    int n_kv, n_q;
+    const float* part_o;
+    const float2* part_ml;
+    __nv_bfloat16* out;
+};
+
+template <int WPR>
+__global__ void __launch_bounds__(256) pkv_tree_merge_kernel(const MergeArgs A) {
+    __shared__ long sums[8][2];
+    __shared__ float4 acc_s[8][32];
+    __shared__ float2 ml_s[8];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, z = blockIdx.y, b = blockIdx.z;
+    const int r = blockIdx.x * (8 / WPR) + warp / WPR, w0 = warp % WPR;
+    pkv_grid_launch_dependents();
+    pkv_grid_wait();
+    int lo, n, T;
+    const int pages = A.B.pages(b, lo, n, T);
+    const Tiles& X = A.X;
+    const int first = z / X.groups * X.qpb, nq = min(X.qpb, n - first);
+    if (pages == 0 || nq <= 0) return;
+    long before = 0, total = 0;
+    for (int i = tid; i < A.B.batch; i += 256) {
+        int lo2, n2, T2;
+        const int p = A.B.pages(i, lo2, n2, T2);
+        total += p;
+        if (i < b) before += p;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+    }
+    if (lane == 0) { sums[warp][0] = before; sums[warp][1] = total; }
+    __syncthreads();
+    before = total = 0;
+    for (int w = 0; w < 8; ++w) { before += sums[w][0]; total += sums[w][1]; }
+    const long U = total * X.passes, u0 = before * X.passes + (long)(z / X.gang) * pages;
+    const int gangs = (int)min((long)X.gangs, U), x0 = gang_of(U, gangs, u0), x1 = gang_of(U, gangs, u0 + pages - 1);
+    if (x0 == x1) return;                            // one CTA did the whole tile and has written it
+    const int gl = r / X.rph, rr = r % X.rph, g = z % X.groups * X.G + gl;
+    const bool live = gl < X.G && g < A.n_kv && rr < nq * X.rep;
+    auto slot = [&](int x) { return ((size_t)(x * X.gang + z % X.gang) * 2 + (x == x0)) * ROWS + r; };
+    float M = -INFINITY, l = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (live) {
+        for (int x = x0 + lane; x <= x1; x += 32) M = fmaxf(M, A.part_ml[slot(x)].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+        constexpr int DEEP = 8;
+        for (int xb = x0 + w0; xb <= x1; xb += WPR * DEEP) {
+            float4 o[DEEP];
+            float2 ml[DEEP];
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) {
+                const int x = xb + k * WPR;
+                ml[k] = x <= x1 ? A.part_ml[slot(x)] : make_float2(-INFINITY, 0.0f);
+                o[k] = x <= x1 ? *reinterpret_cast<const float4*>(A.part_o + slot(x) * DH + lane * 4) : acc;
+            }
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) {
+                if (ml[k].x > -INFINITY) {
+                    const float f = exp2f(ml[k].x - M);
+                    l = fmaf(ml[k].y, f, l);
+                    acc.x = fmaf(o[k].x, f, acc.x); acc.y = fmaf(o[k].y, f, acc.y);
+                    acc.z = fmaf(o[k].z, f, acc.z); acc.w = fmaf(o[k].w, f, acc.w);
+                } else {
+                    l += ml[k].y;                    // 0, or NaN
+                }
+            }
+        }
+    }
+    if constexpr (WPR > 1) {
+        acc_s[warp][lane] = acc;
+        if (lane == 0) ml_s[warp] = make_float2(M, l);
+        __syncthreads();
+        if (w0 != 0) return;
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) {
+            const float4 o = acc_s[warp + w][lane];
+            acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
+            l += ml_s[warp + w].y;
+        }
+    }
+    if (!live) return;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const size_t row = (size_t)(lo + first + rr / X.rep) * A.n_q + g * X.rep + rr % X.rep;
+    *reinterpret_cast<uint2*>(A.out + row * DH + lane * 4) = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+}
+
+// ------------------------------------------------------------------------------------------------ host
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+
+int init_encoder() {
+    if (!g_encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult qres;
+        PKV_CUDA_TRY(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qres));
+        if (!fn || qres != cudaDriverEntryPointSuccess) return PKV_ERR_CUDA;
+        g_encode = (PFN_cuTensorMapEncodeTiled_v12000)fn;
+    }
+    return PKV_OK;
+}
+
+// rows of 128 bytes, or (bf16) of 128 values in two boxes of 64 with the 128-byte swizzle
+int encode_map(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_rows, bool bf16) {
+    cuuint64_t dims[2] = {128, rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(bf16 ? 256 : 128)};
+    cuuint32_t box[2] = {(cuuint32_t)(bf16 ? 64 : 128), box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = g_encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box,
+                          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { g_pkv_last_cuda_error = (int)r; return PKV_ERR_CUDA; }
+    return PKV_OK;
+}
+
+constexpr int N_SM = 148;                            // CTAs of the attention launch: one per SM of a B200
+
+// Rows of a kv head: rep query heads of up to qpb drafted tokens, in blocks of equal size when there are more than 128; padded
+// to the 16 columns an MMA takes. As many kv heads per tile as fit, evenly over the tiles.
+Tiles make_tiles(int n_q, int n_kv, int max_draft) {
+    Tiles X;
+    X.rep = n_q / n_kv;
+    const int most = ROWS / X.rep, blocks = (max_draft + most - 1) / most;
+    X.qpb = (max_draft + blocks - 1) / blocks;
+    X.rph = (X.rep * X.qpb + 15) / 16 * 16;
+    const int fit = ROWS / X.rph, groups = (n_kv + fit - 1) / fit;
+    X.G = (n_kv + groups - 1) / groups;
+    X.groups = (n_kv + X.G - 1) / X.G;
+    X.Z = X.groups * blocks;
+    // a gang of all tiles if that leaves few SMs idle, else of a half, a third, ...: up to 16 side by side
+    X.passes = (X.Z + 15) / 16;
+    X.gang = (X.Z + X.passes - 1) / X.passes;
+    X.gangs = N_SM / X.gang;
+    return X;
+}
+
+struct Layout { size_t blobs, part_o, part_ml, total; };
+
+Layout make_layout(const Tiles& X, int batch, int WP) {
+    Layout y;
+    const size_t ctas = (size_t)X.gangs * X.gang;
+    y.blobs = 0;
+    y.part_o = ((size_t)batch * X.Z * blob_bytes(WP) + 1023) / 1024 * 1024;
+    y.part_ml = y.part_o + ctas * 2 * ROWS * DH * 4;
+    y.total = y.part_ml + ctas * 2 * ROWS * 8;
+    return y;
+}
+
+template <int WP, bool VQ>
+int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, AttnArgs& at, const MergeArgs& mg, size_t blob_rows, cudaStream_t st) {
+    using C = Cfg<WP, VQ>;
+    const Tiles& X = ab.X;
+    CUtensorMap kmap, qmap, vmap;
+    int rc = encode_map(&kmap, cache->latent_dev, (uint64_t)cache->n_pages * (C::PAGE / 128), C::PAGE / 128, false);
+    if (!rc) rc = encode_map(&qmap, ab.blobs, blob_rows, C::PAGE / 128, false);
+    if (!rc) rc = VQ ? encode_map(&vmap, cache->vq_dev, (uint64_t)cache->n_pages * cache->n_kv * (PKV_VQ_TILE_BYTES / 128), C::RAW_BYTES / 128, false)
+                     : encode_map(&vmap, cache->v_dev, (uint64_t)cache->n_pages * cache->n_kv * PKV_PAGE_TOKENS, HALF, true);
+    if (rc) return rc;
+    static pkv_attr_flags attr;
+    PKV_CUDA_TRY(pkv_set_max_smem(pkv_tree_attn_kernel<WP, VQ>, C::SMEM, attr));
+    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_absorb_kernel<WP>, dim3(ROWS / AR, X.Z, ab.B.batch), dim3(AR * WP / 16), 0, st, ab));
+    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ>, dim3(X.gangs * X.gang), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
+    // parts of a tile: about one per CTA and tile; a warp takes some eight of them
+    const int parts = X.gangs / (ab.B.batch * X.passes) + 1;
+    const dim3 grid(ROWS / 8, X.Z, ab.B.batch), block(256);
+    if (parts <= 8) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1>, grid, block, 0, st, mg));
+    else if (parts <= 16) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<2>, dim3(ROWS / 4, X.Z, ab.B.batch), block, 0, st, mg));
+    else PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<8>, dim3(ROWS, X.Z, ab.B.batch), block, 0, st, mg));
+    return PKV_OK;
+}
+
+int check_shape(const pkv_layer_t* L, int32_t batch, int32_t max_draft, int32_t max_pages) {
+    int st = pkv_check_layer(L);
+    if (st) return st;
+    if (batch < 0 || max_draft <= 0 || max_pages <= 0) return PKV_ERR_INVALID;
+    if (L->head_dim != DH || max_draft > PKV_TREE_MAX || L->n_q / L->n_kv > 64 || batch > 4096 || max_pages > (1 << 23)) return PKV_ERR_UNSUPPORTED;
+    return PKV_OK;
 }
 
 }  // namespace
 
 extern "C" int64_t pkv_tree_workspace_bytes(const pkv_layer_t* layer, int32_t batch, int32_t max_draft, int32_t max_pages) {
-    if (!layer || batch < 0 || max_draft <= 0 || max_pages <= 0) return PKV_ERR_INVALID;
-    if (max_draft > PKV_TREE_MAX) return PKV_ERR_UNSUPPORTED;
-    return 0;
+    int st = check_shape(layer, batch, max_draft, max_pages);
+    if (st) return st;
+    return (int64_t)make_layout(make_tiles(layer->n_q, layer->n_kv, max_draft), batch, pkv_padded_width(2 * layer->R + layer->R_s)).total;
 }
 
 extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache, const pkv_pages_t* pages, const void* q_dev, int32_t q_dtype,
                              const int32_t* positions_dev, const int64_t* mask_dev, const int32_t* cu_dev, int32_t n_tokens,
                              int32_t max_draft, void* workspace_dev, int64_t workspace_bytes, void* out_dev, int32_t* status_dev,
                              void* stream) {
-    int st = pkv_check_layer(layer);
+    if (!pages || !pages->page_table_dev || !pages->seqlens_dev || n_tokens < 0) return PKV_ERR_INVALID;
+    int st = check_shape(layer, pages->batch, max_draft, pages->max_pages);
     if (st) return st;
     st = pkv_check_cache(cache);
     if (st) return st;
-    if (!pages || !pages->page_table_dev || !pages->seqlens_dev || pages->batch < 0 || pages->max_pages <= 0 || n_tokens < 0 || max_draft <= 0)
-        return PKV_ERR_INVALID;
     if (cache->W != 2 * layer->R + layer->R_s || cache->n_kv != layer->n_kv || cache->head_dim != layer->head_dim) return PKV_ERR_INVALID;
-    if (layer->head_dim != DH || max_draft > PKV_TREE_MAX || layer->n_q / layer->n_kv > 64 || pages->batch > 4096) return PKV_ERR_UNSUPPORTED;
-    if (!(cache->v_bits ? cache->vq_dev : cache->v_dev)) return PKV_ERR_INVALID;
+    const void* v = cache->v_bits ? cache->vq_dev : cache->v_dev;
+    if (!v || (((uintptr_t)v) & (cache->v_bits ? 127u : 15u))) return PKV_ERR_INVALID;
     if (q_dtype != PKV_F32 && q_dtype != PKV_BF16) return PKV_ERR_UNSUPPORTED;
     if (pages->batch == 0 || n_tokens == 0) return PKV_OK;
     if (!q_dev || !positions_dev || !cu_dev || !out_dev || (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15u)) return PKV_ERR_INVALID;
-    Args A{*layer, *cache, *pages, q_dev, q_dtype == PKV_BF16, n_tokens, max_draft, positions_dev, cu_dev, mask_dev, (__nv_bfloat16*)out_dev, status_dev};
-    const int rep = layer->n_q / layer->n_kv;
-    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel, dim3(n_tokens, layer->n_kv, (rep + RC - 1) / RC), dim3(NT), 0, (cudaStream_t)stream, A));
-    return PKV_OK;
+    const int WP = pkv_padded_width(cache->W);
+    // coordinates of the tensor maps are 31 bits
+    if ((int64_t)cache->n_pages * cache->n_kv * PKV_PAGE_TOKENS > 0x7fffffff || (int64_t)cache->n_pages * 144 > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
+    const Tiles X = make_tiles(layer->n_q, layer->n_kv, max_draft);
+    const Layout y = make_layout(X, pages->batch, WP);
+    const size_t blob_rows = (size_t)pages->batch * X.Z * (blob_bytes(WP) / 128);
+    if (blob_rows > 0x7fffffff || X.Z > 65535) return PKV_ERR_UNSUPPORTED;
+    if (!workspace_dev || (((uintptr_t)workspace_dev) & 1023u) || workspace_bytes < (int64_t)y.total) return PKV_ERR_INVALID;
+    st = init_encoder();
+    if (st) return st;
+    uint8_t* ws = (uint8_t*)workspace_dev;
+    const Batch B{cu_dev, pages->seqlens_dev, pages->batch, pages->max_pages, n_tokens, max_draft};
+    const AbsorbArgs ab{*layer, B, X, q_dev, q_dtype == PKV_BF16, positions_dev, ws, status_dev};
+    AttnArgs at;
+    at.B = B; at.X = X; at.page_table = pages->page_table_dev; at.mask = mask_dev; at.blobs = ws; at.vq = (const uint8_t*)cache->vq_dev;
+    at.n_pages = cache->n_pages; at.n_kv = layer->n_kv; at.n_q = layer->n_q;
+    at.col_scale = layer->second * PKV_LOG2E / sqrtf((float)DH);
+    at.part_o = (float*)(ws + y.part_o); at.part_ml = (float2*)(ws + y.part_ml);
+    at.out = (__nv_bfloat16*)out_dev; at.status = status_dev;
+    const MergeArgs mg{B, X, layer->n_kv, layer->n_q, at.part_o, at.part_ml, at.out};
+    cudaStream_t s = (cudaStream_t)stream;
+    if (cache->v_bits) return WP == 256 ? launch<256, true>(cache, ab, at, mg, blob_rows, s) : launch<128, true>(cache, ab, at, mg, blob_rows, s);
+    return WP == 256 ? launch<256, false>(cache, ab, at, mg, blob_rows, s) : launch<128, false>(cache, ab, at, mg, blob_rows, s);
 }
