@@ -30,6 +30,7 @@ using namespace pkv;
 
 constexpr int DH = 128, ROWS = 128;                  // head dim; rows of a tile
 constexpr int HALF = 64;                             // tokens per V stage: half a page of one kv head
+constexpr int SOFT = 256;                            // softmax threads: two per row, 64 tokens of a page each
 constexpr int MAX_G = 8;                             // kv heads of a tile (16 rows at least each)
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in base-2 logits
 constexpr uint32_t WAIT_LIMIT = 1u << 19;            // probes of a bounded wait
@@ -101,14 +102,16 @@ struct AbsorbArgs {
 
 constexpr int AR = 16;                               // rows per CTA
 
-// CTA (16 rows of a tile, tile, sequence); WP / 16 threads per row, each with one 16-column block in registers. Rows that
+// CTA (16 rows of a tile, tile, sequence). Rows that
 // no drafted token has are not written: a row of garbage only reaches its own column of the result, which nobody reads.
 template <int WP>
 __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const AbsorbArgs A) {
     constexpr int NB = WP / 16, NT = AR * NB, RB = WP / 2;
+    static_assert(NT == WP, "a thread per column");
     __shared__ float2 zq[AR][DH / 2];
     __shared__ float2 ph[AR][DH / 2];
     __shared__ float raw[AR][DH];
+    __shared__ __align__(16) float qa[AR][WP + 4];
     const pkv_layer_t& L = A.L;
     const int tid = threadIdx.x, z = blockIdx.y, b = blockIdx.z, r0 = blockIdx.x * AR;
     pkv_grid_wait();                                 // everything before this launch is done ..
@@ -125,9 +128,21 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     if (nq <= 0 || r0 / A.X.rph >= A.X.G || g >= L.n_kv || rows <= 0) return;
     // this CTA's rows belong to the drafted tokens q_lo .. q_hi
     const int q_lo = rr0 / rep, q_hi = (rr0 + rows - 1) / rep;
+    // the factors of this thread's column, used for all rows
+    const int R = L.R, W = 2 * R + L.R_s, c = tid;
+    int f = 0;
+    float ar = 0.0f, ai = 0.0f, tier = 1.0f;
+    if (c < 2 * R) {
+        const int k = c < R ? c : c - R;
+        f = L.freq_dev[k];
+        ar = L.A_re_dev[g * R + k];
+        ai = L.A_im_dev[g * R + k];
+    }
+    // tiers: the cache's block is in units of its own scale while the attention applies the layer's one
+    if (L.second_blocks_dev && c < W) tier = L.second_blocks_dev[c >> 4] / L.second;
     for (int k = tid; k < rows * (DH / 4); k += NT) {
-        const int r = k / (DH / 4), c = k % (DH / 4) * 4, rr = rr0 + r;
-        const size_t o = ((size_t)(lo + first + rr / rep) * L.n_q + g * rep + rr % rep) * DH + c;
+        const int r = k / (DH / 4), d = k % (DH / 4) * 4, rr = rr0 + r;
+        const size_t o = ((size_t)(lo + first + rr / rep) * L.n_q + g * rep + rr % rep) * DH + d;
         float4 v;
         if (A.q_bf16) {
             const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)A.q + o);
@@ -136,13 +151,16 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
         } else {
             v = *reinterpret_cast<const float4*>((const float*)A.q + o);
         }
-        *reinterpret_cast<float4*>(&raw[r][c]) = v;
+        *reinterpret_cast<float4*>(&raw[r][d]) = v;
     }
-    for (int k = tid; k < (q_hi - q_lo + 1) * (DH / 2); k += NT) {       // phasors: the angle in 64 bits
+    // Phasors: the angle as a number of turns in 64 bits, of which only the fraction counts; that is exact enough in 32 bits
+    // (2^-25 of a turn) and needs no long range reduction (the operand's own residual is 7e-5).
+    for (int k = tid; k < (q_hi - q_lo + 1) * (DH / 2); k += NT) {
         const int j = k % (DH / 2);
-        double sn, cs;
-        sincos((double)A.positions[lo + first + q_lo + k / (DH / 2)] * L.inv_freq_dev[j], &sn, &cs);
-        ph[k / (DH / 2)][j] = make_float2((float)((double)L.attn_scale * cs), (float)((double)L.attn_scale * sn));
+        const double turns = (double)A.positions[lo + first + q_lo + k / (DH / 2)] * L.inv_freq_dev[j] * 0.15915494309189533577;
+        float sn, cs;
+        sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
+        ph[k / (DH / 2)][j] = make_float2(L.attn_scale * cs, L.attn_scale * sn);
     }
     __syncthreads();
     for (int k = tid; k < rows * (DH / 2); k += NT) {
@@ -152,29 +170,31 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
         zq[r][j] = make_float2(x * p.x - y * p.y, x * p.y + y * p.x);
     }
     __syncthreads();
-    const int r = tid / NB, j = tid % NB, R = L.R, W = 2 * R + L.R_s;
-    const bool live = r < rows;
-    float res[16], am = 0.0f;
-    bool fine = true;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const int c = j * 16 + i;
+    // absorbed rows: a column per thread
+#pragma unroll 4
+    for (int r = 0; r < rows; ++r) {
         float v = 0.0f;
-        if (live && c < 2 * R) {                     // conj(A) zq
-            const int k = c < R ? c : c - R;
-            const float2 w = zq[r][L.freq_dev[k]];
-            const float ar = L.A_re_dev[g * R + k], ai = L.A_im_dev[g * R + k];
+        if (c < 2 * R) {                             // conj(A) zq
+            const float2 w = zq[r][f];
             v = c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x;
-        } else if (live && c < W) {                  // slow dims: the raw query
+        } else if (c < W) {                          // slow dims: the raw query
             for (int s = 0; s < 2 * L.n_slow; ++s)
                 v = fmaf(raw[r][s < L.n_slow ? L.slow_dev[s] : L.slow_dev[s - L.n_slow] + DH / 2],
                          L.A_s_dev[((size_t)g * 2 * L.n_slow + s) * L.R_s + c - 2 * R], v);
         }
-        // tiers: the cache's block is in units of its own scale while the attention applies the layer's one
-        if (L.second_blocks_dev && c < W) v *= L.second_blocks_dev[c >> 4] / L.second;
-        res[i] = v;
-        am = fmaxf(am, fabsf(v));
-        fine = fine && fabsf(v) < INFINITY;
+        qa[r][c] = v * tier;
+    }
+    __syncthreads();
+    const int r = tid / NB, j = tid % NB;            // from here on: a 16-column block of a row per thread
+    const bool live = r < rows;
+    float res[16], am = 0.0f;
+    bool fine = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(&res[4 * i]) = *reinterpret_cast<const float4*>(&qa[r][j * 16 + 4 * i]);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        am = fmaxf(am, fabsf(res[i]));
+        fine = fine && fabsf(res[i]) < INFINITY;
     }
 #pragma unroll
     for (int o = NB / 2; o; o >>= 1) {
@@ -210,7 +230,7 @@ struct Cfg {
     static constexpr int RB = WP / 2, KB = WP / 64, PAGE = page_bytes(WP), CODES = PKV_PAGE_TOKENS * RB;
     static constexpr int NK = WP == 256 ? 2 : 4;                                  // latent pages in flight
     static constexpr int NV = VQ ? (WP == 256 ? 3 : 4) : (WP == 256 ? 5 : 7);     // V operand stages (64 tokens of a kv head, bf16)
-    static constexpr int NR = VQ ? (WP == 256 ? 6 : 8) : 0;                       // raw stages of quantised V
+    static constexpr int NR = VQ ? (WP == 256 ? 5 : 8) : 0;                       // raw stages of quantised V
     static constexpr int V_BYTES = HALF * DH * 2, RAW_BYTES = HALF * DH / 2, P_BYTES = ROWS * PKV_PAGE_TOKENS * 2;
     static constexpr int SC_BYTES = MAX_G * PKV_PAGE_TOKENS * 2;                  // token scales of a page
     static constexpr int Q_OFF = 0;
@@ -220,8 +240,8 @@ struct Cfg {
     static constexpr int R_OFF = P_OFF + P_BYTES;
     static constexpr int SC_OFF = R_OFF + NR * RAW_BYTES;
     static constexpr int X_OFF = SC_OFF + (VQ ? 2 * SC_BYTES : 0);
-    static constexpr int SMEM = X_OFF + 2048;
-    static constexpr int NTHREADS = VQ ? 384 : 256;
+    static constexpr int SMEM = X_OFF + 3072;
+    static constexpr int NTHREADS = VQ ? 512 : 384;
     static constexpr uint64_t SWZ = RB == 128 ? SWZ_128B : SWZ_64B;
     static_assert(SMEM <= 232448 && V_OFF % 1024 == 0 && P_OFF % 1024 == 0, "shared memory of a CTA");
 };
@@ -235,9 +255,10 @@ struct Shared {                       // at X_OFF
     Walk start;
     float row_f[ROWS];                // rescale factors, then 1 / sum
     uint32_t bad[MAX_G][2];           // drafted tokens whose value row of a kv head is not finite
-    long scan[12];
+    float row_m[2][ROWS];             // maxima of the two halves of a row, then their sums
+    long scan[16];
 };
-static_assert(sizeof(Shared) <= 2048, "behind the stages");
+static_assert(sizeof(Shared) <= 3072, "behind the stages");
 
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
     for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
@@ -249,14 +270,20 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Sh
     return false;
 }
 
-// the 128 softmax threads meet (named barrier 1) and learn whether the predicate held in any of them
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// the softmax threads meet (named barrier 1) and learn whether the predicate held in any of them
 __device__ __forceinline__ bool softmax_any(bool pred) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
                  : "=r"(r) : "r"(pred ? 1 : 0) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ void softmax_sync() { static_assert(SOFT == 256, "barrier width"); asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2_fast(float x) {     // 2 ulp, results below 2^-126 become 0: a weight needs no more
     float y;
@@ -299,14 +326,14 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     // ---- barriers, tensor memory, and where on the list of pages this CTA starts. Page table, lengths, masks and pages are
     // final: the operand launch in front of this one has started, so everything before that is done.
     if (tid == 0) {
-        mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 129); mbar_init(&X->p_full, 128); mbar_init(&X->pv_done, 1);
-        mbar_init(&X->o_empty, 128);
+        mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, SOFT + 1); mbar_init(&X->p_full, SOFT); mbar_init(&X->pv_done, 1);
+        mbar_init(&X->o_empty, SOFT);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&X->s_full[i], 1); mbar_init(&X->s_empty[i], 128);
-            mbar_init(&X->sc_full[i], 1); mbar_init(&X->sc_empty[i], 128);
+            mbar_init(&X->s_full[i], 1); mbar_init(&X->s_empty[i], SOFT);
+            mbar_init(&X->sc_full[i], 1); mbar_init(&X->sc_empty[i], SOFT);
         }
         for (int i = 0; i < C::NK; ++i) { mbar_init(&X->k_full[i], 1); mbar_init(&X->k_empty[i], 1); }
-        for (int i = 0; i < C::NV; ++i) { mbar_init(&X->v_full[i], VQ ? 128 : 1); mbar_init(&X->v_empty[i], 1); mbar_init(&X->v_clean[i], 128); }
+        for (int i = 0; i < C::NV; ++i) { mbar_init(&X->v_full[i], VQ ? 128 : 1); mbar_init(&X->v_empty[i], 1); mbar_init(&X->v_clean[i], SOFT); }
         for (int i = 0; i < C::NR; ++i) { mbar_init(&X->r_full[i], 1); mbar_init(&X->r_empty[i], 128); }
         X->abort_flag = 0;
         X->start = Walk{0, 0, 0, 0};
@@ -444,58 +471,67 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
         }
     } else if (warp == 2) {
-        // ================================================================== MMAs, all from one thread
-        if (lane == 0) {
-            constexpr uint32_t idesc_s = idesc_nvfp4(ROWS, PKV_PAGE_TOKENS);
-            const uint32_t idesc_o = idesc_bf16(DH, tl.rph, true, false);
-            const uint64_t q_desc = smem_desc(sbase + C::Q_OFF, 0, 8 * C::RB, C::SWZ);
-            const uint64_t p_desc = smem_desc(sbase + C::P_OFF, 0, 1024, SWZ_128B);
-            int k = 0, kv = 0, seg = 0;
-            uint32_t cleaned = 0;                      // phase bit of every stage's v_clean
-            bool ok = true;
-            while (ok && walk.next(A.B, tl, zi, s)) {
-                const int ng = heads(s), base = s.T - s.n;
-                ok = wait_or_abort(&X->q_full, seg & 1, X, A.status, 30);
-                if (!ok) break;
-                tc_fence_after_sync();
+        // ================================================================== MMAs, issued by one elected lane
+        // The whole warp runs the loop, so that every operand of an MMA is warp-uniform: in a branch of one lane the compiler
+        // moves each descriptor through vector registers, and the issue (about 130 cycles an MMA) takes longer than the MMA.
+        const bool leader = elect_one();
+        constexpr uint32_t idesc_s = idesc_nvfp4(ROWS, PKV_PAGE_TOKENS);
+        const uint32_t idesc_o = idesc_bf16(DH, tl.rph, true, false);
+        const uint64_t q_desc = smem_desc(sbase + C::Q_OFF, 0, 8 * C::RB, C::SWZ);
+        const uint64_t p_desc = smem_desc(sbase + C::P_OFF, 0, 1024, SWZ_128B);
+        int k = 0, kv = 0, seg = 0;
+        uint32_t cleaned = 0;                          // phase bit of every stage's v_clean
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+            ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
+            return ok;
+        };
+        while (ok && walk.next(A.B, tl, zi, s)) {
+            const int ng = __shfl_sync(0xffffffffu, heads(s), 0), base = __shfl_sync(0xffffffffu, s.T - s.n, 0);
+            const int p_lo = __shfl_sync(0xffffffffu, s.p_lo, 0), p_hi = __shfl_sync(0xffffffffu, s.p_hi, 0);
+            if (!wait(&X->q_full, seg & 1, 30)) break;
+            tc_fence_after_sync();
+            if (leader)
                 for (int t = 0; t < PKV_QUERY_TERMS; ++t)
                     for (int c = 0; c < C::KB; ++c)
                         tmem_cp_32x128b_warpx4(tb + TM_SFA + (t * C::KB + c) * 4, smem_desc(sbase + C::Q_OFF + t * C::PAGE + C::CODES + c * 512, 0, 128, SWZ_NONE));
-                // O^T += V^T P^T of page p (the page before the one whose scores were just issued)
-                auto values = [&](int p, int kk) -> bool {
-                    if (!wait_or_abort(&X->p_full, kk & 1, X, A.status, 31)) return false;
-                    if (p == s.p_lo && seg > 0 && !wait_or_abort(&X->o_empty, (seg - 1) & 1, X, A.status, 35)) return false;
-                    tc_fence_after_sync();
-                    const bool tail = !VQ && base < (p + 1) * PKV_PAGE_TOKENS;     // rows that are no cached tokens: looked over first
-                    for (int g = 0; g < ng; ++g) {
-                        for (int h = 0; h < 2; ++h, ++kv) {
-                            const int st = kv % C::NV;
-                            if (!wait_or_abort(&X->v_full[st], (kv / C::NV) & 1, X, A.status, 32)) return false;
-                            if (tail) {
-                                if (!wait_or_abort(&X->v_clean[st], cleaned >> st & 1, X, A.status, 36)) return false;
-                                cleaned ^= 1u << st;
-                            }
-                            tc_fence_after_sync();
-                            const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
-                            const uint64_t pg_desc = p_desc + (uint64_t)((h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
+            // O^T += V^T P^T of page p (the page before the one whose scores were just issued)
+            auto values = [&](int p, int kk) {
+                if (!wait(&X->p_full, kk & 1, 31)) return;
+                if (p == p_lo && seg > 0 && !wait(&X->o_empty, (seg - 1) & 1, 35)) return;
+                tc_fence_after_sync();
+                const bool tail = !VQ && base < (p + 1) * PKV_PAGE_TOKENS;     // rows that are no cached tokens: looked over first
+                for (int g = 0; g < ng; ++g) {
+                    for (int h = 0; h < 2; ++h, ++kv) {
+                        const int st = kv % C::NV;
+                        if (!wait(&X->v_full[st], (kv / C::NV) & 1, 32)) return;
+                        if (tail) {
+                            if (!wait(&X->v_clean[st], cleaned >> st & 1, 36)) return;
+                            cleaned ^= 1u << st;
+                        }
+                        tc_fence_after_sync();
+                        const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
+                        const uint64_t pg_desc = p_desc + (uint64_t)((h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
+                        if (leader) {
 #pragma unroll
                             for (int c = 0; c < HALF / 16; ++c)
                                 mma_bf16(tb + TM_O + g * tl.rph, v_desc + (uint64_t)(c * 16 * 128 / 16), pg_desc + (uint64_t)(c * 32 / 16), idesc_o,
-                                         !(p == s.p_lo && h == 0 && c == 0));
+                                         !(p == p_lo && h == 0 && c == 0));
                             tc_commit(&X->v_empty[st]);
                         }
                     }
-                    tc_commit(&X->pv_done);
-                    return true;
-                };
-                for (int p = s.p_lo; p < s.p_hi && ok; ++p, ++k) {
-                    const int st = k % C::NK, sb = k & 1;
-                    ok = wait_or_abort(&X->k_full[st], (k / C::NK) & 1, X, A.status, 33);
-                    if (ok && k >= 2) ok = wait_or_abort(&X->s_empty[sb], ((k >> 1) - 1) & 1, X, A.status, 34);
-                    if (!ok) break;
-                    tc_fence_after_sync();
-                    const uint32_t ka = sbase + C::K_OFF + st * C::PAGE, sfb = tb + TM_SFB + 16 * sb;
-                    const uint64_t k_desc = smem_desc(ka, 0, 8 * C::RB, C::SWZ), sf_desc = smem_desc(ka + C::CODES, 0, 128, SWZ_NONE);
+                }
+                if (leader) tc_commit(&X->pv_done);
+            };
+            for (int p = p_lo; p < p_hi; ++p, ++k) {
+                const int st = k % C::NK, sb = k & 1;
+                wait(&X->k_full[st], (k / C::NK) & 1, 33);
+                if (k >= 2) wait(&X->s_empty[sb], ((k >> 1) - 1) & 1, 34);
+                if (!ok) break;
+                tc_fence_after_sync();
+                const uint32_t ka = sbase + C::K_OFF + st * C::PAGE, sfb = tb + TM_SFB + 16 * sb;
+                const uint64_t k_desc = smem_desc(ka, 0, 8 * C::RB, C::SWZ), sf_desc = smem_desc(ka + C::CODES, 0, 128, SWZ_NONE);
+                if (leader) {
 #pragma unroll
                     for (int c = 0; c < C::KB; ++c) tmem_cp_32x128b_warpx4(sfb + 4 * c, sf_desc + (uint64_t)(c * 512 / 16));
 #pragma unroll
@@ -506,17 +542,18 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                                       tb + TM_SFA + (t * C::KB + c) * 4, sfb + 4 * c, t != 0 || c != 0);
                     tc_commit(&X->k_empty[st]);
                     tc_commit(&X->s_full[sb]);
-                    if (p + 1 == s.p_hi) tc_commit(&X->q_empty);
-                    if (p > s.p_lo) ok = values(p - 1, k - 1);
+                    if (p + 1 == p_hi) tc_commit(&X->q_empty);
                 }
-                if (ok) ok = values(s.p_hi - 1, k - 1);
-                ++seg;
+                __syncwarp();
+                if (p > p_lo) values(p - 1, k - 1);
             }
+            if (ok) values(p_hi - 1, k - 1);
+            ++seg;
         }
-    } else if (VQ && warp >= 8) {
+    } else if (VQ && warp >= 12) {
         // ================================================================== quantised values -> bf16 operand tiles
         // Every E2M1 level is a bf16 number; the token's scale goes into the softmax weight. 128 threads, two per token.
-        const int r = (tid - 256) >> 1, part = tid & 1;
+        const int r = (tid - 384) >> 1, part = tid & 1;
         auto prmt = [](uint32_t a, uint32_t b, uint32_t c) -> uint32_t {
             uint32_t d;
             asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -556,13 +593,15 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
         }
     } else if (warp >= 4) {
-        // ================================================================== softmax: a row per thread
-        const int quad = warp & 3, r = quad * 32 + lane;
+        // ================================================================== softmax: a row per thread, two threads per row
+        // Thread (r, half) takes tokens 64 half .. of every page of row r: two warps per scheduler, so that one's arithmetic
+        // runs while the other waits for the special-function unit. Both hold the same reference maximum.
+        const int quad = warp & 3, half = (warp - 4) >> 2, r = quad * 32 + lane, st_id = half * ROWS + r;
         const uint32_t tl_s = tb + ((uint32_t)(quad * 32) << 16);
         const float* row_scale = reinterpret_cast<const float*>(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE);
-        uint8_t* p_row = smem + C::P_OFF + r * 128;
+        uint8_t* p_row = smem + C::P_OFF + half * (C::P_BYTES / 2) + r * 128;
         int k = 0, kv = 0, seg = 0;
-        bool ok = true;                              // false once any wait of this warp gave up; the loops end for all four together
+        bool ok = true;                              // false once any wait of this warp gave up; the loops end for all eight together
         auto wait_all = [&](uint64_t* bar, uint32_t parity, int where) {
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
         };
@@ -585,22 +624,22 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             for (int p = s.p_lo; p < s.p_hi; ++p, ++k, kv += 2 * ng) {
                 const int sb = k & 1, drafts = base - p * PKV_PAGE_TOKENS;
                 wait_all(&X->s_full[sb], (k >> 1) & 1, 41);
-                float x[128];
+                float x[64];
                 if (ok) {
                     tc_fence_after_sync();
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(tl_s + TM_S + 128 * sb + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
+                    for (int c = 0; c < 2; ++c) tmem_ld32(tl_s + TM_S + 128 * sb + 64 * half + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
                     tmem_ld_wait();
                     tc_fence_before_sync();
                     mbar_arrive(&X->s_empty[sb]);
                 } else {
 #pragma unroll
-                    for (int c = 0; c < 128; ++c) x[c] = 0.0f;
+                    for (int c = 0; c < 64; ++c) x[c] = 0.0f;
                 }
                 if (drafts < PKV_PAGE_TOKENS || !mine) {                // tokens the row does not see
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int j0 = 32 * c - drafts;                 // drafted token of the chunk's first column (negative: cached)
+                    for (int c = 0; c < 2; ++c) {
+                        const int j0 = 64 * half + 32 * c - drafts;     // drafted token of the chunk's first column (negative: cached)
                         uint32_t see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
                         if (!mine) see = 0u;
 #pragma unroll
@@ -610,22 +649,24 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 }
                 float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+                for (int c = 4; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cs;
-                const bool need = top > m + RESCALE_THRESHOLD;
                 // the reference maximum of a row only moves when a page exceeds it by 2^8: then its column of O^T is rescaled
-                if (softmax_any(need || !ok)) {
-                    float f = 1.0f;
-                    if (need) {
-                        if (m > -INFINITY) { f = exp2f(m - top); l *= f; }
-                        m = top;
-                    }
-                    X->row_f[r] = f;
+                if (softmax_any(top > m + RESCALE_THRESHOLD || !ok)) {
+                    X->row_m[half][r] = top;
                     if (p > s.p_lo) wait_all(&X->pv_done, (k - 1) & 1, 42);        // the accumulators are at rest
-                    if (softmax_any(!ok)) { go = false; break; }                   // (the same answer in all four warps)
+                    if (softmax_any(!ok)) { go = false; break; }                   // (the same answer in all warps)
+                    const float both = fmaxf(X->row_m[0][r], X->row_m[1][r]);
+                    float f = 1.0f;
+                    if (both > m + RESCALE_THRESHOLD) {
+                        if (m > -INFINITY) { f = exp2f(m - both); l *= f; }
+                        m = both;
+                    }
                     if (p > s.p_lo) {
+                        if (half == 0) X->row_f[r] = f;
+                        softmax_sync();
                         tc_fence_after_sync();
-                        for (int c0 = 0; c0 < ng * tl.rph; c0 += 16) {
+                        for (int c0 = 16 * half; c0 < ng * tl.rph; c0 += 32) {
                             uint32_t o[16];
                             tmem_ld16(tl_s + TM_O + c0, o);
                             tmem_ld_wait();
@@ -636,17 +677,17 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         tmem_st_wait();
                         tc_fence_before_sync();
                     }
-                    softmax_sync();                                     // row_f has been read
+                    softmax_sync();                                     // row_m, row_f have been read
                 }
                 const float mu = m > -INFINITY ? m : 0.0f;              // nothing seen yet: every weight is 2^-inf
                 float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t w[64];
+                uint32_t w[32];
                 if constexpr (VQ) {
                     // the weight of a token carries its value scale of this row's kv head (a masked one's may be anything)
                     wait_all(&X->sc_full[k & 1], (k >> 1) & 1, 46);
-                    const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + (k & 1) * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2);
+                    const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + (k & 1) * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + half * 128);
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
+                    for (int c = 0; c < 8; ++c) {
                         const uint4 q4 = sc[c];
                         const uint32_t qs[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
@@ -661,17 +702,17 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so that
                     // numerator and denominator agree
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) {
+                    for (int c = 0; c < 32; ++c) {
                         w[c] = pack_bf16(ex2_fast(fmaf(x[2 * c], cs, -mu)), ex2_fast(fmaf(x[2 * c + 1], cs, -mu)));
                         sum[c & 3] += __uint_as_float(w[c] << 16) + __uint_as_float(w[c] & 0xffff0000u);
                     }
                 }
                 l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                 if (k > 0) wait_all(&X->pv_done, (k - 1) & 1, 43);      // the weights of the page before have been read
-                // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, two blocks
+                // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, a block per half
 #pragma unroll
-                for (int c = 0; c < 16; ++c)
-                    *reinterpret_cast<uint4*>(p_row + (c >> 3) * (C::P_BYTES / 2) + (((c & 7) ^ (r & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+                for (int c = 0; c < 8; ++c)
+                    *reinterpret_cast<uint4*>(p_row + ((c ^ (r & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
                 fence_proxy_async_smem();
                 mbar_arrive(&X->p_full);
                 if constexpr (!VQ) {
@@ -686,8 +727,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                             if (!ok) break;
                             uint8_t* tile = smem + C::V_OFF + st * C::V_BYTES;
 #pragma unroll 4
-                            for (int it = 0; it < C::V_BYTES / 16 / 128 && drafts < (h + 1) * HALF; ++it) {
-                                const int id = it * 128 + r, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
+                            for (int it = 0; it < C::V_BYTES / 16 / SOFT && drafts < (h + 1) * HALF; ++it) {
+                                const int id = it * SOFT + st_id, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
                                 if (d < 0) continue;
                                 uint4* at = reinterpret_cast<uint4*>(tile) + id;
                                 if (d >= s.n) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
@@ -710,17 +751,21 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             if (!go) break;
             // ---- the tile's stretch is done: O^T out of tensor memory
             wait_all(&X->pv_done, (k - 1) & 1, 44);
+            X->row_m[half][r] = l;
             if (softmax_any(!ok)) { go = false; break; }
             tc_fence_after_sync();
-            if (!VQ && mine && ((word & 0xffffffffu & X->bad[gl][0]) | ((word >> 32) & X->bad[gl][1]))) l = __int_as_float(0x7fc00000);
             const bool whole = s.p_lo == 0 && s.p_hi == s.pages;
             const size_t slot = (size_t)blockIdx.x * 2 + (s.p_lo == 0);
-            if (whole) X->row_f[r] = l == 0.0f ? 0.0f : 1.0f / l;       // a row that sees nothing: zeros
-            else if (mine) A.part_ml[slot * ROWS + r] = make_float2(m, l);
+            if (half == 0) {
+                l += X->row_m[1][r];
+                if (!VQ && mine && ((word & 0xffffffffu & X->bad[gl][0]) | ((word >> 32) & X->bad[gl][1]))) l = __int_as_float(0x7fc00000);
+                if (whole) X->row_f[r] = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing: zeros
+                else if (mine) A.part_ml[slot * ROWS + r] = make_float2(m, l);
+            }
             softmax_sync();
-            if (r < MAX_G * 2) X->bad[r >> 1][r & 1] = 0u;
+            if (st_id < MAX_G * 2) X->bad[st_id >> 1][st_id & 1] = 0u;
             for (int g = 0; g < ng; ++g) {
-                for (int c0 = 0; c0 < nq * tl.rep; c0 += 16) {
+                for (int c0 = 16 * half; c0 < nq * tl.rep; c0 += 32) {
                     uint32_t o[16];
                     tmem_ld16(tl_s + TM_O + g * tl.rph + c0, o);
                     tmem_ld_wait();
@@ -739,7 +784,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
             tc_fence_before_sync();
             mbar_arrive(&X->o_empty);
-            softmax_sync();                                             // row_f and bad are free again
+            softmax_sync();                                             // row_m, row_f and bad are free again
             ++seg;
         }
     }
