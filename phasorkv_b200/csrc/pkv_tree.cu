@@ -471,58 +471,27 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
         }
     } else if (warp == 2) {
-        // ================================================================== MMAs, issued by one elected lane
+        // ================================================================== score MMAs, issued by one elected lane
         // The whole warp runs the loop, so that every operand of an MMA is warp-uniform: in a branch of one lane the compiler
         // moves each descriptor through vector registers, and the issue (about 130 cycles an MMA) takes longer than the MMA.
+        // Scores and P.V are issued by a warp each: one that waits for values must not hold up the next page's scores.
         const bool leader = elect_one();
         constexpr uint32_t idesc_s = idesc_nvfp4(ROWS, PKV_PAGE_TOKENS);
-        const uint32_t idesc_o = idesc_bf16(DH, tl.rph, true, false);
         const uint64_t q_desc = smem_desc(sbase + C::Q_OFF, 0, 8 * C::RB, C::SWZ);
-        const uint64_t p_desc = smem_desc(sbase + C::P_OFF, 0, 1024, SWZ_128B);
-        int k = 0, kv = 0, seg = 0;
-        uint32_t cleaned = 0;                          // phase bit of every stage's v_clean
+        int k = 0, seg = 0;
         bool ok = true;
         auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
-            return ok;
         };
         while (ok && walk.next(A.B, tl, zi, s)) {
-            const int ng = __shfl_sync(0xffffffffu, heads(s), 0), base = __shfl_sync(0xffffffffu, s.T - s.n, 0);
             const int p_lo = __shfl_sync(0xffffffffu, s.p_lo, 0), p_hi = __shfl_sync(0xffffffffu, s.p_hi, 0);
-            if (!wait(&X->q_full, seg & 1, 30)) break;
+            wait(&X->q_full, seg & 1, 30);
+            if (!ok) break;
             tc_fence_after_sync();
             if (leader)
                 for (int t = 0; t < PKV_QUERY_TERMS; ++t)
                     for (int c = 0; c < C::KB; ++c)
                         tmem_cp_32x128b_warpx4(tb + TM_SFA + (t * C::KB + c) * 4, smem_desc(sbase + C::Q_OFF + t * C::PAGE + C::CODES + c * 512, 0, 128, SWZ_NONE));
-            // O^T += V^T P^T of page p (the page before the one whose scores were just issued)
-            auto values = [&](int p, int kk) {
-                if (!wait(&X->p_full, kk & 1, 31)) return;
-                if (p == p_lo && seg > 0 && !wait(&X->o_empty, (seg - 1) & 1, 35)) return;
-                tc_fence_after_sync();
-                const bool tail = !VQ && base < (p + 1) * PKV_PAGE_TOKENS;     // rows that are no cached tokens: looked over first
-                for (int g = 0; g < ng; ++g) {
-                    for (int h = 0; h < 2; ++h, ++kv) {
-                        const int st = kv % C::NV;
-                        if (!wait(&X->v_full[st], (kv / C::NV) & 1, 32)) return;
-                        if (tail) {
-                            if (!wait(&X->v_clean[st], cleaned >> st & 1, 36)) return;
-                            cleaned ^= 1u << st;
-                        }
-                        tc_fence_after_sync();
-                        const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
-                        const uint64_t pg_desc = p_desc + (uint64_t)((h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
-                        if (leader) {
-#pragma unroll
-                            for (int c = 0; c < HALF / 16; ++c)
-                                mma_bf16(tb + TM_O + g * tl.rph, v_desc + (uint64_t)(c * 16 * 128 / 16), pg_desc + (uint64_t)(c * 32 / 16), idesc_o,
-                                         !(p == p_lo && h == 0 && c == 0));
-                            tc_commit(&X->v_empty[st]);
-                        }
-                    }
-                }
-                if (leader) tc_commit(&X->pv_done);
-            };
             for (int p = p_lo; p < p_hi; ++p, ++k) {
                 const int st = k % C::NK, sb = k & 1;
                 wait(&X->k_full[st], (k / C::NK) & 1, 33);
@@ -545,9 +514,50 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     if (p + 1 == p_hi) tc_commit(&X->q_empty);
                 }
                 __syncwarp();
-                if (p > p_lo) values(p - 1, k - 1);
             }
-            if (ok) values(p_hi - 1, k - 1);
+            ++seg;
+        }
+    } else if (warp == 3) {
+        // ================================================================== P.V MMAs: O^T += V^T P^T
+        const bool leader = elect_one();
+        const uint32_t idesc_o = idesc_bf16(DH, tl.rph, true, false);
+        const uint64_t p_desc = smem_desc(sbase + C::P_OFF, 0, 1024, SWZ_128B);
+        int k = 0, kv = 0, seg = 0;
+        uint32_t cleaned = 0;                          // phase bit of every stage's v_clean
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+            ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
+        };
+        while (ok && walk.next(A.B, tl, zi, s)) {
+            const int ng = __shfl_sync(0xffffffffu, heads(s), 0), base = __shfl_sync(0xffffffffu, s.T - s.n, 0);
+            const int p_lo = __shfl_sync(0xffffffffu, s.p_lo, 0), p_hi = __shfl_sync(0xffffffffu, s.p_hi, 0);
+            for (int p = p_lo; p < p_hi && ok; ++p, ++k) {
+                wait(&X->p_full, k & 1, 31);
+                if (p == p_lo && seg > 0) wait(&X->o_empty, (seg - 1) & 1, 35);
+                const bool tail = !VQ && base < (p + 1) * PKV_PAGE_TOKENS;     // rows that are no cached tokens: looked over first
+                for (int j = 0; j < 2 * ng && ok; ++j, ++kv) {
+                    const int st = kv % C::NV, g = j >> 1, h = j & 1;
+                    wait(&X->v_full[st], (kv / C::NV) & 1, 32);
+                    if (tail) {
+                        wait(&X->v_clean[st], cleaned >> st & 1, 36);
+                        cleaned ^= 1u << st;
+                    }
+                    if (!ok) break;
+                    tc_fence_after_sync();
+                    const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
+                    const uint64_t pg_desc = p_desc + (uint64_t)((h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
+                    if (leader) {
+#pragma unroll
+                        for (int c = 0; c < HALF / 16; ++c)
+                            mma_bf16(tb + TM_O + g * tl.rph, v_desc + (uint64_t)(c * 16 * 128 / 16), pg_desc + (uint64_t)(c * 32 / 16), idesc_o,
+                                     !(p == p_lo && h == 0 && c == 0));
+                        tc_commit(&X->v_empty[st]);
+                    }
+                    __syncwarp();
+                }
+                if (ok && leader) tc_commit(&X->pv_done);
+                __syncwarp();
+            }
             ++seg;
         }
     } else if (VQ && warp >= 12) {
