@@ -30,7 +30,8 @@ using namespace pkv;
 
 constexpr int DH = 128, ROWS = 128;                  // head dim; rows of a tile
 constexpr int HALF = 64;                             // tokens per V stage: half a page of one kv head
-constexpr int SOFT = 256;                            // softmax threads: two per row, 64 tokens of a page each
+constexpr int GROUP = 128;                           // threads of a softmax group: one per row of the tile; two groups, page about
+constexpr int GROUP_WARPS = GROUP / 32;              // what they hand over is counted per warp: 32 arrivals at one word take turns
 constexpr int MAX_G = 8;                             // kv heads of a tile (16 rows at least each)
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in base-2 logits
 constexpr uint32_t WAIT_LIMIT = 1u << 19;            // probes of a bounded wait
@@ -229,36 +230,38 @@ template <int WP, bool VQ>
 struct Cfg {
     static constexpr int RB = WP / 2, KB = WP / 64, PAGE = page_bytes(WP), CODES = PKV_PAGE_TOKENS * RB;
     static constexpr int NK = WP == 256 ? 2 : 4;                                  // latent pages in flight
-    static constexpr int NV = VQ ? (WP == 256 ? 3 : 4) : (WP == 256 ? 5 : 7);     // V operand stages (64 tokens of a kv head, bf16)
-    static constexpr int NR = VQ ? (WP == 256 ? 5 : 8) : 0;                       // raw stages of quantised V
+    static constexpr int NV = VQ ? (WP == 256 ? 2 : 3) : (WP == 256 ? 3 : 5);     // V operand stages (64 tokens of a kv head, bf16)
+    static constexpr int NR = VQ ? (WP == 256 ? 3 : 8) : 0;                       // raw stages of quantised V
     static constexpr int V_BYTES = HALF * DH * 2, RAW_BYTES = HALF * DH / 2, P_BYTES = ROWS * PKV_PAGE_TOKENS * 2;
     static constexpr int SC_BYTES = MAX_G * PKV_PAGE_TOKENS * 2;                  // token scales of a page
     static constexpr int Q_OFF = 0;
     static constexpr int K_OFF = (blob_bytes(WP) + 1023) / 1024 * 1024;
     static constexpr int V_OFF = K_OFF + NK * PAGE;
     static constexpr int P_OFF = V_OFF + NV * V_BYTES;
-    static constexpr int R_OFF = P_OFF + P_BYTES;
+    static constexpr int R_OFF = P_OFF + 2 * P_BYTES;                             // weights: a buffer per softmax group
     static constexpr int SC_OFF = R_OFF + NR * RAW_BYTES;
     static constexpr int X_OFF = SC_OFF + (VQ ? 2 * SC_BYTES : 0);
-    static constexpr int SMEM = X_OFF + 3072;
+    static constexpr int SMEM = X_OFF + 5120;
     static constexpr int NTHREADS = VQ ? 512 : 384;
     static constexpr uint64_t SWZ = RB == 128 ? SWZ_128B : SWZ_64B;
     static_assert(SMEM <= 232448 && V_OFF % 1024 == 0 && P_OFF % 1024 == 0, "shared memory of a CTA");
 };
 
 struct Shared {                       // at X_OFF
-    uint64_t q_full, q_empty, p_full, pv_done, o_empty;
+    uint64_t q_full, q_empty, o_empty, meet;
+    uint64_t p_full[2], pv_done[2], decided[GROUP_WARPS];
     uint64_t k_full[4], k_empty[4], v_full[7], v_empty[7], v_clean[7], s_full[2], s_empty[2];
     uint64_t r_full[8], r_empty[8], sc_full[2], sc_empty[2];
     uint32_t tmem_base;
     volatile int abort_flag;
     Walk start;
-    float row_f[ROWS];                // rescale factors, then 1 / sum
-    uint32_t bad[MAX_G][2];           // drafted tokens whose value row of a kv head is not finite
-    float row_m[2][ROWS];             // maxima of the two halves of a row, then their sums
+    float row_m[ROWS];                // reference maximum of each row after the last page decided
+    float row_f[2][ROWS];             // per group: rescale factors, then 1 / sum
+    float row_l[2][2][ROWS];          // [stretch & 1][group]: sums at the end
+    uint32_t bad[3][MAX_G][2];        // [stretch % 3]: drafted tokens whose value row of a kv head is not finite
     long scan[16];
 };
-static_assert(sizeof(Shared) <= 3072, "behind the stages");
+static_assert(sizeof(Shared) <= 5120, "behind the stages");
 
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
     for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
@@ -276,20 +279,38 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
-// the softmax threads meet (named barrier 1) and learn whether the predicate held in any of them
-__device__ __forceinline__ bool softmax_any(bool pred) {
+// the 128 threads of a softmax group meet (named barrier 1 or 2); do they learn whether the predicate held in any of them
+__device__ __forceinline__ bool group_any(int group, bool pred) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"(pred ? 1 : 0) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(1 + group), "r"(pred ? 1 : 0) : "memory");
     return r != 0;
 }
-__device__ __forceinline__ void softmax_sync() { static_assert(SOFT == 256, "barrier width"); asm volatile("barrier.cta.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void group_sync(int group) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory"); }
+
+// one arrival for the warp, behind everything its lanes did
+__device__ __forceinline__ void arrive_warp(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 
 __device__ __forceinline__ float ex2_fast(float x) {     // 2 ulp, results below 2^-126 become 0: a weight needs no more
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -326,20 +347,21 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     // ---- barriers, tensor memory, and where on the list of pages this CTA starts. Page table, lengths, masks and pages are
     // final: the operand launch in front of this one has started, so everything before that is done.
     if (tid == 0) {
-        mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, SOFT + 1); mbar_init(&X->p_full, SOFT); mbar_init(&X->pv_done, 1);
-        mbar_init(&X->o_empty, SOFT);
+        mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 2 * GROUP_WARPS + 1);
+        mbar_init(&X->o_empty, 2 * GROUP_WARPS); mbar_init(&X->meet, 2 * GROUP_WARPS);
+        for (int i = 0; i < GROUP_WARPS; ++i) mbar_init(&X->decided[i], 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&X->s_full[i], 1); mbar_init(&X->s_empty[i], SOFT);
-            mbar_init(&X->sc_full[i], 1); mbar_init(&X->sc_empty[i], SOFT);
+            mbar_init(&X->p_full[i], GROUP_WARPS); mbar_init(&X->pv_done[i], 1); mbar_init(&X->s_full[i], 1); mbar_init(&X->s_empty[i], GROUP_WARPS);
+            mbar_init(&X->sc_full[i], 1); mbar_init(&X->sc_empty[i], GROUP_WARPS);
         }
         for (int i = 0; i < C::NK; ++i) { mbar_init(&X->k_full[i], 1); mbar_init(&X->k_empty[i], 1); }
-        for (int i = 0; i < C::NV; ++i) { mbar_init(&X->v_full[i], VQ ? 128 : 1); mbar_init(&X->v_empty[i], 1); mbar_init(&X->v_clean[i], SOFT); }
-        for (int i = 0; i < C::NR; ++i) { mbar_init(&X->r_full[i], 1); mbar_init(&X->r_empty[i], 128); }
+        for (int i = 0; i < C::NV; ++i) { mbar_init(&X->v_full[i], VQ ? 4 : 1); mbar_init(&X->v_empty[i], 1); mbar_init(&X->v_clean[i], GROUP_WARPS); }
+        for (int i = 0; i < C::NR; ++i) { mbar_init(&X->r_full[i], 1); mbar_init(&X->r_empty[i], 4); }
         X->abort_flag = 0;
         X->start = Walk{0, 0, 0, 0};
         fence_barrier_init();
     }
-    if (tid < MAX_G * 2) X->bad[tid >> 1][tid & 1] = 0u;
+    if (tid < 3 * MAX_G * 2) (&X->bad[0][0][0])[tid] = 0u;
     if (warp == 3) tmem_alloc(&X->tmem_base, TM_COLS);
     tc_fence_before_sync();
     {
@@ -532,7 +554,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             const int ng = __shfl_sync(0xffffffffu, heads(s), 0), base = __shfl_sync(0xffffffffu, s.T - s.n, 0);
             const int p_lo = __shfl_sync(0xffffffffu, s.p_lo, 0), p_hi = __shfl_sync(0xffffffffu, s.p_hi, 0);
             for (int p = p_lo; p < p_hi && ok; ++p, ++k) {
-                wait(&X->p_full, k & 1, 31);
+                wait(&X->p_full[k & 1], (k >> 1) & 1, 31);
                 if (p == p_lo && seg > 0) wait(&X->o_empty, (seg - 1) & 1, 35);
                 const bool tail = !VQ && base < (p + 1) * PKV_PAGE_TOKENS;     // rows that are no cached tokens: looked over first
                 for (int j = 0; j < 2 * ng && ok; ++j, ++kv) {
@@ -545,7 +567,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
-                    const uint64_t pg_desc = p_desc + (uint64_t)((h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
+                    const uint64_t pg_desc = p_desc + (uint64_t)(((k & 1) * C::P_BYTES + h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
                     if (leader) {
 #pragma unroll
                         for (int c = 0; c < HALF / 16; ++c)
@@ -555,7 +577,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     }
                     __syncwarp();
                 }
-                if (ok && leader) tc_commit(&X->pv_done);
+                if (ok && leader) tc_commit(&X->pv_done[k & 1]);
                 __syncwarp();
             }
             ++seg;
@@ -598,20 +620,21 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     }
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(&X->v_full[st]);
-                mbar_arrive(&X->r_empty[rs]);
+                arrive_warp(&X->v_full[st]);
+                arrive_warp(&X->r_empty[rs]);
             }
         }
     } else if (warp >= 4) {
-        // ================================================================== softmax: a row per thread, two threads per row
-        // Thread (r, half) takes tokens 64 half .. of every page of row r: two warps per scheduler, so that one's arithmetic
-        // runs while the other waits for the special-function unit. Both hold the same reference maximum.
-        const int quad = warp & 3, half = (warp - 4) >> 2, r = quad * 32 + lane, st_id = half * ROWS + r;
+        // ================================================================== softmax: a row per thread, two groups of 128 threads
+        // Group 0 takes the even pages of the CTA, group 1 the odd ones: while one waits (for scores, for tensor memory, for the
+        // tensor core to be done with the weights before), the other computes. A row's reference maximum goes from page to
+        // page between the two threads that share the row.
+        const int quad = warp & 3, grp = (warp - 4) >> 2, r = quad * 32 + lane;
         const uint32_t tl_s = tb + ((uint32_t)(quad * 32) << 16);
         const float* row_scale = reinterpret_cast<const float*>(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE);
-        uint8_t* p_row = smem + C::P_OFF + half * (C::P_BYTES / 2) + r * 128;
-        int k = 0, kv = 0, seg = 0;
-        bool ok = true;                              // false once any wait of this warp gave up; the loops end for all eight together
+        uint8_t* p_row = smem + C::P_OFF + grp * C::P_BYTES + r * 128;
+        int k = 0, kv = 0, seg = 0, own = -1;        // own: this group's last page
+        bool ok = true;                              // false once any wait of this warp gave up; a group's loop ends for all its warps
         auto wait_all = [&](uint64_t* bar, uint32_t parity, int where) {
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
         };
@@ -629,106 +652,129 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             wait_all(&X->q_full, seg & 1, 40);
             float cs = ok ? row_scale[r] * A.col_scale : 0.0f;
             if (cs < 1e-37f) cs = 1e-37f;                               // (keeps NaN; a masked score -inf x cs stays -inf)
-            mbar_arrive(&X->q_empty);
+            arrive_warp(&X->q_empty);
             float m = -INFINITY, l = 0.0f;
             for (int p = s.p_lo; p < s.p_hi; ++p, ++k, kv += 2 * ng) {
-                const int sb = k & 1, drafts = base - p * PKV_PAGE_TOKENS;
-                wait_all(&X->s_full[sb], (k >> 1) & 1, 41);
-                float x[64];
-                if (ok) {
-                    tc_fence_after_sync();
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) tmem_ld32(tl_s + TM_S + 128 * sb + 64 * half + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[32 * c]));
+                if ((k & 1) != grp) continue;
+                const int drafts = base - p * PKV_PAGE_TOKENS;
+                wait_all(&X->s_full[grp], (k >> 1) & 1, 41);
+                // The loops over a page's scores are not unrolled beyond 32 columns, and the scores are read from tensor memory twice:
+                // with everything unrolled the roles' code no longer fits the instruction cache together, and each of them runs
+                // at the speed of instruction fetch.
+                const bool masked = drafts < PKV_PAGE_TOKENS || !mine;
+                const uint32_t s_tm = tl_s + TM_S + 128 * grp;
+                float x[32];
+                auto load = [&](int c) {                                // 32 tokens; those that the row does not see become -inf
+                    tmem_ld32(s_tm + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
                     tmem_ld_wait();
-                    tc_fence_before_sync();
-                    mbar_arrive(&X->s_empty[sb]);
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 64; ++c) x[c] = 0.0f;
-                }
-                if (drafts < PKV_PAGE_TOKENS || !mine) {                // tokens the row does not see
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        const int j0 = 64 * half + 32 * c - drafts;     // drafted token of the chunk's first column (negative: cached)
+                    if (masked) {
+                        const int j0 = 32 * c - drafts;                 // drafted token of the first column (negative: cached)
                         uint32_t see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
                         if (!mine) see = 0u;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
-                            if (!(see >> e & 1)) x[32 * c + e] = -INFINITY;
+                            if (!(see >> e & 1)) x[e] = -INFINITY;
+                    }
+                };
+                tc_fence_after_sync();
+                float top = -INFINITY;
+                if (ok) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        load(c);
+                        float mx[4] = {top, x[0], x[1], x[2]};
+#pragma unroll
+                        for (int e = 3; e < 31; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], x[e], x[e + 1]);
+                        top = max3(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]), x[31]);
                     }
                 }
-                float mx[4] = {x[0], x[1], x[2], x[3]};
+                top *= cs;
+                // The reference of a row only moves when a page exceeds it by 2^8: its column of O^T is then rescaled.
+                float before = -INFINITY;
+                if (p > s.p_lo) {
+                    wait_all(&X->decided[quad], (k - 1) & 1, 42);
+                    before = X->row_m[r];
+                }
+                const bool grows = top > before + RESCALE_THRESHOLD;
+                const float ref = grows ? top : before;
+                if (grows || p == s.p_lo) X->row_m[r] = ref;
+                arrive_warp(&X->decided[quad]);
+                if (ref != m) { l *= exp2f(m - ref); m = ref; }         // (both -inf: equal)
+                const float mu = m > -INFINITY ? m : 0.0f;              // nothing seen yet: every weight is 2^-inf
+                const float2 cs2 = make_float2(cs, cs), mu2 = make_float2(-mu, -mu);
+                float2 sum = make_float2(0.0f, 0.0f);
+                if constexpr (VQ) wait_all(&X->sc_full[grp], (k >> 1) & 1, 46);
+                if (k >= 2) wait_all(&X->pv_done[grp], ((k >> 1) - 1) & 1, 43);     // the weights of this group's page before have been read
+                if (ok) {
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        load(c);
+                        uint32_t w[16];
+                        if constexpr (VQ) {
+                            // the weight of a token carries its value scale of this row's kv head (a masked one's may be anything)
+                            const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + grp * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + c * 64);
 #pragma unroll
-                for (int c = 4; c < 64; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cs;
-                // the reference maximum of a row only moves when a page exceeds it by 2^8: then its column of O^T is rescaled
-                if (softmax_any(top > m + RESCALE_THRESHOLD || !ok)) {
-                    X->row_m[half][r] = top;
-                    if (p > s.p_lo) wait_all(&X->pv_done, (k - 1) & 1, 42);        // the accumulators are at rest
-                    if (softmax_any(!ok)) { go = false; break; }                   // (the same answer in all warps)
-                    const float both = fmaxf(X->row_m[0][r], X->row_m[1][r]);
-                    float f = 1.0f;
-                    if (both > m + RESCALE_THRESHOLD) {
-                        if (m > -INFINITY) { f = exp2f(m - both); l *= f; }
-                        m = both;
+                            for (int u = 0; u < 4; ++u) {
+                                const uint4 q4 = sc[u];
+                                const uint32_t qs[4] = {q4.x, q4.y, q4.z, q4.w};
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float2 t = fma2(make_float2(x[8 * u + 2 * e], x[8 * u + 2 * e + 1]), cs2, mu2);
+                                    const float p0 = ex2_fast(t.x), p1 = ex2_fast(t.y);
+                                    sum = add2(sum, make_float2(p0, p1));
+                                    w[4 * u + e] = pack_bf16(p0 == 0.0f ? 0.0f : p0 * __uint_as_float(qs[e] << 16), p1 == 0.0f ? 0.0f : p1 * __uint_as_float(qs[e] & 0xffff0000u));
+                                }
+                            }
+                        } else {
+                            // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so that
+                            // numerator and denominator agree
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float2 t = fma2(make_float2(x[2 * e], x[2 * e + 1]), cs2, mu2);
+                                w[e] = pack_bf16(ex2_fast(t.x), ex2_fast(t.y));
+                                sum = add2(sum, make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)));
+                            }
+                        }
+                        // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, a block per half page
+                        uint8_t* line = p_row + (c >> 1) * (C::P_BYTES / 2);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            *reinterpret_cast<uint4*>(line + ((((c & 1) * 4 + u) ^ (r & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                     }
+                }
+                tc_fence_before_sync();
+                arrive_warp(&X->s_empty[grp]);
+                if constexpr (VQ) arrive_warp(&X->sc_empty[grp]);
+                l += sum.x + sum.y;
+                if (group_any(grp, grows || !ok)) {
+                    if (group_any(grp, !ok)) { go = false; break; }     // (the same answer in all warps of the group)
                     if (p > s.p_lo) {
-                        if (half == 0) X->row_f[r] = f;
-                        softmax_sync();
+                        wait_all(&X->pv_done[grp ^ 1], ((k - 1) >> 1) & 1, 49);         // the accumulators are at rest
+                        X->row_f[grp][r] = grows && before > -INFINITY ? exp2f(before - ref) : 1.0f;
+                        group_sync(grp);
                         tc_fence_after_sync();
-                        for (int c0 = 16 * half; c0 < ng * tl.rph; c0 += 32) {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < ng * tl.rph; c0 += 16) {
                             uint32_t o[16];
                             tmem_ld16(tl_s + TM_O + c0, o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * X->row_f[c0 + c]);
+                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * X->row_f[grp][c0 + c]);
                             tmem_st16(tl_s + TM_O + c0, o);
                         }
                         tmem_st_wait();
                         tc_fence_before_sync();
-                    }
-                    softmax_sync();                                     // row_m, row_f have been read
-                }
-                const float mu = m > -INFINITY ? m : 0.0f;              // nothing seen yet: every weight is 2^-inf
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                uint32_t w[32];
-                if constexpr (VQ) {
-                    // the weight of a token carries its value scale of this row's kv head (a masked one's may be anything)
-                    wait_all(&X->sc_full[k & 1], (k >> 1) & 1, 46);
-                    const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + (k & 1) * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + half * 128);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) {
-                        const uint4 q4 = sc[c];
-                        const uint32_t qs[4] = {q4.x, q4.y, q4.z, q4.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float p0 = ex2_fast(fmaf(x[8 * c + 2 * e], cs, -mu)), p1 = ex2_fast(fmaf(x[8 * c + 2 * e + 1], cs, -mu));
-                            sum[e] += p0 + p1;
-                            w[4 * c + e] = pack_bf16(p0 == 0.0f ? 0.0f : p0 * __uint_as_float(qs[e] << 16), p1 == 0.0f ? 0.0f : p1 * __uint_as_float(qs[e] & 0xffff0000u));
-                        }
-                    }
-                    mbar_arrive(&X->sc_empty[k & 1]);
-                } else {
-                    // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so that
-                    // numerator and denominator agree
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) {
-                        w[c] = pack_bf16(ex2_fast(fmaf(x[2 * c], cs, -mu)), ex2_fast(fmaf(x[2 * c + 1], cs, -mu)));
-                        sum[c & 3] += __uint_as_float(w[c] << 16) + __uint_as_float(w[c] & 0xffff0000u);
+                        group_sync(grp);                                // row_f has been read
                     }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                if (k > 0) wait_all(&X->pv_done, (k - 1) & 1, 43);      // the weights of the page before have been read
-                // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, a block per half
-#pragma unroll
-                for (int c = 0; c < 8; ++c)
-                    *reinterpret_cast<uint4*>(p_row + ((c ^ (r & 7)) << 4)) = make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
                 fence_proxy_async_smem();
-                mbar_arrive(&X->p_full);
+                arrive_warp(&X->p_full[grp]);
+                own = k;
                 if constexpr (!VQ) {
                     // Values behind the cached tokens: rows past the sequence become zero, and so does what is not finite in a
                     // drafted row (0 x inf would reach rows that do not see it); who does see it gets NaN at the end.
                     if (drafts < PKV_PAGE_TOKENS && ok) {
+                        if (k > 0) wait_all(&X->pv_done[grp ^ 1], ((k - 1) >> 1) & 1, 50);
                         // (Every tile of such a page is handed over, also one with cached rows only: the page before is known to be
                         // consumed, and within this one the stages then advance in step with these waits.)
                         for (int j = 0; j < 2 * ng; ++j) {
@@ -737,8 +783,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                             if (!ok) break;
                             uint8_t* tile = smem + C::V_OFF + st * C::V_BYTES;
 #pragma unroll 4
-                            for (int it = 0; it < C::V_BYTES / 16 / SOFT && drafts < (h + 1) * HALF; ++it) {
-                                const int id = it * SOFT + st_id, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
+                            for (int it = 0; it < C::V_BYTES / 16 / GROUP && drafts < (h + 1) * HALF; ++it) {
+                                const int id = it * GROUP + r, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
                                 if (d < 0) continue;
                                 uint4* at = reinterpret_cast<uint4*>(tile) + id;
                                 if (d >= s.n) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
@@ -750,32 +796,38 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                                     if ((e[q] & 0x7f80u) == 0x7f80u) { e[q] &= 0xffff0000u; hit = true; }
                                     if ((e[q] & 0x7f800000u) == 0x7f800000u) { e[q] &= 0xffffu; hit = true; }
                                 }
-                                if (hit) { *at = v; atomicOr(&X->bad[j >> 1][d >> 5], 1u << (d & 31)); }
+                                if (hit) { *at = v; atomicOr(&X->bad[seg % 3][j >> 1][d >> 5], 1u << (d & 31)); }
                             }
                             fence_proxy_async_smem();
-                            mbar_arrive(&X->v_clean[st]);
+                            arrive_warp(&X->v_clean[st]);
                         }
                     }
                 }
             }
             if (!go) break;
-            // ---- the tile's stretch is done: O^T out of tensor memory
-            wait_all(&X->pv_done, (k - 1) & 1, 44);
-            X->row_m[half][r] = l;
-            if (softmax_any(!ok)) { go = false; break; }
+            // ---- the tile's stretch is done: O^T out of tensor memory, 16 columns by each group in turn
+            // (its own last page first: only neighbouring phases of a barrier can be told apart)
+            if (own >= 0) wait_all(&X->pv_done[grp], (own >> 1) & 1, 44);
+            wait_all(&X->pv_done[(k - 1) & 1], ((k - 1) >> 1) & 1, 44);
+            const float M = X->row_m[r];                                // the last page's reference
+            if (m != M) l *= exp2f(m - M);
+            X->row_l[seg & 1][grp][r] = l;
+            if (r < MAX_G * 2) (&X->bad[(seg + 1) % 3][0][0])[r] = 0u;  // (last read before the meeting of the stretch before)
+            arrive_warp(&X->meet);
+            wait_all(&X->meet, seg & 1, 45);                            // both groups
+            if (group_any(grp, !ok)) { go = false; break; }
             tc_fence_after_sync();
             const bool whole = s.p_lo == 0 && s.p_hi == s.pages;
             const size_t slot = (size_t)blockIdx.x * 2 + (s.p_lo == 0);
-            if (half == 0) {
-                l += X->row_m[1][r];
-                if (!VQ && mine && ((word & 0xffffffffu & X->bad[gl][0]) | ((word >> 32) & X->bad[gl][1]))) l = __int_as_float(0x7fc00000);
-                if (whole) X->row_f[r] = l == 0.0f ? 0.0f : 1.0f / l;   // a row that sees nothing: zeros
-                else if (mine) A.part_ml[slot * ROWS + r] = make_float2(m, l);
-            }
-            softmax_sync();
-            if (st_id < MAX_G * 2) X->bad[st_id >> 1][st_id & 1] = 0u;
+            l = X->row_l[seg & 1][0][r] + X->row_l[seg & 1][1][r];
+            if (!VQ && mine && ((word & 0xffffffffu & X->bad[seg % 3][gl][0]) | ((word >> 32) & X->bad[seg % 3][gl][1]))) l = __int_as_float(0x7fc00000);
+            X->row_f[grp][r] = l == 0.0f ? 0.0f : 1.0f / l;         // a row that sees nothing: zeros
+            if (!whole && mine && grp == 0) A.part_ml[slot * ROWS + r] = make_float2(M, l);
+            group_sync(grp);
+#pragma unroll 1
             for (int g = 0; g < ng; ++g) {
-                for (int c0 = 16 * half; c0 < nq * tl.rep; c0 += 32) {
+#pragma unroll 1
+                for (int c0 = 16 * grp; c0 < nq * tl.rep; c0 += 32) {
                     uint32_t o[16];
                     tmem_ld16(tl_s + TM_O + g * tl.rph + c0, o);
                     tmem_ld_wait();
@@ -785,7 +837,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         if (q >= nq * tl.rep) break;
                         if (whole) {
                             const size_t row = (size_t)(s.lo + first + q / tl.rep) * A.n_q + (s.z % tl.groups * tl.G + g) * tl.rep + q % tl.rep;
-                            A.out[row * DH + r] = __float2bfloat16(__uint_as_float(o[c]) * X->row_f[g * tl.rph + q]);
+                            A.out[row * DH + r] = __float2bfloat16(__uint_as_float(o[c]) * X->row_f[grp][g * tl.rph + q]);
                         } else {
                             A.part_o[(slot * ROWS + g * tl.rph + q) * DH + r] = __uint_as_float(o[c]);
                         }
@@ -793,8 +845,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 }
             }
             tc_fence_before_sync();
-            mbar_arrive(&X->o_empty);
-            softmax_sync();                                             // row_m, row_f and bad are free again
+            arrive_warp(&X->o_empty);
+            group_sync(grp);                                            // row_f is free again
             ++seg;
         }
     }
