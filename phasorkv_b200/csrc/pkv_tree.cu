@@ -230,8 +230,9 @@ template <int WP, bool VQ>
 struct Cfg {
     static constexpr int RB = WP / 2, KB = WP / 64, PAGE = page_bytes(WP), CODES = PKV_PAGE_TOKENS * RB;
     static constexpr int NK = WP == 256 ? 2 : 4;                                  // latent pages in flight
-    static constexpr int NV = VQ ? (WP == 256 ? 2 : 3) : (WP == 256 ? 3 : 5);     // V operand stages (64 tokens of a kv head, bf16)
-    static constexpr int NR = VQ ? (WP == 256 ? 3 : 8) : 0;                       // raw stages of quantised V
+    // V operand stages (64 tokens of a kv head, bf16) and, of quantised V, raw stages: what is left of the shared memory
+    static constexpr int NV = VQ ? (WP == 256 ? 2 : 3) : (WP == 256 ? 3 : 5);
+    static constexpr int NR = VQ ? (WP == 256 ? 3 : 8) : 0;
     static constexpr int V_BYTES = HALF * DH * 2, RAW_BYTES = HALF * DH / 2, P_BYTES = ROWS * PKV_PAGE_TOKENS * 2;
     static constexpr int SC_BYTES = MAX_G * PKV_PAGE_TOKENS * 2;                  // token scales of a page
     static constexpr int Q_OFF = 0;
@@ -263,7 +264,7 @@ struct Shared {                       // at X_OFF
 };
 static_assert(sizeof(Shared) <= 5120, "behind the stages");
 
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
+__device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
     for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 1023u) == 1023u && X->abort_flag) return false;
@@ -271,6 +272,10 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Sh
     X->abort_flag = 1;
     if (status) { atomicExch(&status[0], 1); atomicExch(&status[1], where); }
     return false;
+}
+// bounded; false when it gave up, or another role did (out of line: it is in many places, and the code has to stay small)
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
+    return mbar_try_wait(bar, parity) || wait_longer(bar, parity, X, status, where);
 }
 
 __device__ __forceinline__ bool elect_one() {
@@ -511,6 +516,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             if (!ok) break;
             tc_fence_after_sync();
             if (leader)
+#pragma unroll 1
                 for (int t = 0; t < PKV_QUERY_TERMS; ++t)
                     for (int c = 0; c < C::KB; ++c)
                         tmem_cp_32x128b_warpx4(tb + TM_SFA + (t * C::KB + c) * 4, smem_desc(sbase + C::Q_OFF + t * C::PAGE + C::CODES + c * 512, 0, 128, SWZ_NONE));
@@ -658,58 +664,43 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 if ((k & 1) != grp) continue;
                 const int drafts = base - p * PKV_PAGE_TOKENS;
                 wait_all(&X->s_full[grp], (k >> 1) & 1, 41);
-                // The loops over a page's scores are not unrolled beyond 32 columns, and the scores are read from tensor memory twice:
-                // with everything unrolled the roles' code no longer fits the instruction cache together, and each of them runs
-                // at the speed of instruction fetch.
+                // Weights at the reference that the row had so far, the page's maximum on the way; once the page before has been
+                // decided upon, the reference is looked at again. It only moves when a page exceeds it by 2^8 (its column of O^T is
+                // then rescaled), so the weights are rarely formed a second time (a stretch's first page apart).
+                // The loop is not unrolled beyond 32 columns: the code of all roles has to fit the instruction cache together, or
+                // each of them runs at the speed of instruction fetch (unrolled over the 128 columns: 192 against 165 us).
                 const bool masked = drafts < PKV_PAGE_TOKENS || !mine;
                 const uint32_t s_tm = tl_s + TM_S + 128 * grp;
-                float x[32];
-                auto load = [&](int c) {                                // 32 tokens; those that the row does not see become -inf
-                    tmem_ld32(s_tm + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
-                    tmem_ld_wait();
-                    if (masked) {
-                        const int j0 = 32 * c - drafts;                 // drafted token of the first column (negative: cached)
-                        uint32_t see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
-                        if (!mine) see = 0u;
-#pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!(see >> e & 1)) x[e] = -INFINITY;
-                    }
-                };
-                tc_fence_after_sync();
-                float top = -INFINITY;
-                if (ok) {
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        load(c);
-                        float mx[4] = {top, x[0], x[1], x[2]};
-#pragma unroll
-                        for (int e = 3; e < 31; e += 2) mx[(e >> 1) & 3] = max3(mx[(e >> 1) & 3], x[e], x[e + 1]);
-                        top = max3(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]), x[31]);
-                    }
-                }
-                top *= cs;
-                // The reference of a row only moves when a page exceeds it by 2^8: its column of O^T is then rescaled.
-                float before = -INFINITY;
-                if (p > s.p_lo) {
-                    wait_all(&X->decided[quad], (k - 1) & 1, 42);
-                    before = X->row_m[r];
-                }
-                const bool grows = top > before + RESCALE_THRESHOLD;
-                const float ref = grows ? top : before;
-                if (grows || p == s.p_lo) X->row_m[r] = ref;
-                arrive_warp(&X->decided[quad]);
-                if (ref != m) { l *= exp2f(m - ref); m = ref; }         // (both -inf: equal)
-                const float mu = m > -INFINITY ? m : 0.0f;              // nothing seen yet: every weight is 2^-inf
-                const float2 cs2 = make_float2(cs, cs), mu2 = make_float2(-mu, -mu);
-                float2 sum = make_float2(0.0f, 0.0f);
+                float2 sum;
+                float ref = m, before = -INFINITY;
+                bool grows, again;
                 if constexpr (VQ) wait_all(&X->sc_full[grp], (k >> 1) & 1, 46);
                 if (k >= 2) wait_all(&X->pv_done[grp], ((k >> 1) - 1) & 1, 43);     // the weights of this group's page before have been read
-                if (ok) {
+                tc_fence_after_sync();
+#pragma unroll 1
+                for (bool first_try = true;; first_try = false) {
+                    const float mu = ref > -INFINITY ? ref : 0.0f;      // nothing seen yet: every weight is 2^-inf
+                    const float2 cs2 = make_float2(cs, cs), mu2 = make_float2(-mu, -mu);
+                    float top = -INFINITY;
+                    sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
                     for (int c = 0; c < 4; ++c) {
-                        load(c);
+                        float x[32];
                         uint32_t w[16];
+                        if (ok) tmem_ld32(s_tm + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
+                        tmem_ld_wait();
+                        if (masked) {                                   // tokens that the row does not see
+                            const int j0 = 32 * c - drafts;             // drafted token of the first column (negative: cached)
+                            uint32_t see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
+                            if (!mine) see = 0u;
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!(see >> e & 1)) x[e] = -INFINITY;
+                        }
+                        float mx[2] = {top, x[0]};
+#pragma unroll
+                        for (int e = 1; e < 31; e += 2) mx[(e >> 1) & 1] = max3(mx[(e >> 1) & 1], x[e], x[e + 1]);
+                        top = max3(mx[0], mx[1], x[31]);
                         if constexpr (VQ) {
                             // the weight of a token carries its value scale of this row's kv head (a masked one's may be anything)
                             const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + grp * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + c * 64);
@@ -726,8 +717,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                                 }
                             }
                         } else {
-                            // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so that
-                            // numerator and denominator agree
+                            // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so
+                            // that numerator and denominator agree
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 const float2 t = fma2(make_float2(x[2 * e], x[2 * e + 1]), cs2, mu2);
@@ -741,10 +732,24 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         for (int u = 0; u < 4; ++u)
                             *reinterpret_cast<uint4*>(line + ((((c & 1) * 4 + u) ^ (r & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                     }
+                    if (!first_try) break;
+                    top *= cs;
+                    if (p > s.p_lo) {
+                        wait_all(&X->decided[quad], (k - 1) & 1, 42);
+                        before = X->row_m[r];
+                    }
+                    grows = top > before + RESCALE_THRESHOLD;
+                    const float now = grows ? top : before;
+                    again = __any_sync(0xffffffffu, now != ref);
+                    ref = now;
+                    if (grows || p == s.p_lo) X->row_m[r] = ref;
+                    arrive_warp(&X->decided[quad]);
+                    if (!again) break;
                 }
                 tc_fence_before_sync();
                 arrive_warp(&X->s_empty[grp]);
                 if constexpr (VQ) arrive_warp(&X->sc_empty[grp]);
+                if (ref != m) { l *= exp2f(m - ref); m = ref; }         // (both -inf: equal)
                 l += sum.x + sum.y;
                 if (group_any(grp, grows || !ok)) {
                     if (group_any(grp, !ok)) { go = false; break; }     // (the same answer in all warps of the group)
