@@ -14,10 +14,11 @@
 // With few drafted tokens the V pages bound it (HBM), with many the score MMAs and the softmax.
 //
 // Three launches: the operand (absorbed queries), the attention, the merge of what several CTAs did of one tile.
-#include "pkv_absorb.cuh"
 #include "pkv_common.cuh"
 #include "pkv_tcgen05.cuh"
 
+#include <cuda_fp16.h>
+#include <cuda_fp4.h>
 #include <cudaTypedefs.h>
 #include <cstring>
 
@@ -57,11 +58,19 @@ struct Batch {
     }
 };
 
-// Work is a list of pages: sequence by sequence, `passes` times over its pages. Gang x of X takes the pages
-// [x U / X, (x + 1) U / X) of the U on the list, its CTA zi the tile pass * gang + zi: the tiles of a sequence read a page
-// at about the same time (from L2 all but the first), and every CTA streams as many pages whatever the lengths are.
-__device__ __forceinline__ long gang_start(long U, int gangs, int x) { return U * x / gangs; }
-__device__ __forceinline__ int gang_of(long U, int gangs, long u) { return (int)(((u + 1) * gangs - 1) / U); }
+// Work is a list of pages: sequence by sequence, `passes` times over its pages. It is cut into stretches of U / gangs pages (the
+// first U % gangs of them one longer), one per gang; the gang's CTA zi takes the tile pass * gang + zi of each page. So the
+// tiles of a sequence read a page at about the same time (from L2 all but the first), and every CTA streams as many pages
+// whatever the lengths are.
+struct Cut {
+    int per, longer;                                 // pages of a stretch; how many have one more
+    __device__ __forceinline__ Cut(int U, int gangs) : per(U / gangs), longer(U % gangs) {}
+    __device__ __forceinline__ int start(int x) const { return x * per + min(x, longer); }
+    __device__ __forceinline__ int of(int u) const {     // the stretch that page u of the list belongs to
+        const int head = longer * (per + 1);
+        return u < head ? u / (per + 1) : longer + (u - head) / per;
+    }
+};
 
 struct Part {                                        // a stretch of pages of one tile
     int b, z, p_lo, p_hi, pages, lo, n, T;
@@ -85,6 +94,42 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------------------------------------ operand
+// One residual term of 16 columns: E4M3 scale (in units of the row's `second`) and E2M1 codes; res becomes what is left. The
+// next term is formed from what was stored, so any rounding will do: hardware conversions and an approximate reciprocal.
+__device__ __forceinline__ uint2 residual_term(float (&res)[16], float second, float inv_second, uint8_t& sb, bool more) {
+    float am = fabsf(res[0]);
+#pragma unroll
+    for (int i = 1; i < 15; i += 2) asm("max.f32 %0, %1, %2, %3;" : "=f"(am) : "f"(am), "f"(fabsf(res[i])), "f"(fabsf(res[i + 1])));
+    am = fmaxf(am, fabsf(res[15]));
+    sb = pkv_float_to_e4m3(am * (1.0f / 6.0f) * inv_second);
+    const float scale = pkv_e4m3_to_float(sb) * second;
+    float inv;
+    asm("rcp.approx.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    if (sb == 0) inv = 0.0f;
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float* v = res + 8 * h;
+        asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+            "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
+            : "=r"(w[h]) : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+    }
+    if (more) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __half2_raw p = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(w[h] >> (8 * i)), __NV_E2M1);
+                const float2 f = __half22float2(__half2(p));
+                res[8 * h + 2 * i] = fmaf(-f.x, scale, res[8 * h + 2 * i]);
+                res[8 * h + 2 * i + 1] = fmaf(-f.y, scale, res[8 * h + 2 * i + 1]);
+            }
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
 // Tile operand of a (sequence, tile): four residual terms, each a 128-row tile laid out like a cache page (swizzled codes,
 // then the block scales), and 128 fp32 row scales.
 __host__ __device__ constexpr int page_bytes(int WP) { return PKV_PAGE_TOKENS * WP / 2 + WP / 64 * 512; }
@@ -98,6 +143,7 @@ struct AbsorbArgs {
     int q_bf16;
     const int32_t* positions;
     uint8_t* blobs;
+    int32_t* first_page;
     int32_t* status;
 };
 
@@ -112,11 +158,30 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     __shared__ float2 zq[AR][DH / 2];
     __shared__ float2 ph[AR][DH / 2];
     __shared__ float raw[AR][DH];
+    __shared__ int sums[NT / 32][2];
     __shared__ __align__(16) float qa[AR][WP + 4];
     const pkv_layer_t& L = A.L;
     const int tid = threadIdx.x, z = blockIdx.y, b = blockIdx.z, r0 = blockIdx.x * AR;
     pkv_grid_wait();                                 // everything before this launch is done ..
     pkv_grid_launch_dependents();                    // .. so the attention behind it may stream pages while this one still runs
+    if (blockIdx.x == 0 && z == 0) {                 // for the merge: this sequence's place on the list of pages (the last one's: all)
+        int before = 0, all = 0, lo, n, T;
+        for (int i = tid; i < A.B.batch; i += NT) {
+            const int p = A.B.pages(i, lo, n, T);
+            all += p;
+            if (i < b) before += p;
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        all = __reduce_add_sync(0xffffffffu, all);
+        if ((tid & 31) == 0) { sums[tid >> 5][0] = before; sums[tid >> 5][1] = all; }
+        __syncthreads();
+        if (tid == 0) {
+            before = all = 0;
+            for (int w = 0; w < NT / 32; ++w) { before += sums[w][0]; all += sums[w][1]; }
+            A.first_page[b] = before;
+            if (b == A.B.batch - 1) A.first_page[A.B.batch] = all;
+        }
+    }
     int lo, n, T;
     const int pages = A.B.pages(b, lo, n, T);
     if (pages == 0) {
@@ -141,6 +206,7 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     }
     // tiers: the cache's block is in units of its own scale while the attention applies the layer's one
     if (L.second_blocks_dev && c < W) tier = L.second_blocks_dev[c >> 4] / L.second;
+#pragma unroll 1
     for (int k = tid; k < rows * (DH / 4); k += NT) {
         const int r = k / (DH / 4), d = k % (DH / 4) * 4, rr = rr0 + r;
         const size_t o = ((size_t)(lo + first + rr / rep) * L.n_q + g * rep + rr % rep) * DH + d;
@@ -156,6 +222,7 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     }
     // Phasors: the angle as a number of turns in 64 bits, of which only the fraction counts; that is exact enough in 32 bits
     // (2^-25 of a turn) and needs no long range reduction (the operand's own residual is 7e-5).
+#pragma unroll 1
     for (int k = tid; k < (q_hi - q_lo + 1) * (DH / 2); k += NT) {
         const int j = k % (DH / 2);
         const double turns = (double)A.positions[lo + first + q_lo + k / (DH / 2)] * L.inv_freq_dev[j] * 0.15915494309189533577;
@@ -164,6 +231,7 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
         ph[k / (DH / 2)][j] = make_float2(L.attn_scale * cs, L.attn_scale * sn);
     }
     __syncthreads();
+#pragma unroll 1
     for (int k = tid; k < rows * (DH / 2); k += NT) {
         const int r = k / (DH / 2), j = k % (DH / 2);
         const float2 p = ph[(rr0 + r) / rep - q_lo][j];
@@ -209,7 +277,7 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
 #pragma unroll 1
     for (int t = 0; t < PKV_QUERY_TERMS; ++t) {
         uint8_t sb;
-        const uint2 packed = pkv_absorb_impl::quantize_query_block16(res, second, inv, sb);
+        const uint2 packed = residual_term(res, second, inv, sb, t + 1 < PKV_QUERY_TERMS);
         uint8_t* tile = blob + t * page_bytes(WP);
         *reinterpret_cast<uint2*>(tile + pkv_code_offset(row, j * 8, RB)) = packed;
         tile[PKV_PAGE_TOKENS * RB + pkv_scale_offset(row, j)] = sb;
@@ -242,7 +310,7 @@ struct Cfg {
     static constexpr int R_OFF = P_OFF + 2 * P_BYTES;                             // weights: a buffer per softmax group
     static constexpr int SC_OFF = R_OFF + NR * RAW_BYTES;
     static constexpr int X_OFF = SC_OFF + (VQ ? 2 * SC_BYTES : 0);
-    static constexpr int SMEM = X_OFF + 5120;
+    static constexpr int SMEM = X_OFF + 6144;
     static constexpr int NTHREADS = VQ ? 512 : 384;
     static constexpr uint64_t SWZ = RB == 128 ? SWZ_128B : SWZ_64B;
     static_assert(SMEM <= 232448 && V_OFF % 1024 == 0 && P_OFF % 1024 == 0, "shared memory of a CTA");
@@ -260,9 +328,10 @@ struct Shared {                       // at X_OFF
     float row_f[2][ROWS];             // per group: rescale factors, then 1 / sum
     float row_l[2][2][ROWS];          // [stretch & 1][group]: sums at the end
     uint32_t bad[3][MAX_G][2];        // [stretch % 3]: drafted tokens whose value row of a kv head is not finite
-    long scan[16];
+    int scan[16];
+    int row_o[2][ROWS];               // per group: where a row's result goes, or -1
 };
-static_assert(sizeof(Shared) <= 5120, "behind the stages");
+static_assert(sizeof(Shared) <= 6144, "behind the stages");
 
 __device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
     for (uint32_t i = 0; i < WAIT_LIMIT; ++i) {
@@ -333,6 +402,7 @@ struct AttnArgs {
     float col_scale;                  // tensor scale of the latent x log2(e) / sqrt(d)
     float* part_o;                    // [2 per CTA][128 rows][128 dims]
     float2* part_ml;                  // [2 per CTA][128 rows]
+    const int32_t* first_page;        // [batch + 1]: pages of the sequences before each one, and of all
     __nv_bfloat16* out;
     int32_t* status;
 };
@@ -340,7 +410,7 @@ struct AttnArgs {
 template <int WP, bool VQ>
 __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                                  const __grid_constant__ CUtensorMap qmap,
-                                                                                 const __grid_constant__ CUtensorMap vmap, const AttnArgs A) {
+                                                                                 const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnArgs A) {
     using C = Cfg<WP, VQ>;
     extern __shared__ __align__(1024) uint8_t smem[];
     Shared* X = reinterpret_cast<Shared*>(smem + C::X_OFF);
@@ -351,19 +421,22 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
 
     // ---- barriers, tensor memory, and where on the list of pages this CTA starts. Page table, lengths, masks and pages are
     // final: the operand launch in front of this one has started, so everything before that is done.
-    if (tid == 0) {
-        mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 2 * GROUP_WARPS + 1);
-        mbar_init(&X->o_empty, 2 * GROUP_WARPS); mbar_init(&X->meet, 2 * GROUP_WARPS);
-        for (int i = 0; i < GROUP_WARPS; ++i) mbar_init(&X->decided[i], 1);
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&X->p_full[i], GROUP_WARPS); mbar_init(&X->pv_done[i], 1); mbar_init(&X->s_full[i], 1); mbar_init(&X->s_empty[i], GROUP_WARPS);
-            mbar_init(&X->sc_full[i], 1); mbar_init(&X->sc_empty[i], GROUP_WARPS);
+    // (Code that runs once per CTA costs what its bytes take to fetch: it is kept short, loops are left rolled.)
+    if (warp == 0) {                                 // lane i takes entry i of every array
+        if (lane == 0) {
+            mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 2 * GROUP_WARPS + 1);
+            mbar_init(&X->o_empty, 2 * GROUP_WARPS); mbar_init(&X->meet, 2 * GROUP_WARPS);
+            X->abort_flag = 0;
+            X->start = Walk{0, 0, 0, 0};
         }
-        for (int i = 0; i < C::NK; ++i) { mbar_init(&X->k_full[i], 1); mbar_init(&X->k_empty[i], 1); }
-        for (int i = 0; i < C::NV; ++i) { mbar_init(&X->v_full[i], VQ ? 4 : 1); mbar_init(&X->v_empty[i], 1); mbar_init(&X->v_clean[i], GROUP_WARPS); }
-        for (int i = 0; i < C::NR; ++i) { mbar_init(&X->r_full[i], 1); mbar_init(&X->r_empty[i], 4); }
-        X->abort_flag = 0;
-        X->start = Walk{0, 0, 0, 0};
+        if (lane < GROUP_WARPS) mbar_init(&X->decided[lane], 1);
+        if (lane < 2) {
+            mbar_init(&X->p_full[lane], GROUP_WARPS); mbar_init(&X->pv_done[lane], 1); mbar_init(&X->s_full[lane], 1); mbar_init(&X->s_empty[lane], GROUP_WARPS);
+            mbar_init(&X->sc_full[lane], 1); mbar_init(&X->sc_empty[lane], GROUP_WARPS);
+        }
+        if (lane < C::NK) { mbar_init(&X->k_full[lane], 1); mbar_init(&X->k_empty[lane], 1); }
+        if (lane < C::NV) { mbar_init(&X->v_full[lane], VQ ? 4 : 1); mbar_init(&X->v_empty[lane], 1); mbar_init(&X->v_clean[lane], GROUP_WARPS); }
+        if (lane < C::NR) { mbar_init(&X->r_full[lane], 1); mbar_init(&X->r_empty[lane], 4); }
         fence_barrier_init();
     }
     if (tid < 3 * MAX_G * 2) (&X->bad[0][0][0])[tid] = 0u;
@@ -371,35 +444,39 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     tc_fence_before_sync();
     {
         const int per = (A.B.batch + C::NTHREADS - 1) / C::NTHREADS, b_lo = min(tid * per, A.B.batch), b_hi = min(b_lo + per, A.B.batch);
-        long mine = 0;
-        int lo, n, T;
+        int mine = 0, lo, n, T;
+#pragma unroll 1
         for (int b = b_lo; b < b_hi; ++b) mine += A.B.pages(b, lo, n, T);
-        long incl = mine;
-#pragma unroll
+        int incl = mine;
+#pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-            const long y = __shfl_up_sync(0xffffffffu, incl, o);
+            const int y = __shfl_up_sync(0xffffffffu, incl, o);
             if (lane >= o) incl += y;
         }
         if (lane == 31) X->scan[warp] = incl;
         __syncthreads();
-        long before = incl - mine, U = 0;
+        int before = incl - mine, U = 0;
+#pragma unroll 1
         for (int w = 0; w < C::NTHREADS / 32; ++w) {
             if (w < warp) before += X->scan[w];
             U += X->scan[w];
         }
         U *= tl.passes;
-        const int gangs = (int)min((long)tl.gangs, U);
+        before *= tl.passes;
+        const int gangs = min(tl.gangs, U);
         if (gang < gangs) {
-            const long u0 = gang_start(U, gangs, gang), u1 = gang_start(U, gangs, gang + 1);
-            if (mine > 0 && before * tl.passes <= u0 && u0 < (before + mine) * tl.passes) {
-                long u = u0 - before * tl.passes;
+            const Cut cut(U, gangs);
+            const int u0 = cut.start(gang);
+            if (mine > 0 && before <= u0 && u0 < before + mine * tl.passes) {
+                int u = u0 - before;
+#pragma unroll 1
                 for (int b = b_lo; b < b_hi; ++b) {
                     const int pages = A.B.pages(b, lo, n, T);
-                    if (u < (long)pages * tl.passes) {
-                        X->start = Walk{b, (int)(u / pages), (int)(u % pages), (int)(u1 - u0)};
+                    if (u < pages * tl.passes) {
+                        X->start = Walk{b, u / pages, u % pages, cut.start(gang + 1) - u0};
                         break;
                     }
-                    u -= (long)pages * tl.passes;
+                    u -= pages * tl.passes;
                 }
             }
         }
@@ -826,32 +903,27 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             const size_t slot = (size_t)blockIdx.x * 2 + (s.p_lo == 0);
             l = X->row_l[seg & 1][0][r] + X->row_l[seg & 1][1][r];
             if (!VQ && mine && ((word & 0xffffffffu & X->bad[seg % 3][gl][0]) | ((word >> 32) & X->bad[seg % 3][gl][1]))) l = __int_as_float(0x7fc00000);
-            X->row_f[grp][r] = l == 0.0f ? 0.0f : 1.0f / l;         // a row that sees nothing: zeros
+            X->row_f[grp][r] = l == 0.0f ? 0.0f : 1.0f / l;             // a row that sees nothing: zeros
+            X->row_o[grp][r] = mine ? (s.lo + first + rr / tl.rep) * A.n_q + (s.z % tl.groups * tl.G + gl) * tl.rep + rr % tl.rep : -1;
             if (!whole && mine && grp == 0) A.part_ml[slot * ROWS + r] = make_float2(M, l);
             group_sync(grp);
+            // (four columns at a time in a rolled loop: this thread's dim is r)
 #pragma unroll 1
-            for (int g = 0; g < ng; ++g) {
-#pragma unroll 1
-                for (int c0 = 16 * grp; c0 < nq * tl.rep; c0 += 32) {
-                    uint32_t o[16];
-                    tmem_ld16(tl_s + TM_O + g * tl.rph + c0, o);
-                    tmem_ld_wait();
+            for (int c0 = 64 * grp; c0 < min(ng * tl.rph, 64 * grp + 64); c0 += 4) {
+                uint32_t o[4];
+                tmem_ldn<4>(tl_s + TM_O + c0, o);
+                tmem_ld_wait();
 #pragma unroll
-                    for (int c = 0; c < 16; ++c) {
-                        const int q = c0 + c;                           // row of the kv head; this thread's dim is r
-                        if (q >= nq * tl.rep) break;
-                        if (whole) {
-                            const size_t row = (size_t)(s.lo + first + q / tl.rep) * A.n_q + (s.z % tl.groups * tl.G + g) * tl.rep + q % tl.rep;
-                            A.out[row * DH + r] = __float2bfloat16(__uint_as_float(o[c]) * X->row_f[grp][g * tl.rph + q]);
-                        } else {
-                            A.part_o[(slot * ROWS + g * tl.rph + q) * DH + r] = __uint_as_float(o[c]);
-                        }
-                    }
+                for (int c = 0; c < 4; ++c) {
+                    const int to = X->row_o[grp][c0 + c];
+                    if (to < 0) continue;
+                    if (whole) A.out[(size_t)to * DH + r] = __float2bfloat16(__uint_as_float(o[c]) * X->row_f[grp][c0 + c]);
+                    else A.part_o[(slot * ROWS + c0 + c) * DH + r] = __uint_as_float(o[c]);
                 }
             }
             tc_fence_before_sync();
             arrive_warp(&X->o_empty);
-            group_sync(grp);                                            // row_f is free again
+            group_sync(grp);                                            // row_f, row_o are free again
             ++seg;
         }
     }
@@ -865,78 +937,57 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-// O = sum 2^(m - M) o / sum 2^(m - M) l over the stretches of a tile that several CTAs did. CTA: 8 / WPR rows of a tile,
-// WPR warps per row; a lane holds four dims.
-struct MergeArgs {
-    Batch B;
-    Tiles X;
-    int n_kv, n_q;
-    const float* part_o;
-    const float2* part_ml;
-    __nv_bfloat16* out;
-};
-
+// O = sum 2^(m - M) o / sum 2^(m - M) l over the stretches of a tile that several gangs had. WPR warps per row, a lane holds four
+// dims; the references, sums and outputs of eight stretches are asked for together (two round trips in all, the first
+// for the lengths).
 template <int WPR>
-__global__ void __launch_bounds__(256) pkv_tree_merge_kernel(const MergeArgs A) {
-    __shared__ long sums[8][2];
+__global__ void __launch_bounds__(256) pkv_tree_merge_kernel(const AttnArgs A) {
     __shared__ float4 acc_s[8][32];
     __shared__ float2 ml_s[8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, z = blockIdx.y, b = blockIdx.z;
     const int r = blockIdx.x * (8 / WPR) + warp / WPR, w0 = warp % WPR;
+    const Tiles& X = A.X;
+    const int gl = r / X.rph, rr = r % X.rph, g = z % X.groups * X.G + gl, first = z / X.groups * X.qpb;
     pkv_grid_launch_dependents();
     pkv_grid_wait();
     int lo, n, T;
-    const int pages = A.B.pages(b, lo, n, T);
-    const Tiles& X = A.X;
-    const int first = z / X.groups * X.qpb, nq = min(X.qpb, n - first);
-    if (pages == 0 || nq <= 0) return;
-    long before = 0, total = 0;
-    for (int i = tid; i < A.B.batch; i += 256) {
-        int lo2, n2, T2;
-        const int p = A.B.pages(i, lo2, n2, T2);
-        total += p;
-        if (i < b) before += p;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        before += __shfl_xor_sync(0xffffffffu, before, o);
-        total += __shfl_xor_sync(0xffffffffu, total, o);
-    }
-    if (lane == 0) { sums[warp][0] = before; sums[warp][1] = total; }
-    __syncthreads();
-    before = total = 0;
-    for (int w = 0; w < 8; ++w) { before += sums[w][0]; total += sums[w][1]; }
-    const long U = total * X.passes, u0 = before * X.passes + (long)(z / X.gang) * pages;
-    const int gangs = (int)min((long)X.gangs, U), x0 = gang_of(U, gangs, u0), x1 = gang_of(U, gangs, u0 + pages - 1);
+    const int pages = A.B.pages(b, lo, n, T), U = A.first_page[A.B.batch] * X.passes, u0 = A.first_page[b] * X.passes + z / X.gang * pages;
+    if (pages == 0) return;
+    const Cut cut(U, min(X.gangs, U));
+    const int x0 = cut.of(u0), x1 = cut.of(u0 + pages - 1);
     if (x0 == x1) return;                            // one CTA did the whole tile and has written it
-    const int gl = r / X.rph, rr = r % X.rph, g = z % X.groups * X.G + gl;
-    const bool live = gl < X.G && g < A.n_kv && rr < nq * X.rep;
-    auto slot = [&](int x) { return ((size_t)(x * X.gang + z % X.gang) * 2 + (x == x0)) * ROWS + r; };
+    const bool live = gl < X.G && g < A.n_kv && rr < min(X.qpb, n - first) * X.rep;
     float M = -INFINITY, l = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (live) {
-        for (int x = x0 + lane; x <= x1; x += 32) M = fmaxf(M, A.part_ml[slot(x)].x);
-#pragma unroll
-        for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
         constexpr int DEEP = 8;
+#pragma unroll 1
         for (int xb = x0 + w0; xb <= x1; xb += WPR * DEEP) {
             float4 o[DEEP];
             float2 ml[DEEP];
 #pragma unroll
             for (int k = 0; k < DEEP; ++k) {
                 const int x = xb + k * WPR;
-                ml[k] = x <= x1 ? A.part_ml[slot(x)] : make_float2(-INFINITY, 0.0f);
-                o[k] = x <= x1 ? *reinterpret_cast<const float4*>(A.part_o + slot(x) * DH + lane * 4) : acc;
+                const size_t slot = ((size_t)(x * X.gang + z % X.gang) * 2 + (x == x0)) * ROWS + r;
+                ml[k] = x <= x1 ? A.part_ml[slot] : make_float2(-INFINITY, 0.0f);
+                if (x <= x1) o[k] = reinterpret_cast<const float4*>(A.part_o + slot * DH)[lane];
             }
+            float top = M;
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k) top = fmaxf(top, ml[k].x);
+            const float f0 = M > -INFINITY ? exp2f(M - top) : 1.0f;
+            acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
+            l *= f0;
+            M = top;
 #pragma unroll
             for (int k = 0; k < DEEP; ++k) {
-                if (ml[k].x > -INFINITY) {
+                if (ml[k].x > -INFINITY) {               // (a stretch that saw nothing of the row holds zeros)
                     const float f = exp2f(ml[k].x - M);
                     l = fmaf(ml[k].y, f, l);
                     acc.x = fmaf(o[k].x, f, acc.x); acc.y = fmaf(o[k].y, f, acc.y);
                     acc.z = fmaf(o[k].z, f, acc.z); acc.w = fmaf(o[k].w, f, acc.w);
                 } else {
-                    l += ml[k].y;                    // 0, or NaN
+                    l += ml[k].y;                        // 0, or NaN
                 }
             }
         }
@@ -946,12 +997,20 @@ __global__ void __launch_bounds__(256) pkv_tree_merge_kernel(const MergeArgs A) 
         if (lane == 0) ml_s[warp] = make_float2(M, l);
         __syncthreads();
         if (w0 != 0) return;
-#pragma unroll
-        for (int w = 1; w < WPR; ++w) {
+        float top = M;
+#pragma unroll 1
+        for (int w = 1; w < WPR; ++w) top = fmaxf(top, ml_s[warp + w].x);
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        l = 0.0f;
+#pragma unroll 1
+        for (int w = 0; w < WPR; ++w) {
+            const float2 ml = ml_s[warp + w];
+            const float f = ml.x > -INFINITY ? exp2f(ml.x - top) : 1.0f;      // (nothing there: zeros, or NaN)
             const float4 o = acc_s[warp + w][lane];
-            acc.x += o.x; acc.y += o.y; acc.z += o.z; acc.w += o.w;
-            l += ml_s[warp + w].y;
+            sum.x = fmaf(o.x, f, sum.x); sum.y = fmaf(o.y, f, sum.y); sum.z = fmaf(o.z, f, sum.z); sum.w = fmaf(o.w, f, sum.w);
+            l = fmaf(ml.y, f, l);
         }
+        acc = sum;
     }
     if (!live) return;
     const float f = l == 0.0f ? 0.0f : 1.0f / l;
@@ -1007,7 +1066,7 @@ Tiles make_tiles(int n_q, int n_kv, int max_draft) {
     return X;
 }
 
-struct Layout { size_t blobs, part_o, part_ml, total; };
+struct Layout { size_t blobs, part_o, part_ml, first_page, total; };
 
 Layout make_layout(const Tiles& X, int batch, int WP) {
     Layout y;
@@ -1015,12 +1074,13 @@ Layout make_layout(const Tiles& X, int batch, int WP) {
     y.blobs = 0;
     y.part_o = ((size_t)batch * X.Z * blob_bytes(WP) + 1023) / 1024 * 1024;
     y.part_ml = y.part_o + ctas * 2 * ROWS * DH * 4;
-    y.total = y.part_ml + ctas * 2 * ROWS * 8;
+    y.first_page = y.part_ml + ctas * 2 * ROWS * 8;
+    y.total = y.first_page + ((size_t)batch + 1) * 4;
     return y;
 }
 
 template <int WP, bool VQ>
-int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, AttnArgs& at, const MergeArgs& mg, size_t blob_rows, cudaStream_t st) {
+int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, const AttnArgs& at, size_t blob_rows, cudaStream_t st) {
     using C = Cfg<WP, VQ>;
     const Tiles& X = ab.X;
     CUtensorMap kmap, qmap, vmap;
@@ -1035,10 +1095,9 @@ int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, AttnArgs& at, const M
     PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ>, dim3(X.gangs * X.gang), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
     // parts of a tile: about one per CTA and tile; a warp takes some eight of them
     const int parts = X.gangs / (ab.B.batch * X.passes) + 1;
-    const dim3 grid(ROWS / 8, X.Z, ab.B.batch), block(256);
-    if (parts <= 8) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1>, grid, block, 0, st, mg));
-    else if (parts <= 16) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<2>, dim3(ROWS / 4, X.Z, ab.B.batch), block, 0, st, mg));
-    else PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<8>, dim3(ROWS, X.Z, ab.B.batch), block, 0, st, mg));
+    if (parts <= 8) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1>, dim3(ROWS / 8, X.Z, ab.B.batch), dim3(256), 0, st, at));
+    else if (parts <= 16) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<2>, dim3(ROWS / 4, X.Z, ab.B.batch), dim3(256), 0, st, at));
+    else PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<8>, dim3(ROWS, X.Z, ab.B.batch), dim3(256), 0, st, at));
     return PKV_OK;
 }
 
@@ -1079,21 +1138,21 @@ extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache,
     const Tiles X = make_tiles(layer->n_q, layer->n_kv, max_draft);
     const Layout y = make_layout(X, pages->batch, WP);
     const size_t blob_rows = (size_t)pages->batch * X.Z * (blob_bytes(WP) / 128);
-    if (blob_rows > 0x7fffffff || X.Z > 65535) return PKV_ERR_UNSUPPORTED;
+    if (blob_rows > 0x7fffffff || X.Z > 65535 || (int64_t)pages->batch * pages->max_pages * X.passes > 0x3fffffff) return PKV_ERR_UNSUPPORTED;
+    if ((int64_t)n_tokens * layer->n_q > 0x7fffffff) return PKV_ERR_UNSUPPORTED;      // rows of the result are 31 bits
     if (!workspace_dev || (((uintptr_t)workspace_dev) & 1023u) || workspace_bytes < (int64_t)y.total) return PKV_ERR_INVALID;
     st = init_encoder();
     if (st) return st;
     uint8_t* ws = (uint8_t*)workspace_dev;
     const Batch B{cu_dev, pages->seqlens_dev, pages->batch, pages->max_pages, n_tokens, max_draft};
-    const AbsorbArgs ab{*layer, B, X, q_dev, q_dtype == PKV_BF16, positions_dev, ws, status_dev};
+    const AbsorbArgs ab{*layer, B, X, q_dev, q_dtype == PKV_BF16, positions_dev, ws, (int32_t*)(ws + y.first_page), status_dev};
     AttnArgs at;
     at.B = B; at.X = X; at.page_table = pages->page_table_dev; at.mask = mask_dev; at.blobs = ws; at.vq = (const uint8_t*)cache->vq_dev;
     at.n_pages = cache->n_pages; at.n_kv = layer->n_kv; at.n_q = layer->n_q;
     at.col_scale = layer->second * PKV_LOG2E / sqrtf((float)DH);
-    at.part_o = (float*)(ws + y.part_o); at.part_ml = (float2*)(ws + y.part_ml);
+    at.part_o = (float*)(ws + y.part_o); at.part_ml = (float2*)(ws + y.part_ml); at.first_page = (int32_t*)(ws + y.first_page);
     at.out = (__nv_bfloat16*)out_dev; at.status = status_dev;
-    const MergeArgs mg{B, X, layer->n_kv, layer->n_q, at.part_o, at.part_ml, at.out};
     cudaStream_t s = (cudaStream_t)stream;
-    if (cache->v_bits) return WP == 256 ? launch<256, true>(cache, ab, at, mg, blob_rows, s) : launch<128, true>(cache, ab, at, mg, blob_rows, s);
-    return WP == 256 ? launch<256, false>(cache, ab, at, mg, blob_rows, s) : launch<128, false>(cache, ab, at, mg, blob_rows, s);
+    if (cache->v_bits) return WP == 256 ? launch<256, true>(cache, ab, at, blob_rows, s) : launch<128, true>(cache, ab, at, blob_rows, s);
+    return WP == 256 ? launch<256, false>(cache, ab, at, blob_rows, s) : launch<128, false>(cache, ab, at, blob_rows, s);
 }
