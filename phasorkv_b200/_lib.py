@@ -119,7 +119,7 @@ SIGNATURES = {
     "pkv_vq_read": (c_int32, [POINTER(Cache), c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]),
     "pkv_plan_step": (c_int32, [POINTER(Pages), c_void_p, c_void_p, POINTER(Plan), c_void_p]),
     "pkv_truncate": (c_int32, [POINTER(Pages), c_void_p, c_void_p, c_void_p]),
-    "pkv_keep_rows": (c_int32, [POINTER(POINTER(Cache)), c_int32, POINTER(Pages), c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
+    "pkv_keep_rows": (c_int32, [POINTER(c_void_p), c_int32, POINTER(Pages), c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
                                 c_void_p, c_void_p]),
     "pkv_tree_workspace_bytes": (c_int64, [POINTER(Layer), c_int32, c_int32, c_int32]),
     "pkv_tree_attn": (c_int32, [POINTER(Layer), POINTER(Cache), POINTER(Pages), c_void_p, c_int32, c_void_p, c_void_p, c_void_p,
@@ -166,17 +166,28 @@ def current_stream() -> c_void_p:
 
 def need(t, dtype, shape, device, what: str) -> None:
     """Refuses a tensor that a kernel would misread: another type, shape, device or order."""
-    if t.dtype is not dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous() or t.device.type != device.type or \
-            (device.index is not None and t.device.index != device.index):
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, "
                          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def on_device(device):
-    """Context in which `device` is the current one (nothing to do when it is already)."""
-    import contextlib
+class on_device:
+    """``with on_device(d) as stream``: `d` is the current device inside, `stream` its current stream as an integer. The calls of a
+    step cost the host more than the GPU, so this does without torch's stream and guard objects."""
+    __slots__ = ("index", "before")
 
-    import torch
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        import torch
+        self.before = torch._C._cuda_getDevice()
+        if self.before != self.index:
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.before != self.index:
+            import torch
+            torch._C._cuda_setDevice(self.before)
+        return False

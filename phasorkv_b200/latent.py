@@ -72,6 +72,7 @@ class PagedLatentCache:
         self.status = None                                  # status words of truncate / keep_rows, made with the first plan
         self.c = _lib.Cache(self.latent.data_ptr(), 0 if self.v is None else self.v.data_ptr(), self.n_pages, W,
                             n_kv, head_dim, 0 if self.vq is None else self.vq.data_ptr(), self.v_bits)
+        self.at = ctypes.addressof(self.c)                  # of the C struct
 
     def slots(self, seq: torch.Tensor, local_pos: torch.Tensor) -> torch.Tensor:
         """Slot (page * 128 + row) of token `local_pos` of sequence `seq`; int32 tensors on the device."""
@@ -119,19 +120,20 @@ class PagedLatentCache:
             if plan.mask is None:
                 raise ValueError("parents need a plan with masks: step_plan(capacity, tree=True)")
         plan._match(self)
-        pg = self._pages()
-        with _lib.on_device(self.latent.device):
-            _lib.check(_lib.load().pkv_plan_step(ctypes.byref(pg), _lib.ptr(n_new), _lib.ptr(parents), ctypes.byref(plan.c),
-                                                 _lib.current_stream()), "pkv_plan_step")
+        with _lib.on_device(self.latent.device) as stream:
+            st = _lib.load().pkv_plan_step(ctypes.byref(self._pages()), n_new.data_ptr(), None if parents is None else parents.data_ptr(),
+                                           plan.ref, stream)
+        if st:
+            _lib.check(st, "pkv_plan_step")
 
     def truncate(self, lengths: torch.Tensor) -> None:
         """At most ``lengths[b]`` (int32 [batch], on the device) tokens of every sequence stay; whole pages behind them go back
         to the pool. Negative lengths are refused (nothing changes, ``status[0]`` = 4)."""
         _lib.need(lengths, torch.int32, (self.batch,), self.latent.device, "lengths")
-        pg = self._pages()
-        with _lib.on_device(self.latent.device):
-            _lib.check(_lib.load().pkv_truncate(ctypes.byref(pg), _lib.ptr(lengths), _lib.ptr(self._status()), _lib.current_stream()),
-                       "pkv_truncate")
+        with _lib.on_device(self.latent.device) as stream:
+            st = _lib.load().pkv_truncate(ctypes.byref(self._pages()), lengths.data_ptr(), self._status().data_ptr(), stream)
+        if st:
+            _lib.check(st, "pkv_truncate")
 
     def keep_rows(self, plan: "StepPlan", keep: torch.Tensor, n_keep: torch.Tensor, lengths: Optional[torch.Tensor] = None,
                   layers: Optional[Sequence["PagedLatentCache"]] = None) -> None:
@@ -145,14 +147,14 @@ class PagedLatentCache:
             _lib.need(lengths, torch.int32, (self.batch,), self.latent.device, "lengths")
         plan._match(self)
         layers = [self] if layers is None else list(layers)
-        if any(c.page_table.data_ptr() != self.page_table.data_ptr() for c in layers):
+        if any(c.page_table is not self.page_table for c in layers):
             raise ValueError("layers must share this cache's page table (share_pages)")
-        pg = self._pages()
-        arr = (ctypes.POINTER(_lib.Cache) * len(layers))(*[ctypes.pointer(c.c) for c in layers])
-        with _lib.on_device(self.latent.device):
-            _lib.check(_lib.load().pkv_keep_rows(arr, len(layers), ctypes.byref(pg), _lib.ptr(plan.cu), plan.capacity, _lib.ptr(keep),
-                                                 _lib.ptr(n_keep), _lib.ptr(lengths), _lib.ptr(self._status()), _lib.current_stream()),
-                       "pkv_keep_rows")
+        arr = (ctypes.c_void_p * len(layers))(*[c.at for c in layers])
+        with _lib.on_device(self.latent.device) as stream:
+            st = _lib.load().pkv_keep_rows(arr, len(layers), ctypes.byref(self._pages()), plan.c.cu_dev, plan.capacity, keep.data_ptr(),
+                                           n_keep.data_ptr(), None if lengths is None else lengths.data_ptr(), self._status().data_ptr(), stream)
+        if st:
+            _lib.check(st, "pkv_keep_rows")
 
     def v_rows(self, slots: torch.Tensor) -> torch.Tensor:
         """Value rows [n, n_kv, head_dim] stored at `slots` (page * 128 + row); quantised pages: dequantised fp32."""
@@ -227,14 +229,16 @@ class StepPlan:
     def __init__(self, batch: int, capacity: int, tree: bool, device):
         if capacity < 0:
             raise ValueError("capacity must not be negative")
-        self.batch, self.capacity, self.device = batch, capacity, torch.device(device)
+        self.batch, self.capacity = batch, capacity
         z = lambda n, dt: torch.zeros(n, dtype=dt, device=device)
         self.cu = z(batch + 1, torch.int32)
+        self.device = self.cu.device
         self.seq, self.positions, self.slots = z(capacity, torch.int32), z(capacity, torch.int32), z(capacity, torch.int32)
         self.mask = z(capacity, torch.int64) if tree else None
         self.ticket, self.status = z(1, torch.int32), z(4, torch.int32)
         self.c = _lib.Plan(self.cu.data_ptr(), self.seq.data_ptr(), self.positions.data_ptr(), self.slots.data_ptr(),
                            0 if self.mask is None else self.mask.data_ptr(), self.ticket.data_ptr(), self.status.data_ptr(), capacity)
+        self.ref = ctypes.byref(self.c)
 
     def _match(self, cache: "PagedLatentCache") -> None:
         if self.batch != cache.batch or self.device != cache.latent.device:
@@ -278,6 +282,7 @@ class TreeWorkspace:
             _lib.check(n, "pkv_tree_workspace_bytes")
         self.buffer = _aligned_bytes(n, pk.device)
         self.status = torch.zeros(4, dtype=torch.int32, device=pk.device)
+        self.at, self.bytes, self.status_at = self.buffer.data_ptr(), n, self.status.data_ptr()
 
 
 class PhasorKey:
@@ -702,13 +707,12 @@ class PhasorKey:
         plan._match(cache)
         if n > plan.capacity or n > ws.capacity or ws.batch != cache.batch or ws.max_pages < cache.max_pages or ws.key != self._tree_key():
             raise ValueError("q has more rows than the plan or the workspace, or the workspace was made for another layer shape or cache")
-        pg = cache._pages()
-        L = self._layer()
-        with _lib.on_device(dev):
-            _lib.check(_lib.load().pkv_tree_attn(ctypes.byref(L), ctypes.byref(cache.c), ctypes.byref(pg), _lib.ptr(q), self._xdt(q),
-                                                 _lib.ptr(plan.positions), _lib.ptr(plan.mask), _lib.ptr(plan.cu), n, ws.max_draft,
-                                                 _lib.ptr(ws.buffer), ws.buffer.numel(), _lib.ptr(out), _lib.ptr(ws.status),
-                                                 _lib.current_stream()), "pkv_tree_attn")
+        with _lib.on_device(dev) as stream:
+            st = _lib.load().pkv_tree_attn(ctypes.byref(self._layer()), ctypes.byref(cache.c), ctypes.byref(cache._pages()), q.data_ptr(),
+                                           self._xdt(q), plan.c.positions_dev, plan.c.mask_dev, plan.c.cu_dev, n, ws.max_draft, ws.at, ws.bytes,
+                                           out.data_ptr(), ws.status_at, stream)
+        if st:
+            _lib.check(st, "pkv_tree_attn")
         return out
 
     def _tree_key(self):

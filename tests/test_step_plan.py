@@ -93,7 +93,7 @@ def test_c_entries_refuse_bad_arguments(lib):
     assert lib.pkv_truncate(pg(), None, None, None) == -1
     assert lib.pkv_truncate(pg(), 8192, None, None) == -1                              # the lengths themselves
     cache = _lib.Cache(4096, 4096, 8, 256, 8, 128)
-    layers = lambda *c: (ctypes.POINTER(_lib.Cache) * len(c))(*[ctypes.pointer(x) for x in c])
+    layers = lambda *c: (ctypes.c_void_p * len(c))(*[ctypes.addressof(x) for x in c])
     keep = lambda arr, n, p=None, cap=4, out=None: lib.pkv_keep_rows(arr, n, p or pg(), 1024, cap, 1024, 1024, out, None, None)
     assert keep(None, 1) == -1 and keep(layers(cache), 0) == -1 and keep(layers(cache), 1, cap=-1) == -1
     assert keep(layers(cache), 1, out=8192) == -1
