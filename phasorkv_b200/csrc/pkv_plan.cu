@@ -204,9 +204,9 @@ __global__ void __launch_bounds__(NT) pkv_truncate_kernel(const pkv_pages_t pg, 
 }
 
 // ------------------------------------------------------------------------------------------------ accepted rows
-constexpr int KT = 128;                              // threads of a CTA, one column unit of a row each
+constexpr int KC = 32, KR = 8, KT = KC * KR;         // threads of a CTA: column units of a row x groups of rows
 constexpr int MAX_LAYERS = 48;                       // layers per launch (their pools are kernel arguments)
-constexpr int DEEP = 16;                             // rows in flight per thread
+constexpr int DEEP = PKV_TREE_MAX / KR;              // rows per thread, all in flight
 
 struct KeepLayer {
     uint8_t* latent;
@@ -227,35 +227,8 @@ __host__ __device__ inline int keep_units(int W, int n_kv, int head_dim, int v_b
     return lat + (!with_v ? 0 : v_bits ? n_kv * 5 : n_kv * (head_dim / 8));
 }
 
-template <typename T>
-__device__ __forceinline__ void move_rows(const int2* moves, int n, uint8_t* pool, size_t page_bytes, int unit, int RB, int kind, int g,
-                                          int head_dim, int n_kv) {
-    // byte offset of this thread's unit inside the page, for a row
-    auto at = [&](int slot) -> T* {
-        const uint32_t r = slot % PKV_PAGE_TOKENS;
-        uint32_t o;
-        if (kind == 0) o = pkv_code_offset(r, unit * 16, RB);                                   // codes of the latent
-        else if (kind == 1) o = PKV_PAGE_TOKENS * RB + pkv_scale_offset(r, unit * 4);           // four block scales
-        else if (kind == 2) o = ((uint32_t)g * PKV_PAGE_TOKENS + r) * head_dim * 2 + unit * 16; // bf16 values
-        else if (kind == 3) o = (uint32_t)g * 8192 + r * 64 + ((unit ^ ((r >> 1) & 3u)) << 4);  // value codes
-        else o = (uint32_t)n_kv * 8192 + g * 256 + r * 2;                                       // their scale
-        return reinterpret_cast<T*>(pool + (size_t)(slot / PKV_PAGE_TOKENS) * page_bytes + o);
-    };
-    // Indices ascend, so a row's target lies at or before its source and before every later source: groups of rows in
-    // order, the loads of a group before its stores, never overwrite a row that is still to be read.
-    for (int j0 = 0; j0 < n; j0 += DEEP) {
-        T val[DEEP];
-#pragma unroll
-        for (int k = 0; k < DEEP; ++k)
-            if (j0 + k < n) val[k] = *at(moves[j0 + k].x);
-#pragma unroll
-        for (int k = 0; k < DEEP; ++k)
-            if (j0 + k < n) *at(moves[j0 + k].y) = val[k];
-    }
-}
-
-// CTA (column units, sequence, layer). A thread owns one 16-byte (or smaller) column unit of the row and moves it for
-// every kept row: no two threads touch the same bytes, no barrier is needed between reading and writing.
+// CTA (32 column units, sequence, layer); a unit is 16 bytes of a row (or the few bytes of its scales). All rows of the units are
+// read before any is written: a row's target is another one's source.
 __global__ void __launch_bounds__(KT) pkv_keep_rows_kernel(const KeepArgs A) {
     __shared__ int2 moves[PKV_TREE_MAX];
     __shared__ int n_moves;
@@ -286,22 +259,53 @@ __global__ void __launch_bounds__(KT) pkv_keep_rows_kernel(const KeepArgs A) {
     }
     if (refused || n_moves == 0) return;
     const int RB = pkv_row_bytes(Y.W), nc = RB / 16, ns = pkv_padded_width(Y.W) / 64;
-    int u = blockIdx.x * KT + tid;
+    int u = blockIdx.x * KC + tid % KC, size = 16, g = 0;
+    // what unit u is: codes of the latent, four of its block scales, bf16 values, value codes, or a value scale
+    int kind = 5;
+    uint8_t* pool = Y.latent;
+    size_t page_bytes = pkv_page_bytes(Y.W);
     if (u < nc) {
-        move_rows<uint4>(moves, n_moves, Y.latent, pkv_page_bytes(Y.W), u, RB, 0, 0, 0, 0);
+        kind = 0;
     } else if ((u -= nc) < ns) {
-        move_rows<uint32_t>(moves, n_moves, Y.latent, pkv_page_bytes(Y.W), u, RB, 1, 0, 0, 0);
+        kind = 1; size = 4;
     } else if (Y.v) {
         u -= ns;
-        if (!Y.v_bits) {
-            const int per = Y.head_dim / 8;
-            if (u < Y.n_kv * per)
-                move_rows<uint4>(moves, n_moves, Y.v, (size_t)Y.n_kv * PKV_PAGE_TOKENS * Y.head_dim * 2, u % per, 0, 2, u / per, Y.head_dim, 0);
-        } else if (u < Y.n_kv * 4) {
-            move_rows<uint4>(moves, n_moves, Y.v, (size_t)Y.n_kv * PKV_VQ_TILE_BYTES, u & 3, 0, 3, u >> 2, 0, 0);
-        } else if ((u -= Y.n_kv * 4) < Y.n_kv) {
-            move_rows<uint16_t>(moves, n_moves, Y.v, (size_t)Y.n_kv * PKV_VQ_TILE_BYTES, 0, 0, 4, u, 0, Y.n_kv);
-        }
+        pool = Y.v;
+        const int per = Y.v_bits ? 4 : Y.head_dim / 8;
+        page_bytes = Y.v_bits ? (size_t)Y.n_kv * PKV_VQ_TILE_BYTES : (size_t)Y.n_kv * PKV_PAGE_TOKENS * Y.head_dim * 2;
+        g = u / per;
+        if (g < Y.n_kv) { kind = Y.v_bits ? 3 : 2; u %= per; }
+        else if (Y.v_bits && (g = u - Y.n_kv * 4) < Y.n_kv) { kind = 4; size = 2; }
+    }
+    auto at = [&](int slot) -> uint8_t* {
+        const uint32_t r = slot % PKV_PAGE_TOKENS;
+        const uint32_t o = kind == 0   ? pkv_code_offset(r, u * 16, RB)
+                           : kind == 1 ? PKV_PAGE_TOKENS * RB + pkv_scale_offset(r, u * 4)
+                           : kind == 2 ? ((uint32_t)g * PKV_PAGE_TOKENS + r) * Y.head_dim * 2 + u * 16
+                           : kind == 3 ? (uint32_t)g * 8192 + r * 64 + ((u ^ ((r >> 1) & 3u)) << 4)
+                                       : (uint32_t)Y.n_kv * 8192 + g * 256 + r * 2;
+        return pool + (size_t)(slot / PKV_PAGE_TOKENS) * page_bytes + o;
+    };
+    const int n_rows = kind < 5 ? n_moves : 0;
+    uint4 val[DEEP];
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+        const int j = tid / KC + k * KR;
+        if (j >= n_rows) continue;
+        const uint8_t* src = at(moves[j].x);
+        if (size == 16) val[k] = *reinterpret_cast<const uint4*>(src);
+        else if (size == 4) val[k].x = *reinterpret_cast<const uint32_t*>(src);
+        else val[k].x = *reinterpret_cast<const uint16_t*>(src);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < DEEP; ++k) {
+        const int j = tid / KC + k * KR;
+        if (j >= n_rows) continue;
+        uint8_t* dst = at(moves[j].y);
+        if (size == 16) *reinterpret_cast<uint4*>(dst) = val[k];
+        else if (size == 4) *reinterpret_cast<uint32_t*>(dst) = val[k].x;
+        else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)val[k].x;
     }
 }
 
@@ -365,7 +369,7 @@ extern "C" int pkv_keep_rows(const pkv_cache_t* const* layers, int32_t n_layers,
         }
         A.pg = *pages; A.cu = cu_dev; A.keep = keep_dev; A.n_keep = n_keep_dev; A.capacity = capacity;
         A.lengths_out = i0 == 0 ? lengths_out_dev : nullptr; A.status = status_dev;
-        PKV_CUDA_TRY(pkv_launch_chained(pkv_keep_rows_kernel, dim3((units + KT - 1) / KT, pages->batch, n), dim3(KT), 0, (cudaStream_t)stream, A));
+        PKV_CUDA_TRY(pkv_launch_chained(pkv_keep_rows_kernel, dim3((units + KC - 1) / KC, pages->batch, n), dim3(KT), 0, (cudaStream_t)stream, A));
     }
     return PKV_OK;
 }

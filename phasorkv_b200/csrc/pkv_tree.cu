@@ -240,18 +240,23 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     }
     __syncthreads();
     // absorbed rows: a column per thread
+    if (c < 2 * R || c >= W) {
 #pragma unroll 4
-    for (int r = 0; r < rows; ++r) {
-        float v = 0.0f;
-        if (c < 2 * R) {                             // conj(A) zq
+        for (int r = 0; r < rows; ++r) {             // conj(A) zq
             const float2 w = zq[r][f];
-            v = c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x;
-        } else if (c < W) {                          // slow dims: the raw query
-            for (int s = 0; s < 2 * L.n_slow; ++s)
-                v = fmaf(raw[r][s < L.n_slow ? L.slow_dev[s] : L.slow_dev[s - L.n_slow] + DH / 2],
-                         L.A_s_dev[((size_t)g * 2 * L.n_slow + s) * L.R_s + c - 2 * R], v);
+            qa[r][c] = (c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x) * tier;      // (padding: ar = ai = 0)
         }
-        qa[r][c] = v * tier;
+    } else {                                         // slow dims: the raw query; a factor serves all rows
+        float acc[AR] = {};
+#pragma unroll 4
+        for (int s = 0; s < 2 * L.n_slow; ++s) {
+            const int d = s < L.n_slow ? L.slow_dev[s] : L.slow_dev[s - L.n_slow] + DH / 2;
+            const float a = L.A_s_dev[((size_t)g * 2 * L.n_slow + s) * L.R_s + c - 2 * R];
+#pragma unroll
+            for (int r = 0; r < AR; ++r) acc[r] = fmaf(raw[r][d], a, acc[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < AR; ++r) qa[r][c] = acc[r] * tier;
     }
     __syncthreads();
     const int r = tid / NB, j = tid % NB;            // from here on: a 16-column block of a row per thread
