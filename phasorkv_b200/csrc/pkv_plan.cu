@@ -13,7 +13,7 @@ namespace {
 
 constexpr int NT = 1024;
 constexpr int MAX_BATCH = 4096;                      // two prefix sums of the batch in static shared memory
-constexpr int FILL = 2048;                           // tokens per CTA before another CTA joins
+constexpr int FILL = 4 * NT;                         // tokens per CTA before another CTA joins: four per thread
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + PKV_PAGE_TOKENS - 1) / PKV_PAGE_TOKENS; }
 
@@ -33,7 +33,7 @@ __device__ __forceinline__ int owner_of(const int* sums, int n, int i) {
 
 // Exclusive sums of a pair per thread over the block (one barrier pair); the totals are added to `run`, which every
 // thread carries from one group of NT entries to the next. 64 bits: a caller's lengths may be anything.
-__device__ __forceinline__ void block_scan2(long long& a, long long& b, long long (&run)[2], long long (*warp_sums)[2]) {
+__device__ __forceinline__ void block_scan2(long long& a, long long& b, long long (&run)[2], long long (*warp_sums)[2], int entries) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long a0 = a, b0 = b;
 #pragma unroll
@@ -44,8 +44,8 @@ __device__ __forceinline__ void block_scan2(long long& a, long long& b, long lon
     if (lane == 31) { warp_sums[warp][0] = a; warp_sums[warp][1] = b; }
     __syncthreads();
     long long before_a = run[0], before_b = run[1];
-#pragma unroll 8
-    for (int w = 0; w < NT / 32; ++w) {
+#pragma unroll 1
+    for (int w = 0; w < (min(entries, NT) + 31) / 32; ++w) {           // (the other warps have none)
         const long long x = warp_sums[w][0], y = warp_sums[w][1];
         if (w < warp) { before_a += x; before_b += y; }
         run[0] += x; run[1] += y;
@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(NT) pkv_plan_step_kernel(const PlanArgs A) {
                 if (pool) pages = pages_of(L + m) - pages_of(L);
             }
         }
-        block_scan2(n, pages, run, warp_sums);
+        block_scan2(n, pages, run, warp_sums, B - b0);
         if (b < B) {                                 // (sums past 2^31 are refused below, before anyone uses them)
             cu_s[b] = (int)n;
             off_s[b] = (int)pages;
@@ -112,31 +112,56 @@ __global__ void __launch_bounds__(NT) pkv_plan_step_kernel(const PlanArgs A) {
     }
     if (bad && blockIdx.x == 0) refuse(A.plan.status_dev, bad, where);
 
-    for (int i = blockIdx.x * NT + tid; i < A.plan.capacity; i += gridDim.x * NT) {
-        if (refused || i >= total) {                 // no token here: a slot that every writer skips
-            A.plan.slots_dev[i] = -1;
-            continue;
-        }
-        const int b = owner_of(cu_s, B, i), L = seqlens[b], row = i - cu_s[b], t = L + row;
-        const int p = t / PKV_PAGE_TOKENS, had = pages_of(L);
-        int page;
-        if (pool && p >= had) page = pool[count - (off_s[b] + p - had)];
-        else page = table[(size_t)b * max_pages + p];
-        A.plan.seq_dev[i] = b;
-        A.plan.slots_dev[i] = page >= 0 && page < n_pages ? page * PKV_PAGE_TOKENS + t % PKV_PAGE_TOKENS : -1;
-        int pos = t;
-        if (tree) {
-            const int32_t* parents = A.parents + cu_s[b];
-            unsigned long long word = 0;
-            int depth = -1;
-            for (int j = row; j >= 0; j = parents[j]) {      // strictly downwards, as checked above
-                word |= 1ull << j;
-                ++depth;
+    // Four tokens per thread, stored as one vector each where the arrays allow it: mostly of one sequence and page, so one search,
+    // one length and one page index serve them.
+    const bool wide = ((((uintptr_t)A.plan.slots_dev) | ((uintptr_t)A.plan.seq_dev) | ((uintptr_t)A.plan.positions_dev)) & 15u) == 0;
+    for (int i0 = (blockIdx.x * NT + tid) * 4; i0 < A.plan.capacity; i0 += gridDim.x * NT * 4) {
+        int slot[4], seq[4], pos[4];
+        int b = -1, L = 0, had = 0, at = -1, page = -1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = i0 + e;
+            slot[e] = -1;                            // no token here: a slot that every writer skips
+            if (refused || i >= total) continue;
+            if (b < 0 || i >= cu_s[b + 1]) {
+                b = owner_of(cu_s, B, i);
+                L = seqlens[b];
+                had = pages_of(L);
+                at = -1;
             }
-            pos = L + depth;
-            A.plan.mask_dev[i] = (int64_t)word;
+            const int row = i - cu_s[b], t = L + row, p = t / PKV_PAGE_TOKENS;
+            if (p != at) {
+                at = p;
+                if (pool && p >= had) page = pool[count - (off_s[b] + p - had)];
+                else page = table[(size_t)b * max_pages + p];
+            }
+            seq[e] = b;
+            if (page >= 0 && page < n_pages) slot[e] = page * PKV_PAGE_TOKENS + t % PKV_PAGE_TOKENS;
+            pos[e] = t;
+            if (tree) {
+                const int32_t* parents = A.parents + cu_s[b];
+                unsigned long long word = 0;
+                int depth = -1;
+                for (int j = row; j >= 0; j = parents[j]) {      // strictly downwards, as checked above
+                    word |= 1ull << j;
+                    ++depth;
+                }
+                pos[e] = L + depth;
+                A.plan.mask_dev[i] = (int64_t)word;
+            }
         }
-        A.plan.positions_dev[i] = pos;
+        if (wide && !refused && i0 + 4 <= total) {
+            *reinterpret_cast<int4*>(A.plan.slots_dev + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+            *reinterpret_cast<int4*>(A.plan.seq_dev + i0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+            *reinterpret_cast<int4*>(A.plan.positions_dev + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (i0 + e >= A.plan.capacity) break;
+                A.plan.slots_dev[i0 + e] = slot[e];
+                if (!refused && i0 + e < total) { A.plan.seq_dev[i0 + e] = seq[e]; A.plan.positions_dev[i0 + e] = pos[e]; }
+            }
+        }
     }
     if (blockIdx.x == 0)
         for (int b = tid; b <= B; b += NT) A.plan.cu_dev[b] = refused ? 0 : cu_s[b];
@@ -183,7 +208,7 @@ __global__ void __launch_bounds__(NT) pkv_truncate_kernel(const pkv_pages_t pg, 
             if (keep < 0 || L < 0 || L > pg.max_pages * PKV_PAGE_TOKENS) { bad = 4; where = b; }
             else if (pg.free_dev && keep < L) gone = pages_of(L) - pages_of(keep);
         }
-        block_scan2(gone, none, run, warp_sums);
+        block_scan2(gone, none, run, warp_sums, B - b0);
         if (b < B) off_s[b] = (int)gone;
     }
     if (tid == 0) off_s[B] = (int)run[0];
@@ -322,6 +347,7 @@ extern "C" int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev,
     int st = check_pages(pages);
     if (st) return st;
     if (!n_new_dev || !plan || !plan->cu_dev || !plan->ticket_dev || plan->capacity < 0 || plan->cu_dev == pages->seqlens_dev) return PKV_ERR_INVALID;
+    if (plan->capacity > 0x3fffffff) return PKV_ERR_UNSUPPORTED;
     if (plan->capacity > 0 && (!plan->seq_dev || !plan->positions_dev || !plan->slots_dev || (parents_dev && !plan->mask_dev))) return PKV_ERR_INVALID;
     if (pages->batch == 0) return PKV_OK;
     PlanArgs A{*pages, *plan, n_new_dev, parents_dev};

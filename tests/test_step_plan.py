@@ -90,6 +90,7 @@ def test_c_entries_refuse_bad_arguments(lib):
     assert lib.pkv_plan_step(pg(), 1024, None, plan(ticket=0), None) == -1
     assert lib.pkv_plan_step(pg(), 1024, 1024, plan(mask=0), None) == -1               # parents without room for masks
     assert lib.pkv_plan_step(pg(), 1024, None, plan(cap=-1), None) == -1
+    assert lib.pkv_plan_step(pg(), 1024, None, plan(cap=1 << 30), None) == -2
     assert lib.pkv_truncate(pg(), None, None, None) == -1
     assert lib.pkv_truncate(pg(), 8192, None, None) == -1                              # the lengths themselves
     cache = _lib.Cache(4096, 4096, 8, 256, 8, 128)
