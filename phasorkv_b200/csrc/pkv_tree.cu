@@ -38,11 +38,26 @@ constexpr float RESCALE_THRESHOLD = 8.0f;            // in base-2 logits
 constexpr uint32_t WAIT_LIMIT = 1u << 19;            // probes of a bounded wait
 
 // ------------------------------------------------------------------------------------------------ tiles and their pages
-// A tile index z = blk * groups + group: `qpb` drafted tokens from blk * qpb on, kv heads group * G .. . Row r of the tile:
-// kv head r / rph, drafted token (r % rph) / rep, query head (r % rph) % rep of the kv head.
+// How a sequence with n drafted tokens is cut into tiles: z = blk * groups + group covers `qpb` drafted tokens from blk * qpb on, kv
+// heads group * G .. . Row r of a tile: kv head r / rph, drafted token (r % rph) / rep, query head (r % rph) % rep of the kv head.
+struct Shape { int qpb, rph, G, groups, Z, cost; };
+// What a page costs a tile: a score tile and its softmax, or, from two kv heads on, the values of the kv heads (in quarters of the
+// former: 2500 cycles a page for one kv head, some 6000 for four).
+constexpr int COST_ONE = 4, COST_MOST = 20;
+constexpr int N_SM = 148;                            // CTAs of the attention launch: one per SM of a B200
+
 struct Tiles {
-    int rep, qpb, rph, G, groups, Z;
-    int gang, passes, gangs;                         // CTAs that walk the same pages side by side; rounds over the tiles
+    int rep, Z;                                      // query heads per kv head; most tiles of a sequence
+    int quantised;                                   // value pages hold codes
+    uint32_t shape[PKV_TREE_MAX + 1];                // by drafted tokens: qpb - 1 | rph / 16 - 1 | G - 1 | groups - 1, 6 + 3 + 3 bits and the rest
+    __device__ __forceinline__ Shape of(int n) const {
+        const uint32_t w = shape[n];
+        Shape t;
+        t.qpb = (w & 63u) + 1; t.rph = ((w >> 6 & 7u) + 1) * 16; t.G = (w >> 9 & 7u) + 1; t.groups = (w >> 12) + 1;
+        t.Z = t.groups * (n > t.qpb ? (n + t.qpb - 1) / t.qpb : 1);
+        t.cost = quantised ? COST_ONE + t.G : max(COST_ONE, t.G * 5 / 2);
+        return t;
+    }
 };
 
 struct Batch {
@@ -58,10 +73,58 @@ struct Batch {
     }
 };
 
-// Work is a list of pages: sequence by sequence, `passes` times over its pages. It is cut into stretches of U / gangs pages (the
-// first U % gangs of them one longer), one per gang; the gang's CTA zi takes the tile pass * gang + zi of each page. So the
-// tiles of a sequence read a page at about the same time (from L2 all but the first), and every CTA streams as many pages
-// whatever the lengths are.
+// Work is a list: sequence by sequence, `passes` times over its pages. It is cut into stretches of U / gangs (the first U % gangs of
+// them one longer), one per gang of CTAs; a page belongs to the stretch in which it begins, and the gang's CTA zi takes the tile
+// pass * gang + zi of it. So every CTA has as much to do whatever the lengths are.
+//   Every sequence has as many tiles (the usual step: as many drafts): a page counts 1, a gang has a CTA per tile (up to 16, then there are
+//   passes), and the tiles of a sequence read a page at about the same time, from L2 all but the first.
+//   Otherwise every CTA is a gang of its own, a sequence has a pass per tile, and a page counts what it costs the tile: no CTA idles
+//   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts: MIXED us, gangs for the largest: GANGS us).
+struct List { int gang, gangs, U; };                 // gang: CTAs, or 0 for CTAs on their own
+constexpr int LIST_WORDS = 6;
+
+__device__ __forceinline__ int passes_of(const Shape& t, int gang) { return gang == 0 ? t.Z : (t.Z + gang - 1) / gang; }
+__device__ __forceinline__ int cost_of(const Shape& t, int gang) { return gang == 0 ? t.cost : 1; }
+
+// by all nt threads of a CTA; red: LIST_WORDS words per warp
+__device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid, int nt, int (*red)[LIST_WORDS]) {
+    int v[LIST_WORDS] = {0, 0, 0, 0, 1 << 30, 1 << 30};      // pages, pages x tiles x cost, most tiles, most pages, fewest of each
+#pragma unroll 1
+    for (int b = tid; b < B.batch; b += nt) {
+        int lo, n, T;
+        const int pages = B.pages(b, lo, n, T);
+        if (pages == 0) continue;
+        const Shape t = X.of(n);
+        const int Z = t.Z;
+        v[0] += pages; v[1] += pages * Z * t.cost;
+        v[2] = max(v[2], Z); v[3] = max(v[3], pages); v[4] = min(v[4], Z); v[5] = min(v[5], pages);
+    }
+    v[0] = __reduce_add_sync(0xffffffffu, v[0]); v[1] = __reduce_add_sync(0xffffffffu, v[1]);
+    v[2] = __reduce_max_sync(0xffffffffu, v[2]); v[3] = __reduce_max_sync(0xffffffffu, v[3]);
+    v[4] = __reduce_min_sync(0xffffffffu, v[4]); v[5] = __reduce_min_sync(0xffffffffu, v[5]);
+    if ((tid & 31) == 0)
+#pragma unroll
+        for (int i = 0; i < LIST_WORDS; ++i) red[tid >> 5][i] = v[i];
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < nt / 32; ++w) {
+        if (w == (tid >> 5)) continue;
+        v[0] += red[w][0]; v[1] += red[w][1];
+        v[2] = max(v[2], red[w][2]); v[3] = max(v[3], red[w][3]); v[4] = min(v[4], red[w][4]); v[5] = min(v[5], red[w][5]);
+    }
+    List y;
+    const int passes = (v[2] + 15) >> 4;
+    y.gang = v[2] == v[4] ? (v[2] + passes - 1) / passes : 0;
+    y.gangs = y.gang ? N_SM / y.gang : N_SM;
+    y.U = v[2] == v[4] ? v[0] * passes : v[1];
+    if (v[2] == v[4] && v[3] == v[5] && v[3] > 0) {          // sequences of one length: no stretch across two of them if few SMs idle for it
+        const int whole = y.U / v[3], even = y.gangs >= whole ? y.gangs / whole * whole : 0;
+        if ((y.gangs - even) * 8 <= y.gangs) y.gangs = even;
+    }
+    y.gangs = min(y.gangs, y.gang ? y.U : max(y.U / COST_MOST, min(y.U, 1)));      // (a stretch that is not its tile's first or last has a page)
+    return y;
+}
+
 struct Cut {
     int per, longer;                                 // pages of a stretch; how many have one more
     __device__ __forceinline__ Cut(int U, int gangs) : per(U / gangs), longer(U % gangs) {}
@@ -74,20 +137,22 @@ struct Cut {
 
 struct Part {                                        // a stretch of pages of one tile
     int b, z, p_lo, p_hi, pages, lo, n, T;
+    Shape t;
 };
 
 struct Walk {
-    int b, pass, p, left;
+    int b, pass, p, at, end, gang;                   // at: place on the list of the (sequence, pass); end: of the stretch
     __device__ __forceinline__ bool next(const Batch& B, const Tiles& X, int zi, Part& s) {
-        while (left > 0 && b < B.batch) {
+        while (at < end && b < B.batch) {
             s.pages = B.pages(b, s.lo, s.n, s.T);
             if (s.pages == 0) { ++b; continue; }
-            const int take = min(left, s.pages - p);
-            s.b = b; s.z = pass * X.gang + zi; s.p_lo = p; s.p_hi = p + take;
-            left -= take;
-            p += take;
-            if (p == s.pages) { p = 0; if (++pass == X.passes) { pass = 0; ++b; } }
-            if (s.z < X.Z && s.z / X.groups * X.qpb < s.n) return true;      // else: no row of this tile in this sequence
+            s.t = X.of(s.n);
+            const int cost = cost_of(s.t, gang), here = end - at;
+            s.b = b; s.z = gang ? pass * gang + zi : pass; s.p_lo = p; s.p_hi = min(s.pages, (here + cost - 1) / cost);
+            at = here > s.pages * cost ? at + s.pages * cost : end;
+            p = 0;
+            if (++pass == passes_of(s.t, gang)) { pass = 0; ++b; }
+            if (s.p_lo < s.p_hi && s.z < s.t.Z) return true;         // else: this CTA has no tile in this pass
         }
         return false;
     }
@@ -155,31 +220,37 @@ template <int WP>
 __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const AbsorbArgs A) {
     constexpr int NB = WP / 16, NT = AR * NB, RB = WP / 2;
     static_assert(NT == WP, "a thread per column");
+    // raw queries and phasors first, later (in the same place) the absorbed rows
+    constexpr int PITCH = WP + 4, FIRST = AR * DH * 4 + AR * DH / 2 * 8, THEN = AR * PITCH * 4;
+    __shared__ __align__(16) uint8_t both[FIRST > THEN ? FIRST : THEN];
     __shared__ float2 zq[AR][DH / 2];
-    __shared__ float2 ph[AR][DH / 2];
-    __shared__ float raw[AR][DH];
-    __shared__ int sums[NT / 32][2];
-    __shared__ __align__(16) float qa[AR][WP + 4];
+    __shared__ int sums[NT / 32][LIST_WORDS];
+    float (*raw)[DH] = reinterpret_cast<float (*)[DH]>(both);
+    float2 (*ph)[DH / 2] = reinterpret_cast<float2 (*)[DH / 2]>(both + AR * DH * 4);
+    float (*qa)[PITCH] = reinterpret_cast<float (*)[PITCH]>(both);
     const pkv_layer_t& L = A.L;
     const int tid = threadIdx.x, z = blockIdx.y, b = blockIdx.z, r0 = blockIdx.x * AR;
     pkv_grid_wait();                                 // everything before this launch is done ..
     pkv_grid_launch_dependents();                    // .. so the attention behind it may stream pages while this one still runs
-    if (blockIdx.x == 0 && z == 0) {                 // for the merge: this sequence's place on the list of pages (the last one's: all)
-        int before = 0, all = 0, lo, n, T;
-        for (int i = tid; i < A.B.batch; i += NT) {
-            const int p = A.B.pages(i, lo, n, T);
-            all += p;
-            if (i < b) before += p;
+    if (blockIdx.x == 0 && z == 0) {                 // for the merge: this sequence's place on the list; the last one's CTA: the list itself
+        const List y = list_of(A.B, A.X, tid, NT, sums);
+        int before = 0;
+#pragma unroll 1
+        for (int i = tid; i < b; i += NT) {
+            int lo, n, T;
+            const int pages = A.B.pages(i, lo, n, T);
+            if (pages) { const Shape t = A.X.of(n); before += pages * passes_of(t, y.gang) * cost_of(t, y.gang); }
         }
         before = __reduce_add_sync(0xffffffffu, before);
-        all = __reduce_add_sync(0xffffffffu, all);
-        if ((tid & 31) == 0) { sums[tid >> 5][0] = before; sums[tid >> 5][1] = all; }
+        __syncthreads();
+        if ((tid & 31) == 0) sums[tid >> 5][0] = before;
         __syncthreads();
         if (tid == 0) {
-            before = all = 0;
-            for (int w = 0; w < NT / 32; ++w) { before += sums[w][0]; all += sums[w][1]; }
+            before = 0;
+#pragma unroll 1
+            for (int w = 0; w < NT / 32; ++w) before += sums[w][0];
             A.first_page[b] = before;
-            if (b == A.B.batch - 1) A.first_page[A.B.batch] = all;
+            if (b == A.B.batch - 1) { A.first_page[b + 1] = y.U; A.first_page[b + 2] = y.gang; A.first_page[b + 3] = y.gangs; }
         }
     }
     int lo, n, T;
@@ -188,10 +259,12 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
         if (n != 0 && A.status && tid == 0 && blockIdx.x == 0 && z == 0) { atomicExch(&A.status[0], 4); atomicExch(&A.status[1], b); }
         return;
     }
-    const int rep = A.X.rep, blk = z / A.X.groups, first = blk * A.X.qpb, nq = min(A.X.qpb, n - first);
-    const int g = (z % A.X.groups) * A.X.G + r0 / A.X.rph, rr0 = r0 % A.X.rph;      // rph is a multiple of 16: one kv head per CTA
+    const Shape t = A.X.of(n);
+    if (z >= t.Z) return;
+    const int rep = A.X.rep, blk = z / t.groups, first = blk * t.qpb, nq = min(t.qpb, n - first);
+    const int g = z % t.groups * t.G + r0 / t.rph, rr0 = r0 % t.rph;      // rph is a multiple of 16: one kv head per CTA
     const int rows = min(AR, nq * rep - rr0);
-    if (nq <= 0 || r0 / A.X.rph >= A.X.G || g >= L.n_kv || rows <= 0) return;
+    if (nq <= 0 || r0 / t.rph >= t.G || g >= L.n_kv || rows <= 0) return;
     // this CTA's rows belong to the drafted tokens q_lo .. q_hi
     const int q_lo = rr0 / rep, q_hi = (rr0 + rows - 1) / rep;
     // the factors of this thread's column, used for all rows
@@ -240,14 +313,8 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     }
     __syncthreads();
     // absorbed rows: a column per thread
-    if (c < 2 * R || c >= W) {
-#pragma unroll 4
-        for (int r = 0; r < rows; ++r) {             // conj(A) zq
-            const float2 w = zq[r][f];
-            qa[r][c] = (c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x) * tier;      // (padding: ar = ai = 0)
-        }
-    } else {                                         // slow dims: the raw query; a factor serves all rows
-        float acc[AR] = {};
+    float acc[AR] = {};
+    if (c >= 2 * R && c < W) {                       // slow dims: the raw query; a factor serves all rows
 #pragma unroll 4
         for (int s = 0; s < 2 * L.n_slow; ++s) {
             const int d = s < L.n_slow ? L.slow_dev[s] : L.slow_dev[s - L.n_slow] + DH / 2;
@@ -255,8 +322,15 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
 #pragma unroll
             for (int r = 0; r < AR; ++r) acc[r] = fmaf(raw[r][d], a, acc[r]);
         }
+    }
+    __syncthreads();                                 // the raw queries are done with
 #pragma unroll
-        for (int r = 0; r < AR; ++r) qa[r][c] = acc[r] * tier;
+    for (int r = 0; r < AR; ++r) {
+        if (c < 2 * R) {                             // conj(A) zq
+            const float2 w = zq[r][f];
+            acc[r] = c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x;
+        }
+        qa[r][c] = acc[r] * tier;                    // (padding: 0)
     }
     __syncthreads();
     const int r = tid / NB, j = tid % NB;            // from here on: a 16-column block of a row per thread
@@ -333,7 +407,7 @@ struct Shared {                       // at X_OFF
     float row_f[2][ROWS];             // per group: rescale factors, then 1 / sum
     float row_l[2][2][ROWS];          // [stretch & 1][group]: sums at the end
     uint32_t bad[3][MAX_G][2];        // [stretch % 3]: drafted tokens whose value row of a kv head is not finite
-    int scan[16];
+    int scan[16], red[16][LIST_WORDS];
     int row_o[2][ROWS];               // per group: where a row's result goes, or -1
 };
 static_assert(sizeof(Shared) <= 6144, "behind the stages");
@@ -351,6 +425,9 @@ __device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, Shared*
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, Shared* X, int32_t* status, int where) {
     return mbar_try_wait(bar, parity) || wait_longer(bar, parity, X, status, where);
 }
+
+// a value that all lanes hold, as one the compiler knows to be uniform (a warp reduction ends in a uniform register)
+__device__ __forceinline__ int uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
@@ -407,7 +484,7 @@ struct AttnArgs {
     float col_scale;                  // tensor scale of the latent x log2(e) / sqrt(d)
     float* part_o;                    // [2 per CTA][128 rows][128 dims]
     float2* part_ml;                  // [2 per CTA][128 rows]
-    const int32_t* first_page;        // [batch + 1]: pages of the sequences before each one, and of all
+    const int32_t* first_page;        // [batch + 3]: each sequence's first page on the list; all pages, CTAs per gang, gangs
     __nv_bfloat16* out;
     int32_t* status;
 };
@@ -421,7 +498,6 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     Shared* X = reinterpret_cast<Shared*>(smem + C::X_OFF);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Tiles& tl = A.X;
-    const int gang = blockIdx.x / tl.gang, zi = blockIdx.x % tl.gang;
     pkv_grid_launch_dependents();
 
     // ---- barriers, tensor memory, and where on the list of pages this CTA starts. Page table, lengths, masks and pages are
@@ -432,7 +508,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 2 * GROUP_WARPS + 1);
             mbar_init(&X->o_empty, 2 * GROUP_WARPS); mbar_init(&X->meet, 2 * GROUP_WARPS);
             X->abort_flag = 0;
-            X->start = Walk{0, 0, 0, 0};
+            X->start = Walk{0, 0, 0, 0, 0, 0};
         }
         if (lane < GROUP_WARPS) mbar_init(&X->decided[lane], 1);
         if (lane < 2) {
@@ -448,40 +524,42 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     if (warp == 3) tmem_alloc(&X->tmem_base, TM_COLS);
     tc_fence_before_sync();
     {
+        const List y = list_of(A.B, tl, tid, C::NTHREADS, X->red);
         const int per = (A.B.batch + C::NTHREADS - 1) / C::NTHREADS, b_lo = min(tid * per, A.B.batch), b_hi = min(b_lo + per, A.B.batch);
         int mine = 0, lo, n, T;
 #pragma unroll 1
-        for (int b = b_lo; b < b_hi; ++b) mine += A.B.pages(b, lo, n, T);
-        int incl = mine;
+        for (int b = b_lo; b < b_hi; ++b) {
+            const int pages = A.B.pages(b, lo, n, T);
+            if (pages) { const Shape t = tl.of(n); mine += pages * passes_of(t, y.gang) * cost_of(t, y.gang); }
+        }
+        int before = mine;
 #pragma unroll 1
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
+            const int x = __shfl_up_sync(0xffffffffu, before, o);
+            if (lane >= o) before += x;
         }
-        if (lane == 31) X->scan[warp] = incl;
+        if (lane == 31) X->scan[warp] = before;
         __syncthreads();
-        int before = incl - mine, U = 0;
+        before -= mine;
 #pragma unroll 1
-        for (int w = 0; w < C::NTHREADS / 32; ++w) {
-            if (w < warp) before += X->scan[w];
-            U += X->scan[w];
-        }
-        U *= tl.passes;
-        before *= tl.passes;
-        const int gangs = min(tl.gangs, U);
-        if (gang < gangs) {
-            const Cut cut(U, gangs);
+        for (int w = 0; w < warp; ++w) before += X->scan[w];
+        const int gang = y.gang ? blockIdx.x / y.gang : blockIdx.x;
+        if (gang < y.gangs) {
+            const Cut cut(y.U, y.gangs);
             const int u0 = cut.start(gang);
-            if (mine > 0 && before <= u0 && u0 < before + mine * tl.passes) {
+            if (before <= u0 && u0 < before + mine) {
                 int u = u0 - before;
 #pragma unroll 1
                 for (int b = b_lo; b < b_hi; ++b) {
                     const int pages = A.B.pages(b, lo, n, T);
-                    if (u < pages * tl.passes) {
-                        X->start = Walk{b, u / pages, u % pages, cut.start(gang + 1) - u0};
+                    if (pages == 0) continue;
+                    const Shape t = tl.of(n);
+                    const int cost = cost_of(t, y.gang), block = pages * cost, units = block * passes_of(t, y.gang);
+                    if (u < units) {
+                        X->start = Walk{b, u / block, (u % block + cost - 1) / cost, u0 - u % block, cut.start(gang + 1), y.gang};
                         break;
                     }
-                    u -= pages * tl.passes;
+                    u -= units;
                 }
             }
         }
@@ -490,8 +568,9 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     tc_fence_after_sync();
     const uint32_t tb = X->tmem_base, sbase = smem_u32(smem);
     Walk walk = X->start;
+    const int zi = walk.gang ? blockIdx.x % walk.gang : 0;
     Part s;
-    auto heads = [&](const Part& p) { return min(tl.G, A.n_kv - p.z % tl.groups * tl.G); };      // kv heads of the tile
+    auto heads = [&](const Part& p) { return min(p.t.G, A.n_kv - p.z % p.t.groups * p.t.G); };      // kv heads of the tile
 
     if (warp == 0) {
         // ================================================================== latent pages and query operand
@@ -539,7 +618,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             int k = 0, pg = 0;
             bool ok = true;
             while (ok && walk.next(A.B, tl, zi, s)) {
-                const int g0 = s.z % tl.groups * tl.G, ng = heads(s);
+                const int g0 = s.z % s.t.groups * s.t.G, ng = heads(s);
                 for (int p = s.p_lo; p < s.p_hi && ok; ++p, ++pg) {
                     const int page = A.page_table[(size_t)s.b * A.B.max_pages + p];
                     if (page < 0 || page >= A.n_pages) { ok = false; break; }      // (reported by warp 0)
@@ -593,7 +672,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
         };
         while (ok && walk.next(A.B, tl, zi, s)) {
-            const int p_lo = __shfl_sync(0xffffffffu, s.p_lo, 0), p_hi = __shfl_sync(0xffffffffu, s.p_hi, 0);
+            const int p_lo = uniform(s.p_lo), p_hi = uniform(s.p_hi);
             wait(&X->q_full, seg & 1, 30);
             if (!ok) break;
             tc_fence_after_sync();
@@ -630,7 +709,6 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     } else if (warp == 3) {
         // ================================================================== P.V MMAs: O^T += V^T P^T
         const bool leader = elect_one();
-        const uint32_t idesc_o = idesc_bf16(DH, tl.rph, true, false);
         const uint64_t p_desc = smem_desc(sbase + C::P_OFF, 0, 1024, SWZ_128B);
         int k = 0, kv = 0, seg = 0;
         uint32_t cleaned = 0;                          // phase bit of every stage's v_clean
@@ -639,8 +717,9 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
         };
         while (ok && walk.next(A.B, tl, zi, s)) {
-            const int ng = __shfl_sync(0xffffffffu, heads(s), 0), base = __shfl_sync(0xffffffffu, s.T - s.n, 0);
-            const int p_lo = __shfl_sync(0xffffffffu, s.p_lo, 0), p_hi = __shfl_sync(0xffffffffu, s.p_hi, 0);
+            const int ng = uniform(heads(s)), base = uniform(s.T - s.n), rph = uniform(s.t.rph);
+            const uint32_t idesc_o = idesc_bf16(DH, rph, true, false);
+            const int p_lo = uniform(s.p_lo), p_hi = uniform(s.p_hi);
             for (int p = p_lo; p < p_hi && ok; ++p, ++k) {
                 wait(&X->p_full[k & 1], (k >> 1) & 1, 31);
                 if (p == p_lo && seg > 0) wait(&X->o_empty, (seg - 1) & 1, 35);
@@ -655,11 +734,11 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     if (!ok) break;
                     tc_fence_after_sync();
                     const uint64_t v_desc = smem_desc(sbase + C::V_OFF + st * C::V_BYTES, C::V_BYTES / 2, 1024, SWZ_128B);
-                    const uint64_t pg_desc = p_desc + (uint64_t)(((k & 1) * C::P_BYTES + h * (C::P_BYTES / 2) + g * tl.rph * 128) / 16);
+                    const uint64_t pg_desc = p_desc + (uint64_t)(((k & 1) * C::P_BYTES + h * (C::P_BYTES / 2) + g * rph * 128) / 16);
                     if (leader) {
 #pragma unroll
                         for (int c = 0; c < HALF / 16; ++c)
-                            mma_bf16(tb + TM_O + g * tl.rph, v_desc + (uint64_t)(c * 16 * 128 / 16), pg_desc + (uint64_t)(c * 32 / 16), idesc_o,
+                            mma_bf16(tb + TM_O + g * rph, v_desc + (uint64_t)(c * 16 * 128 / 16), pg_desc + (uint64_t)(c * 32 / 16), idesc_o,
                                      !(p == p_lo && h == 0 && c == 0));
                         tc_commit(&X->v_empty[st]);
                     }
@@ -728,9 +807,10 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
         };
         bool go = true;
         while (go && walk.next(A.B, tl, zi, s)) {
-            const int ng = heads(s), base = s.T - s.n, first = s.z / tl.groups * tl.qpb, nq = min(tl.qpb, s.n - first);
-            const int gl = r / tl.rph, rr = r % tl.rph;
+            const int ng = heads(s), base = s.T - s.n, first = s.z / s.t.groups * s.t.qpb, nq = min(s.t.qpb, s.n - first), rph = s.t.rph;
+            const int gl = r / rph, rr = r % rph;
             const bool mine = gl < ng && rr < nq * tl.rep;              // a drafted token's row
+            const bool busy = __any_sync(0xffffffffu, mine);
             unsigned long long word = 0;
             if (mine) {
                 const int i = first + rr / tl.rep;
@@ -751,7 +831,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 // then rescaled), so the weights are rarely formed a second time (a stretch's first page apart).
                 // The loop is not unrolled beyond 32 columns: the code of all roles has to fit the instruction cache together, or
                 // each of them runs at the speed of instruction fetch (unrolled over the 128 columns: 192 against 165 us).
-                const bool masked = drafts < PKV_PAGE_TOKENS || !mine;
+                const bool masked = drafts < PKV_PAGE_TOKENS;
                 const uint32_t s_tm = tl_s + TM_S + 128 * grp;
                 float2 sum;
                 float ref = m, before = -INFINITY;
@@ -766,7 +846,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     float top = -INFINITY;
                     sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < 4 && busy; ++c) {
                         float x[32];
                         uint32_t w[16];
                         if (ok) tmem_ld32(s_tm + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
@@ -774,7 +854,6 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         if (masked) {                                   // tokens that the row does not see
                             const int j0 = 32 * c - drafts;             // drafted token of the first column (negative: cached)
                             uint32_t see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
-                            if (!mine) see = 0u;
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
                                 if (!(see >> e & 1)) x[e] = -INFINITY;
@@ -815,7 +894,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                             *reinterpret_cast<uint4*>(line + ((((c & 1) * 4 + u) ^ (r & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                     }
                     if (!first_try) break;
-                    top *= cs;
+                    top = mine ? top * cs : -INFINITY;                  // (a row that nobody has: whatever its column becomes, nobody reads it)
                     if (p > s.p_lo) {
                         wait_all(&X->decided[quad], (k - 1) & 1, 42);
                         before = X->row_m[r];
@@ -841,7 +920,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         group_sync(grp);
                         tc_fence_after_sync();
 #pragma unroll 1
-                        for (int c0 = 0; c0 < ng * tl.rph; c0 += 16) {
+                        for (int c0 = 0; c0 < ng * rph; c0 += 16) {
                             uint32_t o[16];
                             tmem_ld16(tl_s + TM_O + c0, o);
                             tmem_ld_wait();
@@ -909,12 +988,12 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             l = X->row_l[seg & 1][0][r] + X->row_l[seg & 1][1][r];
             if (!VQ && mine && ((word & 0xffffffffu & X->bad[seg % 3][gl][0]) | ((word >> 32) & X->bad[seg % 3][gl][1]))) l = __int_as_float(0x7fc00000);
             X->row_f[grp][r] = l == 0.0f ? 0.0f : 1.0f / l;             // a row that sees nothing: zeros
-            X->row_o[grp][r] = mine ? (s.lo + first + rr / tl.rep) * A.n_q + (s.z % tl.groups * tl.G + gl) * tl.rep + rr % tl.rep : -1;
+            X->row_o[grp][r] = mine ? (s.lo + first + rr / tl.rep) * A.n_q + (s.z % s.t.groups * s.t.G + gl) * tl.rep + rr % tl.rep : -1;
             if (!whole && mine && grp == 0) A.part_ml[slot * ROWS + r] = make_float2(M, l);
             group_sync(grp);
             // (four columns at a time in a rolled loop: this thread's dim is r)
 #pragma unroll 1
-            for (int c0 = 64 * grp; c0 < min(ng * tl.rph, 64 * grp + 64); c0 += 4) {
+            for (int c0 = 64 * grp; c0 < min(ng * rph, 64 * grp + 64); c0 += 4) {
                 uint32_t o[4];
                 tmem_ldn<4>(tl_s + TM_O + c0, o);
                 tmem_ld_wait();
@@ -942,85 +1021,95 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
 }
 
 // ------------------------------------------------------------------------------------------------ merge
-// O = sum 2^(m - M) o / sum 2^(m - M) l over the stretches of a tile that several gangs had. WPR warps per row, a lane holds four
-// dims; the references, sums and outputs of eight stretches are asked for together (two round trips in all, the first
-// for the lengths).
-template <int WPR>
+// O = sum 2^(m - M) o / sum 2^(m - M) l over the stretches of a tile that several gangs had. A warp has RW rows (a lane four dims of
+// each); WPR warps share the stretches of their rows. References, sums and outputs of DEEP stretches are asked for together: many
+// rows of few stretches, or few rows of many.
+template <int WPR, int RW, int DEEP>
 __global__ void __launch_bounds__(256) pkv_tree_merge_kernel(const AttnArgs A) {
-    __shared__ float4 acc_s[8][32];
-    __shared__ float2 ml_s[8];
+    __shared__ float4 acc_s[WPR > 1 ? 8 : 1][RW][32];
+    __shared__ float2 ml_s[8][RW];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, z = blockIdx.y, b = blockIdx.z;
-    const int r = blockIdx.x * (8 / WPR) + warp / WPR, w0 = warp % WPR;
+    const int r0 = (blockIdx.x * (8 / WPR) + warp / WPR) * RW, w0 = warp % WPR;
     const Tiles& X = A.X;
-    const int gl = r / X.rph, rr = r % X.rph, g = z % X.groups * X.G + gl, first = z / X.groups * X.qpb;
     pkv_grid_launch_dependents();
     pkv_grid_wait();
     int lo, n, T;
-    const int pages = A.B.pages(b, lo, n, T), U = A.first_page[A.B.batch] * X.passes, u0 = A.first_page[b] * X.passes + z / X.gang * pages;
+    const int pages = A.B.pages(b, lo, n, T), U = A.first_page[A.B.batch], gang = A.first_page[A.B.batch + 1], gangs = A.first_page[A.B.batch + 2];
+    const int list = A.first_page[b];
     if (pages == 0) return;
-    const Cut cut(U, min(X.gangs, U));
-    const int x0 = cut.of(u0), x1 = cut.of(u0 + pages - 1);
+    const Shape t = X.of(n);
+    if (z >= t.Z) return;
+    const int cost = cost_of(t, gang), u0 = list + (gang ? z / gang : z) * pages * cost, zi = gang ? z % gang : 0;
+    const Cut cut(U, gangs);
+    const int x0 = cut.of(u0), x1 = cut.of(u0 + (pages - 1) * cost);
     if (x0 == x1) return;                            // one CTA did the whole tile and has written it
-    const bool live = gl < X.G && g < A.n_kv && rr < min(X.qpb, n - first) * X.rep;
-    float M = -INFINITY, l = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    if (live) {
-        constexpr int DEEP = 8;
+    const int gl = r0 / t.rph, rr0 = r0 % t.rph, g = z % t.groups * t.G + gl, first = z / t.groups * t.qpb;      // (rph is a multiple of 16)
+    const int rows = gl < t.G && g < A.n_kv ? min(RW, min(t.qpb, n - first) * X.rep - rr0) : 0;
+    float M[RW], l[RW];
+    float4 acc[RW];
+#pragma unroll
+    for (int r = 0; r < RW; ++r) { M[r] = -INFINITY; l[r] = 0.0f; acc[r] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    if (rows > 0) {
 #pragma unroll 1
         for (int xb = x0 + w0; xb <= x1; xb += WPR * DEEP) {
-            float4 o[DEEP];
-            float2 ml[DEEP];
+            float4 o[DEEP][RW];
+            float2 ml[DEEP][RW];
 #pragma unroll
             for (int k = 0; k < DEEP; ++k) {
                 const int x = xb + k * WPR;
-                const size_t slot = ((size_t)(x * X.gang + z % X.gang) * 2 + (x == x0)) * ROWS + r;
-                ml[k] = x <= x1 ? A.part_ml[slot] : make_float2(-INFINITY, 0.0f);
-                if (x <= x1) o[k] = reinterpret_cast<const float4*>(A.part_o + slot * DH)[lane];
-            }
-            float top = M;
+                const size_t slot = ((size_t)(gang ? x * gang + zi : x) * 2 + (x == x0)) * ROWS + r0;
 #pragma unroll
-            for (int k = 0; k < DEEP; ++k) top = fmaxf(top, ml[k].x);
-            const float f0 = M > -INFINITY ? exp2f(M - top) : 1.0f;
-            acc.x *= f0; acc.y *= f0; acc.z *= f0; acc.w *= f0;
-            l *= f0;
-            M = top;
-#pragma unroll
-            for (int k = 0; k < DEEP; ++k) {
-                if (ml[k].x > -INFINITY) {               // (a stretch that saw nothing of the row holds zeros)
-                    const float f = exp2f(ml[k].x - M);
-                    l = fmaf(ml[k].y, f, l);
-                    acc.x = fmaf(o[k].x, f, acc.x); acc.y = fmaf(o[k].y, f, acc.y);
-                    acc.z = fmaf(o[k].z, f, acc.z); acc.w = fmaf(o[k].w, f, acc.w);
-                } else {
-                    l += ml[k].y;                        // 0, or NaN
+                for (int r = 0; r < RW; ++r) {
+                    const bool there = x <= x1 && r < rows;
+                    ml[k][r] = there ? A.part_ml[slot + r] : make_float2(-INFINITY, 0.0f);
+                    if (there) o[k][r] = reinterpret_cast<const float4*>(A.part_o + (slot + r) * DH)[lane];
                 }
             }
+#pragma unroll
+            for (int k = 0; k < DEEP; ++k)
+#pragma unroll
+                for (int r = 0; r < RW; ++r) {
+                    if (ml[k][r].x == -INFINITY) {       // (a stretch that saw nothing of the row: zeros, or NaN in the sum)
+                        l[r] += ml[k][r].y;
+                        continue;
+                    }
+                    const float top = fmaxf(M[r], ml[k][r].x), was = exp2f(M[r] - top), now = exp2f(ml[k][r].x - top);
+                    M[r] = top;
+                    l[r] = fmaf(l[r], was, ml[k][r].y * now);
+                    acc[r].x = fmaf(acc[r].x, was, o[k][r].x * now); acc[r].y = fmaf(acc[r].y, was, o[k][r].y * now);
+                    acc[r].z = fmaf(acc[r].z, was, o[k][r].z * now); acc[r].w = fmaf(acc[r].w, was, o[k][r].w * now);
+                }
         }
     }
-    if constexpr (WPR > 1) {
-        acc_s[warp][lane] = acc;
-        if (lane == 0) ml_s[warp] = make_float2(M, l);
+    if constexpr (WPR > 1) {                         // the first of the WPR warps adds the others' sums to its own
+#pragma unroll
+        for (int r = 0; r < RW; ++r) {
+            acc_s[warp][r][lane] = acc[r];
+            if (lane == 0) ml_s[warp][r] = make_float2(M[r], l[r]);
+        }
         __syncthreads();
         if (w0 != 0) return;
-        float top = M;
 #pragma unroll 1
-        for (int w = 1; w < WPR; ++w) top = fmaxf(top, ml_s[warp + w].x);
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        l = 0.0f;
-#pragma unroll 1
-        for (int w = 0; w < WPR; ++w) {
-            const float2 ml = ml_s[warp + w];
-            const float f = ml.x > -INFINITY ? exp2f(ml.x - top) : 1.0f;      // (nothing there: zeros, or NaN)
-            const float4 o = acc_s[warp + w][lane];
-            sum.x = fmaf(o.x, f, sum.x); sum.y = fmaf(o.y, f, sum.y); sum.z = fmaf(o.z, f, sum.z); sum.w = fmaf(o.w, f, sum.w);
-            l = fmaf(ml.y, f, l);
-        }
-        acc = sum;
+        for (int w = 1; w < WPR; ++w)
+#pragma unroll
+            for (int r = 0; r < RW; ++r) {
+                const float2 ml = ml_s[warp + w][r];
+                const float4 o = acc_s[warp + w][r][lane];
+                if (ml.x == -INFINITY) { l[r] += ml.y; continue; }
+                const float top = fmaxf(M[r], ml.x), was = exp2f(M[r] - top), now = exp2f(ml.x - top);
+                M[r] = top;
+                l[r] = fmaf(l[r], was, ml.y * now);
+                acc[r].x = fmaf(acc[r].x, was, o.x * now); acc[r].y = fmaf(acc[r].y, was, o.y * now);
+                acc[r].z = fmaf(acc[r].z, was, o.z * now); acc[r].w = fmaf(acc[r].w, was, o.w * now);
+            }
     }
-    if (!live) return;
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const size_t row = (size_t)(lo + first + rr / X.rep) * A.n_q + g * X.rep + rr % X.rep;
-    *reinterpret_cast<uint2*>(A.out + row * DH + lane * 4) = make_uint2(pack_bf16(acc.x * f, acc.y * f), pack_bf16(acc.z * f, acc.w * f));
+#pragma unroll
+    for (int r = 0; r < RW; ++r) {
+        if (r >= rows) continue;
+        const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        const size_t row = (size_t)(lo + first + (rr0 + r) / X.rep) * A.n_q + g * X.rep + (rr0 + r) % X.rep;
+        *reinterpret_cast<uint2*>(A.out + row * DH + lane * 4) = make_uint2(pack_bf16(acc[r].x * f, acc[r].y * f), pack_bf16(acc[r].z * f, acc[r].w * f));
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -1050,24 +1139,21 @@ int encode_map(CUtensorMap* map, const void* base, uint64_t rows, uint32_t box_r
     return PKV_OK;
 }
 
-constexpr int N_SM = 148;                            // CTAs of the attention launch: one per SM of a B200
-
 // Rows of a kv head: rep query heads of up to qpb drafted tokens, in blocks of equal size when there are more than 128; padded
 // to the 16 columns an MMA takes. As many kv heads per tile as fit, evenly over the tiles.
-Tiles make_tiles(int n_q, int n_kv, int max_draft) {
+Tiles make_tiles(int n_q, int n_kv, int max_draft, bool quantised) {
     Tiles X;
+    X.quantised = quantised;
     X.rep = n_q / n_kv;
-    const int most = ROWS / X.rep, blocks = (max_draft + most - 1) / most;
-    X.qpb = (max_draft + blocks - 1) / blocks;
-    X.rph = (X.rep * X.qpb + 15) / 16 * 16;
-    const int fit = ROWS / X.rph, groups = (n_kv + fit - 1) / fit;
-    X.G = (n_kv + groups - 1) / groups;
-    X.groups = (n_kv + X.G - 1) / X.G;
-    X.Z = X.groups * blocks;
-    // a gang of all tiles if that leaves few SMs idle, else of a half, a third, ...: up to 16 side by side
-    X.passes = (X.Z + 15) / 16;
-    X.gang = (X.Z + X.passes - 1) / X.passes;
-    X.gangs = N_SM / X.gang;
+    X.Z = 1;
+    X.shape[0] = 0;
+    const int most = ROWS / X.rep;
+    for (int n = 1; n <= PKV_TREE_MAX; ++n) {
+        const int blocks = (n + most - 1) / most, qpb = (n + blocks - 1) / blocks, rph = (X.rep * qpb + 15) / 16 * 16;
+        const int fit = ROWS / rph, even = (n_kv + fit - 1) / fit, G = (n_kv + even - 1) / even, groups = (n_kv + G - 1) / G;
+        X.shape[n] = (uint32_t)(qpb - 1) | (uint32_t)(rph / 16 - 1) << 6 | (uint32_t)(G - 1) << 9 | (uint32_t)(groups - 1) << 12;
+        if (n <= max_draft && groups * blocks > X.Z) X.Z = groups * blocks;
+    }
     return X;
 }
 
@@ -1075,12 +1161,12 @@ struct Layout { size_t blobs, part_o, part_ml, first_page, total; };
 
 Layout make_layout(const Tiles& X, int batch, int WP) {
     Layout y;
-    const size_t ctas = (size_t)X.gangs * X.gang;
+    const size_t ctas = N_SM;
     y.blobs = 0;
     y.part_o = ((size_t)batch * X.Z * blob_bytes(WP) + 1023) / 1024 * 1024;
     y.part_ml = y.part_o + ctas * 2 * ROWS * DH * 4;
     y.first_page = y.part_ml + ctas * 2 * ROWS * 8;
-    y.total = y.first_page + ((size_t)batch + 1) * 4;
+    y.total = y.first_page + ((size_t)batch + 3) * 4;
     return y;
 }
 
@@ -1097,12 +1183,13 @@ int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, const AttnArgs& at, s
     static pkv_attr_flags attr;
     PKV_CUDA_TRY(pkv_set_max_smem(pkv_tree_attn_kernel<WP, VQ>, C::SMEM, attr));
     PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_absorb_kernel<WP>, dim3(ROWS / AR, X.Z, ab.B.batch), dim3(AR * WP / 16), 0, st, ab));
-    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ>, dim3(X.gangs * X.gang), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
-    // parts of a tile: about one per CTA and tile; a warp takes some eight of them
-    const int parts = X.gangs / (ab.B.batch * X.passes) + 1;
-    if (parts <= 8) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1>, dim3(ROWS / 8, X.Z, ab.B.batch), dim3(256), 0, st, at));
-    else if (parts <= 16) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<2>, dim3(ROWS / 4, X.Z, ab.B.batch), dim3(256), 0, st, at));
-    else PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<8>, dim3(ROWS, X.Z, ab.B.batch), dim3(256), 0, st, at));
+    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ>, dim3(N_SM), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
+    // stretches of a tile, if all sequences have as many tiles and pages: the more, the more warps share a row's
+    const int parts = N_SM / (ab.B.batch * X.Z) + 1;
+    const dim3 block(256);
+    if (parts <= 4) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1, 4, 2>, dim3(ROWS / 32, X.Z, ab.B.batch), block, 0, st, at));
+    else if (parts <= 16) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<2, 1, 8>, dim3(ROWS / 4, X.Z, ab.B.batch), block, 0, st, at));
+    else PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<8, 1, 8>, dim3(ROWS, X.Z, ab.B.batch), block, 0, st, at));
     return PKV_OK;
 }
 
@@ -1119,7 +1206,7 @@ int check_shape(const pkv_layer_t* L, int32_t batch, int32_t max_draft, int32_t 
 extern "C" int64_t pkv_tree_workspace_bytes(const pkv_layer_t* layer, int32_t batch, int32_t max_draft, int32_t max_pages) {
     int st = check_shape(layer, batch, max_draft, max_pages);
     if (st) return st;
-    return (int64_t)make_layout(make_tiles(layer->n_q, layer->n_kv, max_draft), batch, pkv_padded_width(2 * layer->R + layer->R_s)).total;
+    return (int64_t)make_layout(make_tiles(layer->n_q, layer->n_kv, max_draft, false), batch, pkv_padded_width(2 * layer->R + layer->R_s)).total;
 }
 
 extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache, const pkv_pages_t* pages, const void* q_dev, int32_t q_dtype,
@@ -1140,10 +1227,10 @@ extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache,
     const int WP = pkv_padded_width(cache->W);
     // coordinates of the tensor maps are 31 bits
     if ((int64_t)cache->n_pages * cache->n_kv * PKV_PAGE_TOKENS > 0x7fffffff || (int64_t)cache->n_pages * 144 > 0x7fffffff) return PKV_ERR_UNSUPPORTED;
-    const Tiles X = make_tiles(layer->n_q, layer->n_kv, max_draft);
+    const Tiles X = make_tiles(layer->n_q, layer->n_kv, max_draft, cache->v_bits != 0);
     const Layout y = make_layout(X, pages->batch, WP);
     const size_t blob_rows = (size_t)pages->batch * X.Z * (blob_bytes(WP) / 128);
-    if (blob_rows > 0x7fffffff || X.Z > 65535 || (int64_t)pages->batch * pages->max_pages * X.passes > 0x3fffffff) return PKV_ERR_UNSUPPORTED;
+    if (blob_rows > 0x7fffffff || X.Z > 65535 || (int64_t)pages->batch * pages->max_pages * X.Z > 0x3fffffff / COST_MOST) return PKV_ERR_UNSUPPORTED;
     if ((int64_t)n_tokens * layer->n_q > 0x7fffffff) return PKV_ERR_UNSUPPORTED;      // rows of the result are 31 bits
     if (!workspace_dev || (((uintptr_t)workspace_dev) & 1023u) || workspace_bytes < (int64_t)y.total) return PKV_ERR_INVALID;
     st = init_encoder();
