@@ -86,13 +86,16 @@ constexpr int LIST_WORDS = 6;
 __device__ __forceinline__ int passes_of(const Shape& t, int gang) { return gang == 0 ? t.Z : (t.Z + gang - 1) / gang; }
 __device__ __forceinline__ int cost_of(const Shape& t, int gang) { return gang == 0 ? t.cost : 1; }
 
-// by all nt threads of a CTA; red: LIST_WORDS words per warp
-__device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid, int nt, int (*red)[LIST_WORDS]) {
+// by all nt threads of a CTA; red: LIST_WORDS words per warp. last: pages and drafted tokens of the last sequence that the thread looked at
+// (its only one, in batches of at most nt)
+__device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid, int nt, int (*red)[LIST_WORDS], int2& last) {
+    last = make_int2(0, 0);
     int v[LIST_WORDS] = {0, 0, 0, 0, 1 << 30, 1 << 30};      // pages, pages x tiles x cost, most tiles, most pages, fewest of each
 #pragma unroll 1
     for (int b = tid; b < B.batch; b += nt) {
         int lo, n, T;
         const int pages = B.pages(b, lo, n, T);
+        last = make_int2(pages, n);
         if (pages == 0) continue;
         const Shape t = X.of(n);
         const int Z = t.Z;
@@ -107,7 +110,7 @@ __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid,
         for (int i = 0; i < LIST_WORDS; ++i) red[tid >> 5][i] = v[i];
     __syncthreads();
 #pragma unroll 1
-    for (int w = 0; w < nt / 32; ++w) {
+    for (int w = 0; w < min(nt, B.batch + 31) / 32; ++w) {     // (the other warps have none)
         if (w == (tid >> 5)) continue;
         v[0] += red[w][0]; v[1] += red[w][1];
         v[2] = max(v[2], red[w][2]); v[3] = max(v[3], red[w][3]); v[4] = min(v[4], red[w][4]); v[5] = min(v[5], red[w][5]);
@@ -235,7 +238,8 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     // One more CTA per sequence, for the merge: the sequence's place on the list; the last sequence's: the list itself.
     if (blockIdx.x == ROWS / AR) {
         if (z != 0) return;
-        const List y = list_of(A.B, A.X, tid, NT, sums);
+        int2 last;
+        const List y = list_of(A.B, A.X, tid, NT, sums, last);
         int before = 0;
 #pragma unroll 1
         for (int i = tid; i < b; i += NT) {
@@ -532,12 +536,14 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     if (warp == 3) tmem_alloc(&X->tmem_base, TM_COLS);
     tc_fence_before_sync();
     {
-        const List y = list_of(A.B, tl, tid, C::NTHREADS, X->red);
+        int2 last;
+        const List y = list_of(A.B, tl, tid, C::NTHREADS, X->red, last);
         const int per = (A.B.batch + C::NTHREADS - 1) / C::NTHREADS, b_lo = min(tid * per, A.B.batch), b_hi = min(b_lo + per, A.B.batch);
         int mine = 0, lo, n, T;
+        auto pages_of = [&](int b) { if (per == 1) { n = last.y; return last.x; } return A.B.pages(b, lo, n, T); };
 #pragma unroll 1
         for (int b = b_lo; b < b_hi; ++b) {
-            const int pages = A.B.pages(b, lo, n, T);
+            const int pages = pages_of(b);
             if (pages) { const Shape t = tl.of(n); mine += pages * passes_of(t, y.gang) * cost_of(t, y.gang); }
         }
         int before = mine;
@@ -550,7 +556,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
         __syncthreads();
         before -= mine;
 #pragma unroll 1
-        for (int w = 0; w < warp; ++w) before += X->scan[w];
+        for (int w = 0; w < min(warp, (A.B.batch + 31) / 32); ++w) before += X->scan[w];
         const int gang = y.gang ? blockIdx.x / y.gang : blockIdx.x;
         if (gang < y.gangs) {
             const Cut cut(y.U, y.gangs);
@@ -559,7 +565,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 int u = u0 - before;
 #pragma unroll 1
                 for (int b = b_lo; b < b_hi; ++b) {
-                    const int pages = A.B.pages(b, lo, n, T);
+                    const int pages = pages_of(b);
                     if (pages == 0) continue;
                     const Shape t = tl.of(n);
                     const int cost = cost_of(t, y.gang), block = pages * cost, units = block * passes_of(t, y.gang);
