@@ -79,7 +79,8 @@ struct Batch {
 //   Every sequence has as many tiles (the usual step: as many drafts): a page counts 1, a gang has a CTA per tile (up to 16, then there are
 //   passes), and the tiles of a sequence read a page at about the same time, from L2 all but the first.
 //   Otherwise every CTA is a gang of its own, a sequence has a pass per tile, and a page counts what it costs the tile: no CTA idles
-//   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts: MIXED us, gangs for the largest: GANGS us).
+//   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts: 104 us; tiles of one shape, by the most
+//   drafts, and gangs of them: 130 us).
 struct List { int gang, gangs, U; };                 // gang: CTAs, or 0 for CTAs on their own
 constexpr int LIST_WORDS = 6;
 
