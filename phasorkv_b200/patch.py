@@ -25,6 +25,12 @@ module (``hidden_states, position_embeddings, attention_mask, past_key_values, *
                                        ``o_proj``: keys are never rebuilt, the Hugging Face KV cache
                                        is not touched.
 
+  verification (``attn.kv_tree`` set,  the tokens are drafts: every sequence's row of T tokens is a tree (``kv_tree`` an int
+  T tokens)                            tensor [B, T], the row of each token's parent, -1 for a child of the last cached one) or a
+                                       chain (``kv_tree = "chain"``); they are written behind the cached tokens and attend to
+                                       them and to their ancestors (``plan_step`` -> ``write_paged`` -> ``tree_step`` -> ``o_proj``).
+                                       ``PhasorKeyPatch.accept`` then keeps a path of them in every layer.
+
 Positions are counted by the layer's own cache (``seqlens``, one length per sequence), so the caller runs
 the model with ``use_cache=False`` and feeds one new token per sequence and decode call. A ragged batch is
 prefilled right-padded with ``attn.kv_lengths`` set to the valid token counts, the contract of the reference's
@@ -57,6 +63,8 @@ class LayerDecodeState:
         self.seq = torch.arange(batch, dtype=torch.int32, device=pk.device)
         self.lengths = [0] * batch                          # tokens cached per sequence (host copy of cache.seqlens)
         self.calibrated = False
+        self.drafted = None                                 # plan and lengths before it, between verify() and accept()
+        self.tree = {}                                      # drafts per sequence -> (plan, workspace, write scratch, counts)
 
     @property
     def length(self) -> int:
@@ -65,6 +73,7 @@ class LayerDecodeState:
 
     def reset(self) -> None:
         self.lengths = [0] * self.batch
+        self.drafted = None
         self.cache.seqlens.zero_()
 
     def _need(self, b: int, n: int) -> None:
@@ -74,6 +83,7 @@ class LayerDecodeState:
     def prefill(self, x: torch.Tensor, v: torch.Tensor, lengths=None) -> None:
         """x [B, T, D] layer input, v [B, T, n_kv, d] value rows: append the first ``lengths[b]`` (default: all T)
         tokens of row b to sequence b (rows are right-padded, as the reference's batches are)."""
+        self._settled()
         B, T = x.shape[0], x.shape[1]
         n_new = [T] * B if lengths is None else [int(n) for n in lengths]
         if len(n_new) != B or min(n_new) < 0 or max(n_new) > T:
@@ -100,6 +110,7 @@ class LayerDecodeState:
 
     def decode(self, x: torch.Tensor, q: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         """x [B, D], q [B, n_q, d] pre-RoPE, v [B, n_kv, d] of the one new token of every sequence -> O [B, n_q, d] fp32."""
+        self._settled()
         for b in range(self.batch):
             self._need(b, 1)
         pk = self.pk
@@ -112,6 +123,52 @@ class LayerDecodeState:
         pk.attend_step(self.cache, self.ws, out=self.ws.out, after_prologue=True)
         return self.ws.out
 
+    def _settled(self) -> None:
+        if self.drafted is not None:
+            raise RuntimeError("drafted tokens are waiting for accept()")
+
+    def verify(self, x: torch.Tensor, q: torch.Tensor, v: torch.Tensor, parents: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """x [B, n, D], q [B, n, n_q, d] pre-RoPE, v [B, n, n_kv, d] of n <= 64 drafted tokens per sequence -> O [B, n, n_q, d] bf16.
+        `parents` [B, n]: the row of each token's parent, before it, or -1 for a child of the last cached token; None: a
+        chain. The drafts are written behind the cached tokens; ``accept`` has to follow."""
+        self._settled()
+        B, n = x.shape[0], x.shape[1]
+        pk, dev = self.pk, self.pk.device
+        for b in range(B):
+            self._need(b, n)
+        if n not in self.tree:
+            self.tree[n] = (self.cache.step_plan(B * n, tree=True), pk.tree_workspace(B, B * n, n, self.max_tokens), pk.write_scratch(B * n),
+                            torch.full((B,), n, dtype=torch.int32, device=dev),
+                            torch.arange(-1, n - 1, dtype=torch.int32, device=dev).repeat(B))
+        plan, ws, scratch, n_new, chain = self.tree[n]
+        parents = chain if parents is None else parents.to(device=dev, dtype=torch.int32).reshape(B * n).contiguous()
+        self.cache.plan_step(plan, n_new, parents=parents)
+        pk.write_paged(self.cache, x.reshape(B * n, -1).contiguous(), plan.positions, plan.slots, v=v.reshape(B * n, *v.shape[2:]).contiguous(),
+                       scratch=scratch)
+        q = q.reshape(B * n, pk.n_q, pk.head_dim).contiguous()
+        if q.dtype not in (torch.bfloat16, torch.float32):
+            q = q.float()
+        out = pk.tree_step(self.cache, q, plan, ws)
+        self.drafted = (plan, n)
+        return out.view(B, n, pk.n_q, pk.head_dim)
+
+    def accept(self, keep) -> None:
+        """Keep a path of the drafts that ``verify`` wrote: ``keep[b]`` lists their rows, from the root on (each the parent of
+        the next; none: all drafts of b are dropped). They become the sequence's next tokens."""
+        if self.drafted is None:
+            raise RuntimeError("accept() follows verify()")
+        plan, n = self.drafted
+        keep = [[int(i) for i in rows] for rows in keep]
+        if len(keep) != self.batch or any(not 0 <= i < n for rows in keep for i in rows) or any(a >= b for rows in keep for a, b in zip(rows, rows[1:])):
+            raise ValueError(f"keep gives ascending rows 0 .. {n - 1} for each of the {self.batch} sequences")
+        dev = self.pk.device
+        rows = torch.tensor([r + [-1] * (n - len(r)) for r in keep], dtype=torch.int32).to(dev).reshape(-1)
+        lengths = torch.empty(self.batch, dtype=torch.int32, device=dev)
+        self.cache.keep_rows(plan, rows, torch.tensor([len(r) for r in keep], dtype=torch.int32).to(dev), lengths)
+        self.cache.truncate(lengths)
+        self.lengths = [a + len(r) for a, r in zip(self.lengths, keep)]
+        self.drafted = None
+
 
 def _patched_forward(attn, state_of, original):
     def forward(hidden_states, position_embeddings=None, attention_mask=None, past_key_values=None, **kwargs):
@@ -119,6 +176,11 @@ def _patched_forward(attn, state_of, original):
         st: LayerDecodeState = state_of(B)
         d = attn.head_dim
         v = attn.v_proj(hidden_states).view(B, T, -1, d)
+        tree = getattr(attn, "kv_tree", None)
+        if tree is not None:                                # drafted tokens, one or several
+            q = attn.q_proj(hidden_states).view(B, T, -1, d)
+            o = st.verify(hidden_states, q, v, parents=None if isinstance(tree, str) else tree)
+            return attn.o_proj(o.to(hidden_states.dtype).reshape(B, T, -1)), None
         if T > 1:
             out = original(hidden_states, position_embeddings=position_embeddings, attention_mask=attention_mask,
                            past_key_values=None, **kwargs)
@@ -148,6 +210,11 @@ class PhasorKeyPatch:
         """Forget the cached tokens of every patched layer (a new prompt follows)."""
         for st in self.states.values():
             st.reset()
+
+    def accept(self, keep) -> None:
+        """``LayerDecodeState.accept`` in every patched layer, after a verification pass of the model."""
+        for st in self.states.values():
+            st.accept(keep)
 
     @property
     def name(self) -> str:

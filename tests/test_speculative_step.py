@@ -1,0 +1,124 @@
+"""The operators of a speculative step together, as a patched layer runs them: drafts planned, written, attended to, a path kept,
+and decoding going on from there -- against the same tokens decoded one by one.
+
+Tolerance: the token-by-token outputs are within 2e-3 of the formula in the 2-norm (what decode attention is held to), the
+drafted ones within 5e-3 (two roundings to bf16 of at most 2^-8, uniform: 3.2e-3, and the logits' share). The two write paths form
+a row's sums in another order, so a latent may differ in its last bit and, at a tie, in one code: far below 1e-3. In all 8e-3."""
+import random
+import types
+
+import pytest
+import torch
+
+from phasorkv_b200 import PhasorKey, PhasorKeyPatch, synth
+from phasorkv_b200.patch import LayerDecodeState
+
+pytestmark = pytest.mark.gpu
+NORM = 8e-3
+D = 256
+
+
+def rel(a, b):
+    return float((a.double() - b.double()).norm() / b.double().norm())
+
+
+def state(pk, B, v_bits, x, v):
+    st = LayerDecodeState(pk, B, 512, v_bits=v_bits)
+    st.prefill(x, v)
+    return st
+
+
+@pytest.mark.parametrize("config,v_bits", [("cfg2", 0), ("cfg3", 0), ("cfg5", 0), ("cfg2", 3)])
+@pytest.mark.parametrize("kind", ["tree", "chain"])
+def test_verified_drafts_match_tokens_decoded_one_by_one(config, v_bits, kind):
+    spec = synth.make_layer(config, 0, d_model=D, factor_gain=16.0)
+    pk = PhasorKey.from_spec(spec)
+    B, T, n = 3, 122, 11                                             # the drafts cross a page
+    g, r = torch.Generator(device="cuda").manual_seed(5), random.Random(5)
+    t = lambda *s: torch.randn(s, generator=g, device="cuda")
+    x0, v0 = t(B, T, D), t(B, T, spec.n_kv, 128).to(torch.bfloat16)
+    one, many = state(pk, B, v_bits, x0, v0), state(pk, B, v_bits, x0, v0)
+    for round_ in range(3):
+        x, q, v = t(B, n, D), t(B, n, spec.n_q, 128), t(B, n, spec.n_kv, 128).to(torch.bfloat16)
+        parents = [[i - 1 if kind == "chain" else r.randint(max(-1, i - 4), i - 1) for i in range(n)] for _ in range(B)]
+        out = many.verify(x, q, v, None if kind == "chain" else torch.tensor(parents))
+        with pytest.raises(RuntimeError):
+            many.decode(x[:, 0], q[:, 0], v[:, 0])
+        # a path of the same length in every sequence (the plain decode steps all sequences together)
+        paths = []
+        for b in range(B):
+            path = [r.randrange(n)]
+            while parents[b][path[0]] >= 0:
+                path.insert(0, parents[b][path[0]])
+            paths.append(path)
+        k = min(map(len, paths)) if round_ != 1 else 0
+        paths = [p[:k] for p in paths]
+        many.accept(paths)
+        for j in range(k):
+            pick = lambda a: torch.stack([a[b, paths[b][j]] for b in range(B)])
+            want = one.decode(pick(x), pick(q), pick(v))
+            assert rel(pick(out), want) < NORM, (round_, j)
+        assert one.lengths == many.lengths and many.cache.seqlens.tolist() == many.lengths
+        x, q, v = t(B, D), t(B, spec.n_q, 128), t(B, spec.n_kv, 128).to(torch.bfloat16)
+        assert rel(many.decode(x, q, v), one.decode(x, q, v)) < NORM
+    for s in (many.ws, many.cache, *[w[1] for w in many.tree.values()], *[w[0] for w in many.tree.values()]):
+        assert int(s.status.abs().sum()) == 0
+
+
+def test_patched_layer_verifies_and_accepts():
+    """Through the patched forward of an attention module: drafts in one pass, then the path in every layer."""
+    spec = synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    lin = lambda i, o: torch.nn.Linear(i, o, bias=False, device="cuda", dtype=torch.float32)
+
+    class Attn(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.head_dim = 128
+            self.q_proj, self.v_proj, self.o_proj = lin(D, 32 * 128), lin(D, 8 * 128), lin(32 * 128, D)
+
+        def forward(self, hidden_states, **kw):
+            return hidden_states, None
+    layers = [types.SimpleNamespace(self_attn=Attn()) for _ in range(2)]
+    patch = PhasorKeyPatch(install_forward=True, max_tokens=512)
+    undo = [patch.patch(i, y, spec, 8, 128, 32, "cuda") for i, y in enumerate(layers)]
+    h = lambda n: torch.randn((2, n, D), generator=g, device="cuda")
+    prompt, drafts = h(40), h(4)
+    with torch.no_grad():
+        for y in layers:
+            y.self_attn(prompt)
+            y.self_attn.kv_tree = torch.tensor([[-1, 0, 0, 2], [-1, -1, 1, 2]])
+        tree = [y.self_attn(drafts)[0] for y in layers]
+        for y in layers:
+            y.self_attn.kv_tree = None
+        patch.accept([[0, 2, 3], [1, 2, 3]])
+        assert all(st.lengths == [43, 43] for st in patch.states.values())
+        after = [y.self_attn(h(1))[0] for y in layers]
+        patch.reset()
+        for i, y in enumerate(layers):
+            y.self_attn(prompt)
+            for j in range(3):
+                step = torch.stack([drafts[0, [0, 2, 3][j]], drafts[1, [1, 2, 3][j]]])[:, None]
+                got = torch.stack([tree[i][0, [0, 2, 3][j]], tree[i][1, [1, 2, 3][j]]])
+                assert rel(got, y.self_attn(step)[0][:, 0]) < NORM
+    assert all(a.isfinite().all() for a in after)
+    for u in undo:
+        u()
+
+
+def test_refusals_of_a_layer_state():
+    pk = PhasorKey.from_spec(synth.make_layer("cfg2", 0, d_model=D))
+    t = lambda *s: torch.randn(s, device="cuda")
+    st = state(pk, 2, 0, t(2, 500, D), t(2, 500, 8, 128).to(torch.bfloat16))
+    with pytest.raises(RuntimeError):
+        st.accept([[], []])
+    with pytest.raises(RuntimeError):
+        st.verify(t(2, 13, D), t(2, 13, 32, 128), t(2, 13, 8, 128))      # 512 tokens per sequence
+    st.verify(t(2, 4, D), t(2, 4, 32, 128), t(2, 4, 8, 128))
+    with pytest.raises(RuntimeError):
+        st.verify(t(2, 4, D), t(2, 4, 32, 128), t(2, 4, 8, 128))
+    for bad in ([[0]], [[0], [4]], [[1, 0], []], [[0, 0], []], [[-1], []]):
+        with pytest.raises(ValueError):
+            st.accept(bad)
+    st.accept([[0, 1], []])
+    assert st.lengths == [502, 500] and st.cache.seqlens.tolist() == [502, 500]
