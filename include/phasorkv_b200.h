@@ -453,7 +453,7 @@ typedef struct pkv_plan {
  * each token's parent within its sequence, before the token itself, or -1 for a child of the last cached token; then
  * n_new <= PKV_TREE_MAX, and masks are filled too.  The other arrays behind the last token are left as they were.
  * When a length, a parent or the pool does not allow the step, the call changes no table and no length, cu is all zero,
- * every slot is -1 and the status says why.  batch <= 4096. */
+ * every slot is -1 and the status says why.  batch <= 4096.  n_new_dev and parents_dev are not the plan's own arrays. */
 int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev, const int32_t* parents_dev, const pkv_plan_t* plan,
                   void* stream);
 
@@ -482,7 +482,7 @@ int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache, const pkv_
  * rows count) names rows of the step's tokens in ascending order; row base + keep[j] moves to base + j, base = seqlens -
  * (cu[b+1] - cu[b]), in the latent and value pages of every layer (layers: host array of n_layers caches that are addressed
  * by the same table; no cache twice).  Only bytes move: a token keeps its rotation, so a kept path's positions must
- * be base, base + 1, ... (in a tree, depths 0, 1, ...).  lengths_out_dev (optional, [batch], not seqlens_dev): base + n_keep,
+ * be base, base + 1, ... (in a tree, depths 0, 1, ...).  lengths_out_dev (optional, [batch], none of the inputs): base + n_keep,
  * for pkv_truncate.  Lengths and tables stay as they are.  A sequence whose indices do not ascend or are out of range is
  * left alone (status 4, lengths_out = its length). */
 int pkv_keep_rows(const pkv_cache_t* const* layers, int32_t n_layers, const pkv_pages_t* pages, const int32_t* cu_dev,

@@ -348,6 +348,9 @@ extern "C" int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev,
     if (st) return st;
     if (!n_new_dev || !plan || !plan->cu_dev || !plan->ticket_dev || plan->capacity < 0 || plan->cu_dev == pages->seqlens_dev) return PKV_ERR_INVALID;
     if (plan->capacity > 0x3fffffff) return PKV_ERR_UNSUPPORTED;
+    // several CTAs read what the caller gives while the first already writes
+    auto written = [&](const int32_t* p) { return p && (p == plan->cu_dev || p == plan->seq_dev || p == plan->positions_dev || p == plan->slots_dev); };
+    if (written(n_new_dev) || written(parents_dev)) return PKV_ERR_INVALID;
     if (plan->capacity > 0 && (!plan->seq_dev || !plan->positions_dev || !plan->slots_dev || (parents_dev && !plan->mask_dev))) return PKV_ERR_INVALID;
     if (pages->batch == 0) return PKV_OK;
     PlanArgs A{*pages, *plan, n_new_dev, parents_dev};
@@ -371,6 +374,7 @@ extern "C" int pkv_keep_rows(const pkv_cache_t* const* layers, int32_t n_layers,
     int st = check_pages(pages);
     if (st) return st;
     if (!layers || n_layers <= 0 || !cu_dev || (capacity > 0 && !keep_dev) || !n_keep_dev || capacity < 0 || lengths_out_dev == pages->seqlens_dev) return PKV_ERR_INVALID;
+    if (lengths_out_dev && (lengths_out_dev == n_keep_dev || lengths_out_dev == keep_dev || lengths_out_dev == cu_dev)) return PKV_ERR_INVALID;   // (read by other CTAs)
     for (int i = 0; i < n_layers; ++i) {
         const pkv_cache_t* c = layers[i];
         st = pkv_check_cache(c);

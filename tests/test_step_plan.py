@@ -335,3 +335,15 @@ def test_refused_paths_leave_their_sequence_alone(keep, n_keep):
     other.latent.copy_(before[0]), other.v.view(-1).view(torch.uint8).copy_(before[1])
     rest = torch.tensor(sorted(set(range(cache.n_pages * PAGE)) - set(moved.tolist())), dtype=torch.int32, device="cuda")
     assert all(torch.equal(x, y) for x, y in zip(rows_of(cache, rest), rows_of(other, rest)))
+
+
+def test_c_entries_refuse_an_array_given_twice(lib):
+    """Other CTAs still read the inputs when the first writes its results."""
+    pg, cache = _lib.Pages(4096, 8192, 0, 2, 4, 8), _lib.Cache(4096, 4096, 8, 256, 8, 128)
+    for twice in (1024, 2048, 5120, 6144):
+        plan = _lib.Plan(1024, 2048, 5120, 6144, 7168, 9216, 0, 4)
+        assert lib.pkv_plan_step(ctypes.byref(pg), twice, None, ctypes.byref(plan), None) == -1
+        assert lib.pkv_plan_step(ctypes.byref(pg), 10240, twice, ctypes.byref(plan), None) == -1
+    one = (ctypes.c_void_p * 1)(ctypes.addressof(cache))
+    for out in (1024, 2048, 5120, 8192):
+        assert lib.pkv_keep_rows(one, 1, ctypes.byref(pg), 1024, 4, 2048, 5120, out, None, None) == -1
