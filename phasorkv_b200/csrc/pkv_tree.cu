@@ -407,7 +407,7 @@ struct Shared {                       // at X_OFF
     uint64_t q_full, q_empty, o_empty, meet;
     uint64_t p_full[2], pv_done[2], decided[GROUP_WARPS];
     uint64_t k_full[4], k_empty[4], v_full[7], v_empty[7], v_clean[7], s_full[2], s_empty[2];
-    uint64_t r_full[8], r_empty[8], sc_full[2], sc_empty[2];
+    uint64_t r_full[8], r_empty[8], sc_full[2], sc_empty[2], drained[2];
     uint32_t tmem_base;
     volatile int abort_flag;
     Walk start;
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
         if (lane < GROUP_WARPS) mbar_init(&X->decided[lane], 1);
         if (lane < 2) {
             mbar_init(&X->p_full[lane], GROUP_WARPS); mbar_init(&X->pv_done[lane], 1); mbar_init(&X->s_full[lane], 1); mbar_init(&X->s_empty[lane], GROUP_WARPS);
-            mbar_init(&X->sc_full[lane], 1); mbar_init(&X->sc_empty[lane], GROUP_WARPS);
+            mbar_init(&X->sc_full[lane], 1); mbar_init(&X->sc_empty[lane], GROUP_WARPS); mbar_init(&X->drained[lane], 1);
         }
         if (lane < C::NK) { mbar_init(&X->k_full[lane], 1); mbar_init(&X->k_empty[lane], 1); }
         if (lane < C::NV) { mbar_init(&X->v_full[lane], VQ ? 4 : 1); mbar_init(&X->v_empty[lane], 1); mbar_init(&X->v_clean[lane], GROUP_WARPS); }
@@ -585,6 +585,11 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     Walk walk = X->start;
     const int zi = walk.gang ? blockIdx.x % walk.gang : 0;
     Part s;
+    auto drain = [&](bool leader, int i) {           // given up: the MMAs in flight end before the tensor memory goes back
+        if (!X->abort_flag) return;
+        if (leader) tc_commit(&X->drained[i]);
+        mbar_wait(&X->drained[i], 0, 1u << 16);
+    };
     auto heads = [&](const Part& p) { return min(p.t.G, A.n_kv - p.z % p.t.groups * p.t.G); };      // kv heads of the tile
 
     if (warp == 0) {
@@ -725,6 +730,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
             ++seg;
         }
+        drain(leader, 0);
     } else if (warp == 3) {
         // ================================================================== P.V MMAs: O^T += V^T P^T
         const bool leader = elect_one();
@@ -768,6 +774,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
             ++seg;
         }
+        drain(leader, 1);
     } else if (VQ && warp >= 12) {
         // ================================================================== quantised values -> bf16 operand tiles
         // Every E2M1 level is a bf16 number; the token's scale goes into the softmax weight. 128 threads, two per token.
@@ -883,7 +890,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         for (int e = 1; e < 31; e += 2) mx[(e >> 1) & 1] = max3(mx[(e >> 1) & 1], x[e], x[e + 1]);
                         top = max3(mx[0], mx[1], x[31]);
                         if constexpr (VQ) {
-                            // the weight of a token carries its value scale of this row's kv head
+                            // The weight of a token carries its value scale of this row's kv head, and the product is rounded to bf16
+                            // (2^-8 of it); the sum takes the weights themselves, which the scale is no part of.
                             const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + grp * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + c * 64);
 #pragma unroll
                             for (int u = 0; u < 4; ++u) {

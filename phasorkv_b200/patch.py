@@ -43,6 +43,7 @@ from typing import Optional
 
 import torch
 
+from ._lib import TREE_MAX
 from .latent import PAGE_TOKENS, PhasorKey
 
 NVFP4_BITS = 4.5          # E2M1 code + one E4M3 scale per 16 codes (phasorkv/quant.py:9)
@@ -134,6 +135,12 @@ class LayerDecodeState:
         self._settled()
         B, n = x.shape[0], x.shape[1]
         pk, dev = self.pk, self.pk.device
+        if B != self.batch or not 1 <= n <= TREE_MAX:
+            raise ValueError(f"1 .. {TREE_MAX} drafted tokens for each of the {self.batch} sequences, not {n} for {B}")
+        if parents is not None:
+            host = parents.cpu()
+            if host.shape != (B, n) or (host < -1).any() or (host >= torch.arange(n)).any():
+                raise ValueError("parents [batch, drafts] name a row before the token's own, or -1")
         for b in range(B):
             self._need(b, n)
         if n not in self.tree:
@@ -142,12 +149,12 @@ class LayerDecodeState:
                             torch.arange(-1, n - 1, dtype=torch.int32, device=dev).repeat(B))
         plan, ws, scratch, n_new, chain = self.tree[n]
         parents = chain if parents is None else parents.to(device=dev, dtype=torch.int32).reshape(B * n).contiguous()
-        self.cache.plan_step(plan, n_new, parents=parents)
-        pk.write_paged(self.cache, x.reshape(B * n, -1).contiguous(), plan.positions, plan.slots, v=v.reshape(B * n, *v.shape[2:]).contiguous(),
-                       scratch=scratch)
+        x, v = x.reshape(B * n, -1).contiguous(), v.reshape(B * n, pk.n_kv, pk.head_dim).contiguous()
         q = q.reshape(B * n, pk.n_q, pk.head_dim).contiguous()
         if q.dtype not in (torch.bfloat16, torch.float32):
             q = q.float()
+        self.cache.plan_step(plan, n_new, parents=parents)
+        pk.write_paged(self.cache, x, plan.positions, plan.slots, v=v, scratch=scratch)
         out = pk.tree_step(self.cache, q, plan, ws)
         self.drafted = (plan, n)
         return out.view(B, n, pk.n_q, pk.head_dim)

@@ -24,19 +24,27 @@ def rel(a, b):
 
 def state(pk, B, v_bits, x, v):
     st = LayerDecodeState(pk, B, 512, v_bits=v_bits)
+    st.calibrated = pk.second_blocks is not None
     st.prefill(x, v)
     return st
 
 
-@pytest.mark.parametrize("config,v_bits", [("cfg2", 0), ("cfg3", 0), ("cfg5", 0), ("cfg2", 3)])
+@pytest.mark.parametrize("config,v_bits,other", [("cfg2", 0, None), ("cfg3", 0, None), ("cfg5", 0, None), ("cfg2", 3, None),
+                                                 ("cfg2", 0, "attn_scale"), ("cfg2", 0, "tiers"), ("cfg3", 2, "tiers")])
 @pytest.mark.parametrize("kind", ["tree", "chain"])
-def test_verified_drafts_match_tokens_decoded_one_by_one(config, v_bits, kind):
+def test_verified_drafts_match_tokens_decoded_one_by_one(config, v_bits, other, kind):
     spec = synth.make_layer(config, 0, d_model=D, factor_gain=16.0)
+    if other == "attn_scale":
+        spec.attn_scale = 1.3
     pk = PhasorKey.from_spec(spec)
     B, T, n = 3, 122, 11                                             # the drafts cross a page
     g, r = torch.Generator(device="cuda").manual_seed(5), random.Random(5)
     t = lambda *s: torch.randn(s, generator=g, device="cuda")
     x0, v0 = t(B, T, D), t(B, T, spec.n_kv, 128).to(torch.bfloat16)
+    if other == "tiers":                                             # one scale per 16-aligned span instead of the calibrated one
+        W = pk.cache_width
+        edges = [0, 32, 112, W]
+        pk.set_second_tiers([(a, b, 0.01 * 3 ** i) for i, (a, b) in enumerate(zip(edges, edges[1:]))])
     one, many = state(pk, B, v_bits, x0, v0), state(pk, B, v_bits, x0, v0)
     for round_ in range(3):
         x, q, v = t(B, n, D), t(B, n, spec.n_q, 128), t(B, n, spec.n_kv, 128).to(torch.bfloat16)
@@ -112,6 +120,9 @@ def test_refusals_of_a_layer_state():
     st = state(pk, 2, 0, t(2, 500, D), t(2, 500, 8, 128).to(torch.bfloat16))
     with pytest.raises(RuntimeError):
         st.accept([[], []])
+    for B, n, parents in ((3, 4, None), (2, 65, None), (2, 0, None), (2, 2, [[-1, 1], [-1, 0]]), (2, 2, [[-2, 0], [-1, 0]]), (2, 2, [[-1], [0]])):
+        with pytest.raises(ValueError):
+            st.verify(t(B, n, D), t(B, n, 32, 128), t(B, n, 8, 128), None if parents is None else torch.tensor(parents))
     with pytest.raises(RuntimeError):
         st.verify(t(2, 13, D), t(2, 13, 32, 128), t(2, 13, 8, 128))      # 512 tokens per sequence
     st.verify(t(2, 4, D), t(2, 4, 32, 128), t(2, 4, 8, 128))

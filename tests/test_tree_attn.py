@@ -76,7 +76,7 @@ class Case:
     def run(self, **kw):
         return self.pk.tree_step(self.cache, self.q, self.plan, self.ws, **kw)
 
-    def formula(self, b):
+    def formula(self, b, most=25):
         """(O, A = sum p |v|) of sequence b in doubles, on what the pages hold."""
         pk, base, n = self.pk, self.base[b], self.n[b]
         lo = sum(self.n[:b])
@@ -104,7 +104,7 @@ class Case:
                 qa.append(torch.cat([x[:, h][..., s], y[:, h][..., s]], -1) @ pk.A_s[g].double().to(dev))
             S = torch.cat(qa, -1) @ C.T * 128 ** -0.5
             S = torch.where(see[:, None], S, -torch.inf)
-            assert not (S[torch.isfinite(S)].abs() >= 25).any()                 # what the tolerance counts on
+            assert not (S[torch.isfinite(S)].abs() >= most).any()               # what the tolerance counts on
             P = torch.softmax(S, -1)
             P = torch.where(see.any(-1)[:, None, None], P, torch.zeros_like(P))
             for i in range(n):                                                  # only what a row sees enters its sums
@@ -384,3 +384,74 @@ def test_two_calls_at_once_and_the_same_bits_again():
         torch.cuda.synchronize()
         assert torch.equal(x, want[0]) and torch.equal(y, want[1])
     a.check(want[0]), b.check(want[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+def test_a_query_that_is_not_finite_makes_its_rows_nan(bad):
+    c = Case(layer(32, 8), [700, 90], [9, 4], q_dtype=torch.float32)
+    want = c.run()
+    c.q[3, 17, 40] = float(bad)
+    out = c.run()
+    assert out[3, 17].isnan().all()
+    out[3, 17] = want[3, 17]
+    assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v_bits", [0, 2])
+def test_peaked_logits(v_bits):
+    """Queries 12 times as large: one token has most of the weight. The query's terms leave 7e-5 of a logit, here at most 300, so
+    a weight is off by e^(2 x 0.021) - 1 = 0.043 of itself at most and the result by as much of A, next to the roundings."""
+    c = Case(layer(32, 8), [900, 130], [11, 40], v_bits=v_bits, q_dtype=torch.float32)
+    c.q *= 12.0
+    out = c.run()
+    torch.cuda.synchronize()
+    for b, (lo, n) in enumerate(((0, 11), (11, 40))):
+        O, A = c.formula(b, most=300)
+        assert ((out[lo:lo + n].double() - O).abs() <= (ELEM + 0.043) * A).all()
+
+
+@pytest.mark.gpu
+def test_no_sequence_has_a_draft():
+    c = Case(layer(32, 8), [300, 0], [0, 0], pad=3)
+    out = torch.full(c.q.shape, 7.0, device="cuda", dtype=torch.bfloat16)
+    c.run(out=out)
+    torch.cuda.synchronize()
+    assert (out == 7).all() and int(c.ws.status.abs().sum()) == 0
+
+
+@pytest.mark.gpu
+def test_result_in_place_of_the_queries():
+    c = Case(layer(32, 8), [2900, 130], [30, 7])
+    want = c.run()
+    assert torch.equal(c.run(out=c.q), want)
+
+
+@pytest.mark.gpu
+def test_many_sequences():
+    r = random.Random(1)
+    base = [r.choice([0, 5, 126, 128, 200]) for _ in range(1500)]
+    c = Case(layer(32, 4), base, [r.choice([0, 1, 2, 9]) for _ in base])
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+def test_captured_graphs_share_a_workspace():
+    """Two layers' steps captured on their own with one workspace, replayed in any order on one stream."""
+    a, b = Case(layer(32, 8), [900, 31], [9, 16]), Case(layer(32, 8, seed=4), [500, 800], [9, 16], seed=8)
+    b.ws = a.ws = a.pk.tree_workspace(2, a.cap, 16, 1024)
+    outs, graphs = [], []
+    for c in (a, b):
+        out = torch.zeros(c.q.shape, device="cuda", dtype=torch.bfloat16)
+        c.run(out=out)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.run(out=out)
+        outs.append(out)
+        graphs.append(g)
+    for i in (0, 1, 1, 0, 0, 1, 0):
+        outs[i].zero_()
+        graphs[i].replay()
+        (a, b)[i].check(outs[i])
