@@ -31,8 +31,8 @@ using namespace pkv;
 
 constexpr int DH = 128, ROWS = 128;                  // head dim; rows of a tile
 constexpr int HALF = 64;                             // tokens per V stage: half a page of one kv head
-constexpr int GROUP = 128;                           // threads of a softmax group: one per row of the tile; two groups, page about
-constexpr int GROUP_WARPS = GROUP / 32;              // what they hand over is counted per warp: 32 arrivals at one word take turns
+constexpr int GROUP = 128;                           // threads of a softmax group: one per row of the tile; two groups, half a page each
+constexpr int SOFT_WARPS = 2 * GROUP / 32;           // what they hand over is counted per warp: 32 arrivals at one word take turns
 constexpr int MAX_G = 8;                             // kv heads of a tile (16 rows at least each)
 constexpr float RESCALE_THRESHOLD = 8.0f;            // in base-2 logits
 constexpr uint32_t WAIT_LIMIT = 1u << 19;            // probes of a bounded wait
@@ -404,16 +404,15 @@ struct Cfg {
 };
 
 struct Shared {                       // at X_OFF
-    uint64_t q_full, q_empty, o_empty, meet;
-    uint64_t p_full[2], pv_done[2], decided[GROUP_WARPS];
+    uint64_t q_full, q_empty, o_empty;
+    uint64_t p_full[2], pv_done[2];
     uint64_t k_full[4], k_empty[4], v_full[7], v_empty[7], v_clean[7], s_full[2], s_empty[2];
     uint64_t r_full[8], r_empty[8], sc_full[2], sc_empty[2], drained[2];
     uint32_t tmem_base;
     volatile int abort_flag;
     Walk start;
-    float row_m[ROWS];                // reference maximum of each row after the last page decided
-    float row_f[2][ROWS];             // per group: rescale factors, then 1 / sum
-    float row_l[2][2][ROWS];          // [stretch & 1][group]: sums at the end
+    float row_f[2][ROWS];             // rescale factors; at the end, per group: 1 / sum
+    float row_l[2][ROWS];             // per group: a page's maxima where a reference moves; sums at the end
     uint32_t bad[3][MAX_G][2];        // [stretch % 3]: drafted tokens whose value row of a kv head is not finite
     int scan[16], red[16][LIST_WORDS];
     int row_o[2][ROWS];               // per group: where a row's result goes, or -1
@@ -443,13 +442,15 @@ __device__ __forceinline__ bool elect_one() {
     return r != 0;
 }
 
-// the 128 threads of a softmax group meet (named barrier 1 or 2); do they learn whether the predicate held in any of them
-__device__ __forceinline__ bool group_any(int group, bool pred) {
+// the 256 softmax threads meet (named barrier 3) and learn whether the predicate held in any of them
+__device__ __forceinline__ bool softmax_any(bool pred) {
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-                 : "=r"(r) : "r"(1 + group), "r"(pred ? 1 : 0) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 3, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                 : "=r"(r) : "r"(pred ? 1 : 0) : "memory");
     return r != 0;
 }
+__device__ __forceinline__ void softmax_sync() { asm volatile("barrier.cta.sync 3, 256;" ::: "memory"); }
+// the 128 threads of a group (named barrier 1 or 2)
 __device__ __forceinline__ void group_sync(int group) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(1 + group) : "memory"); }
 
 // one arrival for the warp, behind everything its lanes did
@@ -518,18 +519,16 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     // (Code that runs once per CTA costs what its bytes take to fetch: it is kept short, loops are left rolled.)
     if (warp == 0) {                                 // lane i takes entry i of every array
         if (lane == 0) {
-            mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, 2 * GROUP_WARPS + 1);
-            mbar_init(&X->o_empty, 2 * GROUP_WARPS); mbar_init(&X->meet, 2 * GROUP_WARPS);
+            mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, SOFT_WARPS + 1); mbar_init(&X->o_empty, SOFT_WARPS);
             X->abort_flag = 0;
             X->start = Walk{0, 0, 0, 0, 0, 0};
         }
-        if (lane < GROUP_WARPS) mbar_init(&X->decided[lane], 1);
         if (lane < 2) {
-            mbar_init(&X->p_full[lane], GROUP_WARPS); mbar_init(&X->pv_done[lane], 1); mbar_init(&X->s_full[lane], 1); mbar_init(&X->s_empty[lane], GROUP_WARPS);
-            mbar_init(&X->sc_full[lane], 1); mbar_init(&X->sc_empty[lane], GROUP_WARPS); mbar_init(&X->drained[lane], 1);
+            mbar_init(&X->p_full[lane], SOFT_WARPS); mbar_init(&X->pv_done[lane], 1); mbar_init(&X->s_full[lane], 1); mbar_init(&X->s_empty[lane], SOFT_WARPS);
+            mbar_init(&X->sc_full[lane], 1); mbar_init(&X->sc_empty[lane], SOFT_WARPS); mbar_init(&X->drained[lane], 1);
         }
         if (lane < C::NK) { mbar_init(&X->k_full[lane], 1); mbar_init(&X->k_empty[lane], 1); }
-        if (lane < C::NV) { mbar_init(&X->v_full[lane], VQ ? 4 : 1); mbar_init(&X->v_empty[lane], 1); mbar_init(&X->v_clean[lane], GROUP_WARPS); }
+        if (lane < C::NV) { mbar_init(&X->v_full[lane], VQ ? 4 : 1); mbar_init(&X->v_empty[lane], 1); mbar_init(&X->v_clean[lane], SOFT_WARPS); }
         if (lane < C::NR) { mbar_init(&X->r_full[lane], 1); mbar_init(&X->r_empty[lane], 4); }
         fence_barrier_init();
     }
@@ -818,16 +817,16 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
         }
     } else if (warp >= 4) {
-        // ================================================================== softmax: a row per thread, two groups of 128 threads
-        // Group 0 takes the even pages of the CTA, group 1 the odd ones: while one waits (for scores, for tensor memory, for the
-        // tensor core to be done with the weights before), the other computes. A row's reference maximum goes from page to
-        // page between the two threads that share the row.
+        // ================================================================== softmax: two threads per row, half of a page's tokens each
+        // Both halves of a page are worked on at the same time, and the tensor core does the next page's scores meanwhile. (A page
+        // per group, the groups taking turns and handing on the rows' references: 57 against 51 us for 4 x 4096 tokens of 32 kv heads,
+        // 184 against 172 us for 16 x 16384 tokens of quantised values; the same for 64 drafts, where the tensor core is the bound.)
         const int quad = warp & 3, grp = (warp - 4) >> 2, r = quad * 32 + lane;
         const uint32_t tl_s = tb + ((uint32_t)(quad * 32) << 16);
         const float* row_scale = reinterpret_cast<const float*>(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE);
-        uint8_t* p_row = smem + C::P_OFF + grp * C::P_BYTES + r * 128;
-        int k = 0, kv = 0, seg = 0, own = -1;        // own: this group's last page
-        bool ok = true;                              // false once any wait of this warp gave up; a group's loop ends for all its warps
+        uint8_t* p_row = smem + C::P_OFF + grp * (C::P_BYTES / 2) + r * 128;
+        int k = 0, kv = 0, seg = 0;
+        bool ok = true;                              // false once any wait of this warp gave up; the loop ends for all warps together
         auto wait_all = [&](uint64_t* bar, uint32_t parity, int where) {
             ok = __all_sync(0xffffffffu, ok && wait_or_abort(bar, parity, X, A.status, where));
         };
@@ -847,39 +846,37 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             float cs = ok ? row_scale[r] * A.col_scale : 0.0f;
             if (cs < 1e-37f) cs = 1e-37f;                               // (keeps NaN; a masked score -inf x cs stays -inf)
             arrive_warp(&X->q_empty);
-            float m = -INFINITY, l = 0.0f;
+            float m = -INFINITY, l = 0.0f;                              // the row's reference (both threads the same), this thread's sum
             for (int p = s.p_lo; p < s.p_hi; ++p, ++k, kv += 2 * ng) {
-                if ((k & 1) != grp) continue;
-                const int drafts = base - p * PKV_PAGE_TOKENS;
-                wait_all(&X->s_full[grp], (k >> 1) & 1, 41);
-                // Weights at the reference that the row had so far, the page's maximum on the way; once the page before has been
-                // decided upon, the reference is looked at again. It only moves when a page exceeds it by 2^8 (its column of O^T is
-                // then rescaled), so the weights are rarely formed a second time (a stretch's first page apart).
+                const int drafts = base - p * PKV_PAGE_TOKENS, buf = k & 1;
+                const bool masked = drafts < (grp + 1) * HALF;
+                const uint32_t s_tm = tl_s + TM_S + 128 * buf + HALF * grp;
+                float2 sum;
+                bool moved = false;
+                wait_all(&X->s_full[buf], (k >> 1) & 1, 41);
+                if constexpr (VQ) wait_all(&X->sc_full[buf], (k >> 1) & 1, 46);
+                if (k >= 2) wait_all(&X->pv_done[buf], ((k >> 1) - 1) & 1, 43);     // the weights of two pages ago have been read
+                tc_fence_after_sync();
+                // Weights at the reference that the row had so far, the page's maximum on the way. The reference only moves when a
+                // page exceeds it by 2^8 (its column of O^T is then rescaled), so the weights are rarely formed a second time (a
+                // stretch's first page apart).
                 // The loop is not unrolled beyond 32 columns: the code of all roles has to fit the instruction cache together, or
                 // each of them runs at the speed of instruction fetch (unrolled over the 128 columns: 192 against 165 us).
-                const bool masked = drafts < PKV_PAGE_TOKENS;
-                const uint32_t s_tm = tl_s + TM_S + 128 * grp;
-                float2 sum;
-                float ref = m, before = -INFINITY;
-                bool grows, again;
-                if constexpr (VQ) wait_all(&X->sc_full[grp], (k >> 1) & 1, 46);
-                if (k >= 2) wait_all(&X->pv_done[grp], ((k >> 1) - 1) & 1, 43);     // the weights of this group's page before have been read
-                tc_fence_after_sync();
 #pragma unroll 1
                 for (bool first_try = true;; first_try = false) {
-                    const float mu = ref > -INFINITY ? ref : 0.0f;      // nothing seen yet: every weight is 2^-inf
+                    const float mu = m > -INFINITY ? m : 0.0f;          // nothing seen yet: every weight is 2^-inf
                     const float2 cs2 = make_float2(cs, cs), mu2 = make_float2(-mu, -mu);
                     float top = -INFINITY;
                     sum = make_float2(0.0f, 0.0f);
 #pragma unroll 1
-                    for (int c = 0; c < 4 && busy; ++c) {
+                    for (int c = 0; c < 2 && busy; ++c) {
                         float x[32];
                         uint32_t w[16];
                         if (ok) tmem_ld32(s_tm + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
                         tmem_ld_wait();
                         uint32_t see = 0u;
                         if (masked) {                                   // tokens that the row does not see
-                            const int j0 = 32 * c - drafts;             // drafted token of the first column (negative: cached)
+                            const int j0 = HALF * grp + 32 * c - drafts;             // drafted token of the first column (negative: cached)
                             see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
@@ -892,7 +889,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         if constexpr (VQ) {
                             // The weight of a token carries its value scale of this row's kv head, and the product is rounded to bf16
                             // (2^-8 of it); the sum takes the weights themselves, which the scale is no part of.
-                            const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + grp * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + c * 64);
+                            const uint4* sc = reinterpret_cast<const uint4*>(smem + C::SC_OFF + buf * C::SC_BYTES + min(gl, ng - 1) * PKV_PAGE_TOKENS * 2 + (2 * grp + c) * 64);
 #pragma unroll
                             for (int u = 0; u < 4; ++u) {
                                 const uint4 q4 = sc[u];
@@ -921,59 +918,56 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                             }
                         }
                         // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, a block per half page
-                        uint8_t* line = p_row + (c >> 1) * (C::P_BYTES / 2);
+                        uint8_t* line = p_row + buf * C::P_BYTES;
 #pragma unroll
                         for (int u = 0; u < 4; ++u)
-                            *reinterpret_cast<uint4*>(line + ((((c & 1) * 4 + u) ^ (r & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
+                            *reinterpret_cast<uint4*>(line + (((c * 4 + u) ^ (r & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                     }
                     if (!first_try) break;
                     top = mine ? top * cs : -INFINITY;                  // (a row that nobody has: whatever its column becomes, nobody reads it)
-                    if (p > s.p_lo) {
-                        wait_all(&X->decided[quad], (k - 1) & 1, 42);
-                        before = X->row_m[r];
-                    }
-                    grows = top > before + RESCALE_THRESHOLD;
-                    const float now = grows ? top : before;
-                    again = __any_sync(0xffffffffu, now != ref);
-                    ref = now;
-                    if (grows || p == s.p_lo) X->row_m[r] = ref;
-                    arrive_warp(&X->decided[quad]);
+                    if (!softmax_any(top > m + RESCALE_THRESHOLD || !ok)) break;
+                    if (softmax_any(!ok)) { go = false; break; }
+                    moved = true;
+                    X->row_l[grp][r] = top;
+                    softmax_sync();
+                    top = fmaxf(top, X->row_l[grp ^ 1][r]);
+                    const float now = top > m + RESCALE_THRESHOLD ? top : m, f = now != m ? exp2f(m - now) : 1.0f;
+                    if (grp == 0) X->row_f[0][r] = f;
+                    l *= f;
+                    const bool again = __any_sync(0xffffffffu, now != m);
+                    m = now;
                     if (!again) break;
                 }
+                if (!go) break;
                 tc_fence_before_sync();
-                arrive_warp(&X->s_empty[grp]);
-                if constexpr (VQ) arrive_warp(&X->sc_empty[grp]);
-                if (ref != m) { l *= exp2f(m - ref); m = ref; }         // (both -inf: equal)
+                arrive_warp(&X->s_empty[buf]);
+                if constexpr (VQ) arrive_warp(&X->sc_empty[buf]);
                 l += sum.x + sum.y;
-                if (group_any(grp, grows || !ok)) {
-                    if (group_any(grp, !ok)) { go = false; break; }     // (the same answer in all warps of the group)
+                if (moved) {
+                    softmax_sync();                                     // row_f is there; row_l may be written again
                     if (p > s.p_lo) {
-                        wait_all(&X->pv_done[grp ^ 1], ((k - 1) >> 1) & 1, 49);         // the accumulators are at rest
-                        X->row_f[grp][r] = grows && before > -INFINITY ? exp2f(before - ref) : 1.0f;
-                        group_sync(grp);
+                        wait_all(&X->pv_done[buf ^ 1], ((k - 1) >> 1) & 1, 49);         // the accumulators are at rest
                         tc_fence_after_sync();
 #pragma unroll 1
-                        for (int c0 = 0; c0 < ng * rph; c0 += 16) {
+                        for (int c0 = 16 * grp; c0 < ng * rph; c0 += 32) {
                             uint32_t o[16];
                             tmem_ld16(tl_s + TM_O + c0, o);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * X->row_f[grp][c0 + c]);
+                            for (int c = 0; c < 16; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * X->row_f[0][c0 + c]);
                             tmem_st16(tl_s + TM_O + c0, o);
                         }
                         tmem_st_wait();
                         tc_fence_before_sync();
-                        group_sync(grp);                                // row_f has been read
                     }
                 }
                 fence_proxy_async_smem();
-                arrive_warp(&X->p_full[grp]);
-                own = k;
+                arrive_warp(&X->p_full[buf]);
                 if constexpr (!VQ) {
                     // Values behind the cached tokens: rows past the sequence become zero, and so does what is not finite in a
                     // drafted row (0 x inf would reach rows that do not see it); who does see it gets NaN at the end.
                     if (drafts < PKV_PAGE_TOKENS && ok) {
-                        if (k > 0) wait_all(&X->pv_done[grp ^ 1], ((k - 1) >> 1) & 1, 50);
+                        if (k > 0) wait_all(&X->pv_done[buf ^ 1], ((k - 1) >> 1) & 1, 50);
                         // (Every tile of such a page is handed over, also one with cached rows only: the page before is known to be
                         // consumed, and within this one the stages then advance in step with these waits.)
                         for (int j = 0; j < 2 * ng; ++j) {
@@ -982,8 +976,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                             if (!ok) break;
                             uint8_t* tile = smem + C::V_OFF + st * C::V_BYTES;
 #pragma unroll 4
-                            for (int it = 0; it < C::V_BYTES / 16 / GROUP && drafts < (h + 1) * HALF; ++it) {
-                                const int id = it * GROUP + r, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
+                            for (int it = 0; it < C::V_BYTES / 32 / GROUP && drafts < (h + 1) * HALF; ++it) {
+                                const int id = (2 * it + grp) * GROUP + r, d = h * HALF + ((id >> 3) & 63) - drafts;      // drafted token of the row
                                 if (d < 0) continue;
                                 uint4* at = reinterpret_cast<uint4*>(tile) + id;
                                 if (d >= s.n) { *at = make_uint4(0u, 0u, 0u, 0u); continue; }
@@ -1004,25 +998,19 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 }
             }
             if (!go) break;
-            // ---- the tile's stretch is done: O^T out of tensor memory, 16 columns by each group in turn
-            // (its own last page first: only neighbouring phases of a barrier can be told apart)
-            if (own >= 0) wait_all(&X->pv_done[grp], (own >> 1) & 1, 44);
+            // ---- the tile's stretch is done: O^T out of tensor memory, 64 columns by each group
             wait_all(&X->pv_done[(k - 1) & 1], ((k - 1) >> 1) & 1, 44);
-            const float M = X->row_m[r];                                // the last page's reference
-            if (m != M) l *= exp2f(m - M);
-            X->row_l[seg & 1][grp][r] = l;
-            if (r < MAX_G * 2) (&X->bad[(seg + 1) % 3][0][0])[r] = 0u;  // (last read before the meeting of the stretch before)
-            arrive_warp(&X->meet);
-            wait_all(&X->meet, seg & 1, 45);                            // both groups
-            if (group_any(grp, !ok)) { go = false; break; }
+            X->row_l[grp][r] = l;
+            if (r < MAX_G * 2) (&X->bad[(seg + 1) % 3][0][0])[r] = 0u;  // (last read two stretches ago)
+            if (softmax_any(!ok)) { go = false; break; }
             tc_fence_after_sync();
             const bool whole = s.p_lo == 0 && s.p_hi == s.pages;
             const size_t slot = (size_t)blockIdx.x * 2 + (s.p_lo == 0);
-            l = X->row_l[seg & 1][0][r] + X->row_l[seg & 1][1][r];
+            l = X->row_l[0][r] + X->row_l[1][r];
             if (!VQ && mine && ((word & 0xffffffffu & X->bad[seg % 3][gl][0]) | ((word >> 32) & X->bad[seg % 3][gl][1]))) l = __int_as_float(0x7fc00000);
             X->row_f[grp][r] = l == 0.0f ? 0.0f : 1.0f / l;             // a row that sees nothing: zeros
             X->row_o[grp][r] = mine ? (s.lo + first + rr / tl.rep) * A.n_q + (s.z % s.t.groups * s.t.G + gl) * tl.rep + rr % tl.rep : -1;
-            if (!whole && mine && grp == 0) A.part_ml[slot * ROWS + r] = make_float2(M, l);
+            if (!whole && mine && grp == 0) A.part_ml[slot * ROWS + r] = make_float2(m, l);
             group_sync(grp);
             // (four columns at a time in a rolled loop: this thread's dim is r)
 #pragma unroll 1
