@@ -48,6 +48,7 @@ constexpr int N_SM = 148;                            // CTAs of the attention la
 
 struct Tiles {
     int rep, Z;                                      // query heads per kv head; most tiles of a sequence
+    uint32_t rep_inv;                                // row / rep = row * rep_inv >> 16 for the rows of a tile
     int quantised;                                   // value pages hold codes
     uint32_t shape[PKV_TREE_MAX + 1];                // by drafted tokens: qpb - 1 | rph / 16 - 1 | G - 1 | groups - 1, 6 + 3 + 3 bits and the rest
     __device__ __forceinline__ Shape of(int n) const {
@@ -163,12 +164,30 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------------------------------------ operand
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
+
 // One residual term of 16 columns: E4M3 scale (in units of the row's `second`) and E2M1 codes; res becomes what is left. The
 // next term is formed from what was stored, so any rounding will do: hardware conversions and an approximate reciprocal.
 __device__ __forceinline__ uint2 residual_term(float (&res)[16], float second, float inv_second, uint8_t& sb, bool more) {
     float am = fabsf(res[0]);
 #pragma unroll
-    for (int i = 1; i < 15; i += 2) asm("max.f32 %0, %1, %2, %3;" : "=f"(am) : "f"(am), "f"(fabsf(res[i])), "f"(fabsf(res[i + 1])));
+    for (int i = 1; i < 15; i += 2) am = max3(am, fabsf(res[i]), fabsf(res[i + 1]));
     am = fmaxf(am, fabsf(res[15]));
     sb = pkv_float_to_e4m3(am * (1.0f / 6.0f) * inv_second);
     const float scale = pkv_e4m3_to_float(sb) * second;
@@ -178,11 +197,13 @@ __device__ __forceinline__ uint2 residual_term(float (&res)[16], float second, f
     uint32_t w[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const float* v = res + 8 * h;
+        float2 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = mul2(make_float2(res[8 * h + 2 * i], res[8 * h + 2 * i + 1]), make_float2(inv, inv));
         asm("{\n\t.reg .b8 a, b, c, d;\n\t"
             "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
             "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\tmov.b32 %0, {a, b, c, d};\n\t}"
-            : "=r"(w[h]) : "f"(v[0] * inv), "f"(v[1] * inv), "f"(v[2] * inv), "f"(v[3] * inv), "f"(v[4] * inv), "f"(v[5] * inv), "f"(v[6] * inv), "f"(v[7] * inv));
+            : "=r"(w[h]) : "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y), "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y));
     }
     if (more) {
 #pragma unroll
@@ -190,9 +211,9 @@ __device__ __forceinline__ uint2 residual_term(float (&res)[16], float second, f
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const __half2_raw p = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)(w[h] >> (8 * i)), __NV_E2M1);
-                const float2 f = __half22float2(__half2(p));
-                res[8 * h + 2 * i] = fmaf(-f.x, scale, res[8 * h + 2 * i]);
-                res[8 * h + 2 * i + 1] = fmaf(-f.y, scale, res[8 * h + 2 * i + 1]);
+                const float2 f = fma2(__half22float2(__half2(p)), make_float2(-scale, -scale), make_float2(res[8 * h + 2 * i], res[8 * h + 2 * i + 1]));
+                res[8 * h + 2 * i] = f.x;
+                res[8 * h + 2 * i + 1] = f.y;
             }
         }
     }
@@ -225,7 +246,8 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     constexpr int NB = WP / 16, NT = AR * NB, RB = WP / 2;
     static_assert(NT == WP, "a thread per column");
     // raw queries and phasors first, later (in the same place) the absorbed rows
-    constexpr int PITCH = WP + 4, FIRST = AR * DH * 4 + AR * DH / 2 * 8, THEN = AR * PITCH * 4;
+    // (a block of 16 absorbed columns takes 20 words: a thread reads a block, and the blocks of a row then start in different banks)
+    constexpr int PITCH = NB * 20 + 4, FIRST = AR * DH * 4 + AR * DH / 2 * 8, THEN = AR * PITCH * 4;
     __shared__ __align__(16) uint8_t both[FIRST > THEN ? FIRST : THEN];
     __shared__ float2 zq[AR][DH / 2];
     __shared__ int sums[NT / 32][LIST_WORDS];
@@ -274,7 +296,8 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     const int rows = min(AR, nq * rep - rr0);
     if (nq <= 0 || r0 / t.rph >= t.G || g >= L.n_kv || rows <= 0) return;
     // this CTA's rows belong to the drafted tokens q_lo .. q_hi
-    const int q_lo = rr0 / rep, q_hi = (rr0 + rows - 1) / rep;
+    auto token = [&](int row) { return (int)(row * A.X.rep_inv >> 16); };
+    const int q_lo = token(rr0), q_hi = token(rr0 + rows - 1);
     // the factors of this thread's column, used for all rows
     const int R = L.R, W = 2 * R + L.R_s, c = tid;
     int f = 0;
@@ -287,19 +310,20 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     }
     // tiers: the cache's block is in units of its own scale while the attention applies the layer's one
     if (L.second_blocks_dev && c < W) tier = L.second_blocks_dev[c >> 4] / L.second;
-#pragma unroll 1
-    for (int k = tid; k < rows * (DH / 4); k += NT) {
-        const int r = k / (DH / 4), d = k % (DH / 4) * 4, rr = rr0 + r;
-        const size_t o = ((size_t)(lo + first + rr / rep) * L.n_q + g * rep + rr % rep) * DH + d;
-        float4 v;
+    constexpr int QL = AR * (DH / 4) / NT;               // four dims at a time; all loads of a thread in flight
+    float4 qv[QL];
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+        const int k = tid + i * NT, r = k / (DH / 4), d = k % (DH / 4) * 4, rr = rr0 + r, tk = token(rr);
+        const size_t o = ((size_t)(lo + first + tk) * L.n_q + g * rep + rr - tk * rep) * DH + d;
+        if (r >= rows) continue;
         if (A.q_bf16) {
             const uint2 u = *reinterpret_cast<const uint2*>((const uint16_t*)A.q + o);
-            v = make_float4(pkv_bf16_bits_to_float(u.x & 0xffffu), pkv_bf16_bits_to_float(u.x >> 16), pkv_bf16_bits_to_float(u.y & 0xffffu),
-                            pkv_bf16_bits_to_float(u.y >> 16));
+            qv[i] = make_float4(pkv_bf16_bits_to_float(u.x & 0xffffu), pkv_bf16_bits_to_float(u.x >> 16), pkv_bf16_bits_to_float(u.y & 0xffffu),
+                                pkv_bf16_bits_to_float(u.y >> 16));
         } else {
-            v = *reinterpret_cast<const float4*>((const float*)A.q + o);
+            qv[i] = *reinterpret_cast<const float4*>((const float*)A.q + o);
         }
-        *reinterpret_cast<float4*>(&raw[r][d]) = v;
     }
     // Phasors: the angle as a number of turns in 64 bits, of which only the fraction counts; that is exact enough in 32 bits
     // (2^-25 of a turn) and needs no long range reduction (the operand's own residual is 7e-5).
@@ -311,11 +335,16 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
         sincospif(2.0f * (float)(turns - rint(turns)), &sn, &cs);
         ph[k / (DH / 2)][j] = make_float2(L.attn_scale * cs, L.attn_scale * sn);
     }
+#pragma unroll
+    for (int i = 0; i < QL; ++i) {
+        const int k = tid + i * NT;
+        if (k / (DH / 4) < rows) *reinterpret_cast<float4*>(&raw[k / (DH / 4)][k % (DH / 4) * 4]) = qv[i];
+    }
     __syncthreads();
-#pragma unroll 1
+#pragma unroll 2
     for (int k = tid; k < rows * (DH / 2); k += NT) {
         const int r = k / (DH / 2), j = k % (DH / 2);
-        const float2 p = ph[(rr0 + r) / rep - q_lo][j];
+        const float2 p = ph[token(rr0 + r) - q_lo][j];
         const float x = raw[r][j], y = raw[r][j + DH / 2];
         zq[r][j] = make_float2(x * p.x - y * p.y, x * p.y + y * p.x);
     }
@@ -332,31 +361,33 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
         }
     }
     __syncthreads();                                 // the raw queries are done with
+    // conj(A) zq: (ar x + ai y, ar y - ai x), of which the column has one; padding: 0
+    const float ax = c < R ? ar : -ai, ay = c < R ? ai : ar;
+    float* column = &qa[0][(c >> 4) * 20 + (c & 15)];
 #pragma unroll
     for (int r = 0; r < AR; ++r) {
-        if (c < 2 * R) {                             // conj(A) zq
+        if (c < 2 * R) {
             const float2 w = zq[r][f];
-            acc[r] = c < R ? ar * w.x + ai * w.y : ar * w.y - ai * w.x;
+            acc[r] = fmaf(ax, w.x, ay * w.y);
         }
-        qa[r][c] = acc[r] * tier;                    // (padding: 0)
+        column[r * PITCH] = acc[r] * tier;
     }
     __syncthreads();
     const int r = tid / NB, j = tid % NB;            // from here on: a 16-column block of a row per thread
     const bool live = r < rows;
-    float res[16], am = 0.0f;
-    bool fine = true;
+    float res[16];
+    float2 none = make_float2(0.0f, 0.0f);           // NaN as soon as a value is not finite
 #pragma unroll
-    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(&res[4 * i]) = *reinterpret_cast<const float4*>(&qa[r][j * 16 + 4 * i]);
+    for (int i = 0; i < 4; ++i) *reinterpret_cast<float4*>(&res[4 * i]) = *reinterpret_cast<const float4*>(&qa[r][j * 20 + 4 * i]);
+    float am = fmaxf(fabsf(res[0]), fabsf(res[15]));
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        am = fmaxf(am, fabsf(res[i]));
-        fine = fine && fabsf(res[i]) < INFINITY;
-    }
+    for (int i = 0; i < 16; i += 2) none = fma2(make_float2(res[i], res[i + 1]), make_float2(0.0f, 0.0f), none);
 #pragma unroll
-    for (int o = NB / 2; o; o >>= 1) {
-        am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
-        fine = __shfl_xor_sync(0xffffffffu, fine ? 1 : 0, o) && fine;
-    }
+    for (int i = 1; i < 15; i += 2) am = max3(am, fabsf(res[i]), fabsf(res[i + 1]));
+#pragma unroll
+    for (int o = NB / 2; o; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
+    const uint32_t bad = __ballot_sync(0xffffffffu, !(none.x + none.y == 0.0f));
+    const bool fine = (bad >> ((tid & 31) / NB * NB) & ((1u << NB) - 1)) == 0;
     if (!live) return;
     const float second = fmaxf(am, 1e-30f) * (1.0f / (448.0f * 6.0f)), inv = __frcp_rn(second);
     uint8_t* blob = A.blobs + ((size_t)b * A.X.Z + z) * blob_bytes(WP);
@@ -464,23 +495,6 @@ __device__ __forceinline__ float ex2_fast(float x) {     // 2 ulp, results below
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// two fp32 operations per instruction
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)), "l"(*reinterpret_cast<unsigned long long*>(&c)));
-    return d;
-}
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-    return d;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(*reinterpret_cast<unsigned long long*>(&d)) : "l"(*reinterpret_cast<unsigned long long*>(&a)), "l"(*reinterpret_cast<unsigned long long*>(&b)));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) { float d; asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c)); return d; }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -1166,6 +1180,7 @@ Tiles make_tiles(int n_q, int n_kv, int max_draft, bool quantised) {
     Tiles X;
     X.quantised = quantised;
     X.rep = n_q / n_kv;
+    X.rep_inv = 65536 / X.rep + 1;                   // (rows below 128, rep <= 64: 128 / 65536 < 1 / 64)
     X.Z = 1;
     X.shape[0] = 0;
     const int most = ROWS / X.rep;
