@@ -435,18 +435,18 @@ struct Cfg {
 };
 
 struct Shared {                       // at X_OFF
-    uint64_t q_full, q_empty, o_empty;
+    uint64_t q_full[PKV_QUERY_TERMS], q_empty, o_empty;
     uint64_t p_full[2], pv_done[2];
     uint64_t k_full[4], k_empty[4], v_full[7], v_empty[7], v_clean[7], s_full[2], s_empty[2];
     uint64_t r_full[8], r_empty[8], sc_full[2], sc_empty[2], drained[2];
     uint32_t tmem_base;
     volatile int abort_flag;
     Walk start;
-    float row_f[2][ROWS];             // rescale factors; at the end, per group: 1 / sum
+    alignas(16) float row_f[2][ROWS]; // rescale factors; at the end, per group: 1 / sum
     float row_l[2][ROWS];             // per group: a page's maxima where a reference moves; sums at the end
     uint32_t bad[3][MAX_G][2];        // [stretch % 3]: drafted tokens whose value row of a kv head is not finite
     int scan[16], red[16][LIST_WORDS];
-    int row_o[2][ROWS];               // per group: where a row's result goes, or -1
+    alignas(16) int row_o[2][ROWS];   // per group: where a row's result goes, or -1
 };
 static_assert(sizeof(Shared) <= 6144, "behind the stages");
 
@@ -533,10 +533,11 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
     // (Code that runs once per CTA costs what its bytes take to fetch: it is kept short, loops are left rolled.)
     if (warp == 0) {                                 // lane i takes entry i of every array
         if (lane == 0) {
-            mbar_init(&X->q_full, 1); mbar_init(&X->q_empty, SOFT_WARPS + 1); mbar_init(&X->o_empty, SOFT_WARPS);
+            mbar_init(&X->q_empty, SOFT_WARPS + 1); mbar_init(&X->o_empty, SOFT_WARPS);
             X->abort_flag = 0;
             X->start = Walk{0, 0, 0, 0, 0, 0};
         }
+        if (lane < PKV_QUERY_TERMS) mbar_init(&X->q_full[lane], 1);
         if (lane < 2) {
             mbar_init(&X->p_full[lane], SOFT_WARPS); mbar_init(&X->pv_done[lane], 1); mbar_init(&X->s_full[lane], 1); mbar_init(&X->s_empty[lane], SOFT_WARPS);
             mbar_init(&X->sc_full[lane], 1); mbar_init(&X->sc_empty[lane], SOFT_WARPS); mbar_init(&X->drained[lane], 1);
@@ -630,10 +631,12 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         if (!waited) { pkv_grid_wait(); waited = true; }
                         asm volatile("fence.proxy.async;" ::: "memory");   // written by ordinary stores, read by the copy engine
                         const long blob = (long)s.b * tl.Z + s.z;
-                        mbar_arrive_expect_tx(&X->q_full, blob_bytes(WP));
-                        for (int t = 0; t < PKV_QUERY_TERMS; ++t)
-                            tma_load_2d(smem + C::Q_OFF + t * C::PAGE, &qmap, 0, (int)(blob * (blob_bytes(WP) / 128) + t * (C::PAGE / 128)), &X->q_full);
-                        bulk_g2s(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE, A.blobs + blob * blob_bytes(WP) + PKV_QUERY_TERMS * C::PAGE, ROWS * 4, &X->q_full);
+                        for (int t = 0; t < PKV_QUERY_TERMS; ++t) {    // (the scores of a term begin when it is there)
+                            const bool last = t + 1 == PKV_QUERY_TERMS;
+                            mbar_arrive_expect_tx(&X->q_full[t], C::PAGE + (last ? ROWS * 4 : 0));
+                            tma_load_2d(smem + C::Q_OFF + t * C::PAGE, &qmap, 0, (int)(blob * (blob_bytes(WP) / 128) + t * (C::PAGE / 128)), &X->q_full[t]);
+                            if (last) bulk_g2s(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE, A.blobs + blob * blob_bytes(WP) + PKV_QUERY_TERMS * C::PAGE, ROWS * 4, &X->q_full[t]);
+                        }
                         ++seg;
                     }
                     if constexpr (VQ) {
@@ -651,7 +654,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             }
             if (!waited) pkv_grid_wait();
             if (X->abort_flag) {                                        // copies in flight land before anyone leaves
-                if (seg > 0) mbar_wait(&X->q_full, (seg - 1) & 1, 1u << 16);
+                for (int t = 0; t < PKV_QUERY_TERMS && seg > 0; ++t) mbar_wait(&X->q_full[t], (seg - 1) & 1, 1u << 16);
                 for (int j = max(0, k - C::NK); j < k; ++j) mbar_wait(&X->k_full[j % C::NK], (j / C::NK) & 1, 1u << 16);
                 for (int j = max(0, n_sc - 2); j < n_sc; ++j) mbar_wait(&X->sc_full[j & 1], (j >> 1) & 1, 1u << 16);
             }
@@ -710,14 +713,6 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
         };
         while (ok && walk.next(A.B, tl, zi, s)) {
             const int p_lo = uniform(s.p_lo), p_hi = uniform(s.p_hi);
-            wait(&X->q_full, seg & 1, 30);
-            if (!ok) break;
-            tc_fence_after_sync();
-            if (leader)
-#pragma unroll 1
-                for (int t = 0; t < PKV_QUERY_TERMS; ++t)
-                    for (int c = 0; c < C::KB; ++c)
-                        tmem_cp_32x128b_warpx4(tb + TM_SFA + (t * C::KB + c) * 4, smem_desc(sbase + C::Q_OFF + t * C::PAGE + C::CODES + c * 512, 0, 128, SWZ_NONE));
             for (int p = p_lo; p < p_hi; ++p, ++k) {
                 const int st = k % C::NK, sb = k & 1;
                 wait(&X->k_full[st], (k / C::NK) & 1, 33);
@@ -726,15 +721,29 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 tc_fence_after_sync();
                 const uint32_t ka = sbase + C::K_OFF + st * C::PAGE, sfb = tb + TM_SFB + 16 * sb;
                 const uint64_t k_desc = smem_desc(ka, 0, 8 * C::RB, C::SWZ), sf_desc = smem_desc(ka + C::CODES, 0, 128, SWZ_NONE);
-                if (leader) {
+                if (leader)
 #pragma unroll
                     for (int c = 0; c < C::KB; ++c) tmem_cp_32x128b_warpx4(sfb + 4 * c, sf_desc + (uint64_t)(c * 512 / 16));
+#pragma unroll 1
+                for (int t = 0; t < PKV_QUERY_TERMS; ++t) {
+                    if (p == p_lo) {                     // the tile's operand arrives term by term
+                        wait(&X->q_full[t], seg & 1, 30);
+                        if (!ok) break;
+                        tc_fence_after_sync();
+                        if (leader)
 #pragma unroll
-                    for (int t = 0; t < PKV_QUERY_TERMS; ++t)
+                            for (int c = 0; c < C::KB; ++c)
+                                tmem_cp_32x128b_warpx4(tb + TM_SFA + (t * C::KB + c) * 4, smem_desc(sbase + C::Q_OFF + t * C::PAGE + C::CODES + c * 512, 0, 128, SWZ_NONE));
+                        __syncwarp();
+                    }
+                    if (leader)
 #pragma unroll
                         for (int c = 0; c < C::KB; ++c)
                             mma_nvfp4(tb + TM_S + 128 * sb, q_desc + (uint64_t)((t * C::PAGE + c * 32) / 16), k_desc + (uint64_t)(c * 32 / 16), idesc_s,
                                       tb + TM_SFA + (t * C::KB + c) * 4, sfb + 4 * c, t != 0 || c != 0);
+                }
+                if (!ok) break;
+                if (leader) {
                     tc_commit(&X->k_empty[st]);
                     tc_commit(&X->s_full[sb]);
                     if (p + 1 == p_hi) tc_commit(&X->q_empty);
@@ -856,7 +865,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 word = A.mask ? (unsigned long long)A.mask[s.lo + i] : (i >= 63 ? ~0ull : (2ull << i) - 1);
                 if (s.n < 64) word &= (1ull << s.n) - 1;
             }
-            wait_all(&X->q_full, seg & 1, 40);
+            wait_all(&X->q_full[PKV_QUERY_TERMS - 1], seg & 1, 40);      // (the rows' scales come with the last term)
             float cs = ok ? row_scale[r] * A.col_scale : 0.0f;
             if (cs < 1e-37f) cs = 1e-37f;                               // (keeps NaN; a masked score -inf x cs stays -inf)
             arrive_warp(&X->q_empty);
@@ -866,14 +875,14 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 const bool masked = drafts < (grp + 1) * HALF;
                 const uint32_t s_tm = tl_s + TM_S + 128 * buf + HALF * grp;
                 float2 sum;
+                const bool opening = p == s.p_lo;
                 bool moved = false;
                 wait_all(&X->s_full[buf], (k >> 1) & 1, 41);
                 if constexpr (VQ) wait_all(&X->sc_full[buf], (k >> 1) & 1, 46);
                 if (k >= 2) wait_all(&X->pv_done[buf], ((k >> 1) - 1) & 1, 43);     // the weights of two pages ago have been read
                 tc_fence_after_sync();
                 // Weights at the reference that the row had so far, the page's maximum on the way. The reference only moves when a
-                // page exceeds it by 2^8 (its column of O^T is then rescaled), so the weights are rarely formed a second time (a
-                // stretch's first page apart).
+                // page exceeds it by 2^8 (its column of O^T is then rescaled), so the weights are rarely formed a second time.
                 // The loop is not unrolled beyond 32 columns: the code of all roles has to fit the instruction cache together, or
                 // each of them runs at the speed of instruction fetch (unrolled over the 128 columns: 192 against 165 us).
 #pragma unroll 1
@@ -900,6 +909,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
 #pragma unroll
                         for (int e = 1; e < 31; e += 2) mx[(e >> 1) & 1] = max3(mx[(e >> 1) & 1], x[e], x[e + 1]);
                         top = max3(mx[0], mx[1], x[31]);
+                        if (opening && first_try) continue;             // no reference yet: the maximum alone
                         if constexpr (VQ) {
                             // The weight of a token carries its value scale of this row's kv head, and the product is rounded to bf16
                             // (2^-8 of it); the sum takes the weights themselves, which the scale is no part of.
@@ -939,7 +949,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     }
                     if (!first_try) break;
                     top = mine ? top * cs : -INFINITY;                  // (a row that nobody has: whatever its column becomes, nobody reads it)
-                    if (!softmax_any(top > m + RESCALE_THRESHOLD || !ok)) break;
+                    if (!opening && !softmax_any(top > m + RESCALE_THRESHOLD || !ok)) break;
                     if (softmax_any(!ok)) { go = false; break; }
                     moved = true;
                     X->row_l[grp][r] = top;
@@ -948,7 +958,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     const float now = top > m + RESCALE_THRESHOLD ? top : m, f = now != m ? exp2f(m - now) : 1.0f;
                     if (grp == 0) X->row_f[0][r] = f;
                     l *= f;
-                    const bool again = __any_sync(0xffffffffu, now != m);
+                    const bool again = opening || __any_sync(0xffffffffu, now != m);
                     m = now;
                     if (!again) break;
                 }
@@ -959,7 +969,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 l += sum.x + sum.y;
                 if (moved) {
                     softmax_sync();                                     // row_f is there; row_l may be written again
-                    if (p > s.p_lo) {
+                    if (!opening) {
                         wait_all(&X->pv_done[buf ^ 1], ((k - 1) >> 1) & 1, 49);         // the accumulators are at rest
                         tc_fence_after_sync();
 #pragma unroll 1
@@ -1026,18 +1036,24 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
             X->row_o[grp][r] = mine ? (s.lo + first + rr / tl.rep) * A.n_q + (s.z % s.t.groups * s.t.G + gl) * tl.rep + rr % tl.rep : -1;
             if (!whole && mine && grp == 0) A.part_ml[slot * ROWS + r] = make_float2(m, l);
             group_sync(grp);
-            // (four columns at a time in a rolled loop: this thread's dim is r)
+            // (16 columns at a time in a rolled loop: this thread's dim is r)
 #pragma unroll 1
-            for (int c0 = 64 * grp; c0 < min(ng * rph, 64 * grp + 64); c0 += 4) {
-                uint32_t o[4];
-                tmem_ldn<4>(tl_s + TM_O + c0, o);
+            for (int c0 = 64 * grp; c0 < min(ng * rph, 64 * grp + 64); c0 += 16) {
+                uint32_t o[16];
+                tmem_ld16(tl_s + TM_O + c0, o);
                 tmem_ld_wait();
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const int to = X->row_o[grp][c0 + c];
-                    if (to < 0) continue;
-                    if (whole) A.out[(size_t)to * DH + r] = __float2bfloat16(__uint_as_float(o[c]) * X->row_f[grp][c0 + c]);
-                    else A.part_o[(slot * ROWS + c0 + c) * DH + r] = __uint_as_float(o[c]);
+                for (int c4 = 0; c4 < 16; c4 += 4) {
+                    const int4 t4 = *reinterpret_cast<const int4*>(&X->row_o[grp][c0 + c4]);
+                    const float4 f4 = *reinterpret_cast<const float4*>(&X->row_f[grp][c0 + c4]);
+                    const int to[4] = {t4.x, t4.y, t4.z, t4.w};
+                    const float f[4] = {f4.x, f4.y, f4.z, f4.w};
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        if (to[c] < 0) continue;
+                        if (whole) A.out[(size_t)to[c] * DH + r] = __float2bfloat16(__uint_as_float(o[c4 + c]) * f[c]);
+                        else A.part_o[(slot * ROWS + c0 + c4 + c) * DH + r] = __uint_as_float(o[c4 + c]);
+                    }
                 }
             }
             tc_fence_before_sync();
