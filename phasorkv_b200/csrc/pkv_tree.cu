@@ -83,7 +83,7 @@ struct Batch {
 //   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts: 104 us; tiles of one shape, by the most
 //   drafts, and gangs of them: 130 us).
 struct List { int gang, gangs, U; };                 // gang: CTAs, or 0 for CTAs on their own
-constexpr int LIST_WORDS = 6;
+constexpr int LIST_WORDS = 4;
 
 __device__ __forceinline__ int passes_of(const Shape& t, int gang) { return gang == 0 ? t.Z : (t.Z + gang - 1) / gang; }
 __device__ __forceinline__ int cost_of(const Shape& t, int gang) { return gang == 0 ? t.cost : 1; }
@@ -92,7 +92,7 @@ __device__ __forceinline__ int cost_of(const Shape& t, int gang) { return gang =
 // (its only one, in batches of at most nt)
 __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid, int nt, int (*red)[LIST_WORDS], int2& last) {
     last = make_int2(0, 0);
-    int v[LIST_WORDS] = {0, 0, 0, 0, 1 << 30, 1 << 30};      // pages, pages x tiles x cost, most tiles, most pages, fewest of each
+    int v[LIST_WORDS] = {0, 0, 0, 1 << 30};          // pages, pages x tiles x cost, most tiles, fewest tiles
 #pragma unroll 1
     for (int b = tid; b < B.batch; b += nt) {
         int lo, n, T;
@@ -102,11 +102,10 @@ __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid,
         const Shape t = X.of(n);
         const int Z = t.Z;
         v[0] += pages; v[1] += pages * Z * t.cost;
-        v[2] = max(v[2], Z); v[3] = max(v[3], pages); v[4] = min(v[4], Z); v[5] = min(v[5], pages);
+        v[2] = max(v[2], Z); v[3] = min(v[3], Z);
     }
     v[0] = __reduce_add_sync(0xffffffffu, v[0]); v[1] = __reduce_add_sync(0xffffffffu, v[1]);
-    v[2] = __reduce_max_sync(0xffffffffu, v[2]); v[3] = __reduce_max_sync(0xffffffffu, v[3]);
-    v[4] = __reduce_min_sync(0xffffffffu, v[4]); v[5] = __reduce_min_sync(0xffffffffu, v[5]);
+    v[2] = __reduce_max_sync(0xffffffffu, v[2]); v[3] = __reduce_min_sync(0xffffffffu, v[3]);
     if ((tid & 31) == 0)
 #pragma unroll
         for (int i = 0; i < LIST_WORDS; ++i) red[tid >> 5][i] = v[i];
@@ -115,17 +114,13 @@ __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid,
     for (int w = 0; w < min(nt, B.batch + 31) / 32; ++w) {     // (the other warps have none)
         if (w == (tid >> 5)) continue;
         v[0] += red[w][0]; v[1] += red[w][1];
-        v[2] = max(v[2], red[w][2]); v[3] = max(v[3], red[w][3]); v[4] = min(v[4], red[w][4]); v[5] = min(v[5], red[w][5]);
+        v[2] = max(v[2], red[w][2]); v[3] = min(v[3], red[w][3]);
     }
     List y;
     const int passes = (v[2] + 15) >> 4;
-    y.gang = v[2] == v[4] ? (v[2] + passes - 1) / passes : 0;
+    y.gang = v[2] == v[3] ? (v[2] + passes - 1) / passes : 0;
     y.gangs = y.gang ? N_SM / y.gang : N_SM;
-    y.U = v[2] == v[4] ? v[0] * passes : v[1];
-    if (v[2] == v[4] && v[3] == v[5] && v[3] > 0) {          // sequences of one length: no stretch across two of them if few SMs idle for it
-        const int whole = y.U / v[3], even = y.gangs >= whole ? y.gangs / whole * whole : 0;
-        if ((y.gangs - even) * 8 <= y.gangs) y.gangs = even;
-    }
+    y.U = v[2] == v[3] ? v[0] * passes : v[1];
     y.gangs = min(y.gangs, y.gang ? y.U : max(y.U / COST_MOST, min(y.U, 1)));      // (a stretch that is not its tile's first or last has a page)
     return y;
 }
@@ -412,12 +407,15 @@ constexpr uint32_t TM_SFA = 384;      // 4 per (term, K step): scales of the que
 constexpr uint32_t TM_SFB = 448;      // 2 x 16: scales of the page
 constexpr uint32_t TM_COLS = 512;
 
-template <int WP, bool VQ>
+// MANY: tiles of two kv heads or more. Their values are most of what a page brings, and the page after next can wait: one latent page and
+// four stages of values instead of two and three (16 x 16384 tokens, 6 drafts, 4 kv heads per tile: 140 -> 123 us; 32 drafts of one kv
+// head per tile: 134 -> 150 us).
+template <int WP, bool VQ, bool MANY>
 struct Cfg {
     static constexpr int RB = WP / 2, KB = WP / 64, PAGE = page_bytes(WP), CODES = PKV_PAGE_TOKENS * RB;
-    static constexpr int NK = WP == 256 ? 2 : 4;                                  // latent pages in flight
+    static constexpr int NK = WP == 256 ? (MANY ? 1 : 2) : 4;                                  // latent pages in flight
     // V operand stages (64 tokens of a kv head, bf16) and, of quantised V, raw stages: what is left of the shared memory
-    static constexpr int NV = VQ ? (WP == 256 ? 2 : 3) : (WP == 256 ? 3 : 5);
+    static constexpr int NV = VQ ? (WP == 256 ? 2 : 3) : (WP == 256 ? (MANY ? 4 : 3) : 5);
     static constexpr int NR = VQ ? (WP == 256 ? 3 : 8) : 0;
     static constexpr int V_BYTES = HALF * DH * 2, RAW_BYTES = HALF * DH / 2, P_BYTES = ROWS * PKV_PAGE_TOKENS * 2;
     static constexpr int SC_BYTES = MAX_G * PKV_PAGE_TOKENS * 2;                  // token scales of a page
@@ -431,6 +429,7 @@ struct Cfg {
     static constexpr int SMEM = X_OFF + 6144;
     static constexpr int NTHREADS = VQ ? 512 : 384;
     static constexpr uint64_t SWZ = RB == 128 ? SWZ_128B : SWZ_64B;
+    static_assert(!MANY || (WP == 256 && !VQ), "of wide rows and bf16 values alone");
     static_assert(SMEM <= 232448 && V_OFF % 1024 == 0 && P_OFF % 1024 == 0, "shared memory of a CTA");
 };
 
@@ -517,11 +516,11 @@ struct AttnArgs {
     int32_t* status;
 };
 
-template <int WP, bool VQ>
-__global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel(const __grid_constant__ CUtensorMap kmap,
+template <int WP, bool VQ, bool MANY>
+__global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_kernel(const __grid_constant__ CUtensorMap kmap,
                                                                                  const __grid_constant__ CUtensorMap qmap,
                                                                                  const __grid_constant__ CUtensorMap vmap, const __grid_constant__ AttnArgs A) {
-    using C = Cfg<WP, VQ>;
+    using C = Cfg<WP, VQ, MANY>;
     extern __shared__ __align__(1024) uint8_t smem[];
     Shared* X = reinterpret_cast<Shared*>(smem + C::X_OFF);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -799,8 +798,9 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
         drain(leader, 1);
     } else if (VQ && warp >= 12) {
         // ================================================================== quantised values -> bf16 operand tiles
-        // Every E2M1 level is a bf16 number; the token's scale goes into the softmax weight. 128 threads, two per token.
-        const int r = (tid - 384) >> 1, part = tid & 1;
+        // Every E2M1 level is a bf16 number; the token's scale goes into the softmax weight. 128 threads, two per token, eight tokens
+        // side by side, so that the eight lanes of a store have the eight chunks of a swizzled line.
+        const int r = (tid - 384) / 32 * 16 + (lane >> 4) * 8 + (lane & 7), part = lane >> 3 & 1;
         auto prmt = [](uint32_t a, uint32_t b, uint32_t c) -> uint32_t {
             uint32_t d;
             asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -877,9 +877,15 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 float2 sum;
                 const bool opening = p == s.p_lo;
                 bool moved = false;
-                wait_all(&X->s_full[buf], (k >> 1) & 1, 41);
-                if constexpr (VQ) wait_all(&X->sc_full[buf], (k >> 1) & 1, 46);
-                if (k >= 2) wait_all(&X->pv_done[buf], ((k >> 1) - 1) & 1, 43);     // the weights of two pages ago have been read
+                // scores, value scales, and the weights of two pages ago read: usually all there, one vote then
+                bool there = mbar_try_wait(&X->s_full[buf], (k >> 1) & 1);
+                if constexpr (VQ) there = there && mbar_try_wait(&X->sc_full[buf], (k >> 1) & 1);
+                if (k >= 2) there = there && mbar_try_wait(&X->pv_done[buf], ((k >> 1) - 1) & 1);
+                if (!__all_sync(0xffffffffu, there)) {
+                    wait_all(&X->s_full[buf], (k >> 1) & 1, 41);
+                    if constexpr (VQ) wait_all(&X->sc_full[buf], (k >> 1) & 1, 46);
+                    if (k >= 2) wait_all(&X->pv_done[buf], ((k >> 1) - 1) & 1, 43);
+                }
                 tc_fence_after_sync();
                 // Weights at the reference that the row had so far, the page's maximum on the way. The reference only moves when a
                 // page exceeds it by 2^8 (its column of O^T is then rescaled), so the weights are rarely formed a second time.
@@ -898,7 +904,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                         if (ok) tmem_ld32(s_tm + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&x[0]));
                         tmem_ld_wait();
                         uint32_t see = 0u;
-                        if (masked) {                                   // tokens that the row does not see
+                        if (__builtin_expect(masked, false)) {                                   // tokens that the row does not see
                             const int j0 = HALF * grp + 32 * c - drafts;             // drafted token of the first column (negative: cached)
                             see = j0 >= 0 ? (j0 < 64 ? (uint32_t)(word >> j0) : 0u) : (j0 > -32 ? (uint32_t)(word << -j0) | ((1u << -j0) - 1) : ~0u);
 #pragma unroll
@@ -949,7 +955,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                     }
                     if (!first_try) break;
                     top = mine ? top * cs : -INFINITY;                  // (a row that nobody has: whatever its column becomes, nobody reads it)
-                    if (!opening && !softmax_any(top > m + RESCALE_THRESHOLD || !ok)) break;
+                    if (__builtin_expect(!opening && !softmax_any(top > m + RESCALE_THRESHOLD || !ok), true)) break;
                     if (softmax_any(!ok)) { go = false; break; }
                     moved = true;
                     X->row_l[grp][r] = top;
@@ -967,7 +973,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 arrive_warp(&X->s_empty[buf]);
                 if constexpr (VQ) arrive_warp(&X->sc_empty[buf]);
                 l += sum.x + sum.y;
-                if (moved) {
+                if (__builtin_expect(moved, false)) {
                     softmax_sync();                                     // row_f is there; row_l may be written again
                     if (!opening) {
                         wait_all(&X->pv_done[buf ^ 1], ((k - 1) >> 1) & 1, 49);         // the accumulators are at rest
@@ -990,7 +996,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ>::NTHREADS, 1) pkv_tree_attn_kernel
                 if constexpr (!VQ) {
                     // Values behind the cached tokens: rows past the sequence become zero, and so does what is not finite in a
                     // drafted row (0 x inf would reach rows that do not see it); who does see it gets NaN at the end.
-                    if (drafts < PKV_PAGE_TOKENS && ok) {
+                    if (__builtin_expect(drafts < PKV_PAGE_TOKENS && ok, false)) {
                         if (k > 0) wait_all(&X->pv_done[buf ^ 1], ((k - 1) >> 1) & 1, 50);
                         // (Every tile of such a page is handed over, also one with cached rows only: the page before is known to be
                         // consumed, and within this one the stages then advance in step with these waits.)
@@ -1222,9 +1228,9 @@ Layout make_layout(const Tiles& X, int batch, int WP) {
     return y;
 }
 
-template <int WP, bool VQ>
+template <int WP, bool VQ, bool MANY>
 int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, const AttnArgs& at, size_t blob_rows, cudaStream_t st) {
-    using C = Cfg<WP, VQ>;
+    using C = Cfg<WP, VQ, MANY>;
     const Tiles& X = ab.X;
     CUtensorMap kmap, qmap, vmap;
     int rc = encode_map(&kmap, cache->latent_dev, (uint64_t)cache->n_pages * (C::PAGE / 128), C::PAGE / 128, false);
@@ -1233,9 +1239,9 @@ int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, const AttnArgs& at, s
                      : encode_map(&vmap, cache->v_dev, (uint64_t)cache->n_pages * cache->n_kv * PKV_PAGE_TOKENS, HALF, true);
     if (rc) return rc;
     static pkv_attr_flags attr;
-    PKV_CUDA_TRY(pkv_set_max_smem(pkv_tree_attn_kernel<WP, VQ>, C::SMEM, attr));
+    PKV_CUDA_TRY(pkv_set_max_smem(pkv_tree_attn_kernel<WP, VQ, MANY>, C::SMEM, attr));
     PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_absorb_kernel<WP>, dim3(ROWS / AR + 1, X.Z, ab.B.batch), dim3(AR * WP / 16), 0, st, ab));
-    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ>, dim3(N_SM), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
+    PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ, MANY>, dim3(N_SM), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
     // stretches of a tile, if all sequences have as many tiles and pages: the more, the more warps share a row's
     const int parts = N_SM / (ab.B.batch * X.Z) + 1;
     const dim3 block(256);
@@ -1297,6 +1303,8 @@ extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache,
     at.part_o = (float*)(ws + y.part_o); at.part_ml = (float2*)(ws + y.part_ml); at.first_page = (int32_t*)(ws + y.first_page);
     at.out = (__nv_bfloat16*)out_dev; at.status = status_dev;
     cudaStream_t s = (cudaStream_t)stream;
-    if (cache->v_bits) return WP == 256 ? launch<256, true>(cache, ab, at, blob_rows, s) : launch<128, true>(cache, ab, at, blob_rows, s);
-    return WP == 256 ? launch<256, false>(cache, ab, at, blob_rows, s) : launch<128, false>(cache, ab, at, blob_rows, s);
+    if (cache->v_bits) return WP == 256 ? launch<256, true, false>(cache, ab, at, blob_rows, s) : launch<128, true, false>(cache, ab, at, blob_rows, s);
+    if (WP == 128) return launch<128, false, false>(cache, ab, at, blob_rows, s);
+    const bool many = (X.shape[max_draft] >> 9 & 7u) > 0;         // kv heads of the largest tree's tiles
+    return many ? launch<256, false, true>(cache, ab, at, blob_rows, s) : launch<256, false, false>(cache, ab, at, blob_rows, s);
 }
