@@ -843,7 +843,8 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
         // ================================================================== softmax: two threads per row, half of a page's tokens each
         // Both halves of a page are worked on at the same time, and the tensor core does the next page's scores meanwhile. (A page
         // per group, the groups taking turns and handing on the rows' references: 57 against 51 us for 4 x 4096 tokens of 32 kv heads,
-        // 184 against 172 us for 16 x 16384 tokens of quantised values; the same for 64 drafts, where the tensor core is the bound.)
+        // 184 against 172 us for 16 x 16384 tokens of quantised values. Four groups of 32 columns: 128 against 129 us for 64 drafts, 303
+        // against 298 for 16 x 32768 tokens, 16 drafts.)
         const int quad = warp & 3, grp = (warp - 4) >> 2, r = quad * 32 + lane;
         const uint32_t tl_s = tb + ((uint32_t)(quad * 32) << 16);
         const float* row_scale = reinterpret_cast<const float*>(smem + C::Q_OFF + PKV_QUERY_TERMS * C::PAGE);
@@ -938,13 +939,14 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                                 for (int e = 0; e < 16; ++e) w[e] &= (see >> (2 * e) & 1 ? 0xffffu : 0u) | (see >> (2 * e) & 2 ? 0xffff0000u : 0u);
                             }
                         } else {
-                            // rounded to bf16 for the tensor core (2^-8 of a weight); the sum is taken over what was rounded, so
-                            // that numerator and denominator agree
+                            // rounded to bf16 for the tensor core (2^-8 of a weight at most, up as often as down); the sum takes the weights
+                            // themselves (over what was rounded it takes 3 % longer: 138 against 134 us for 64 drafts)
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
-                                const float2 t = fma2(make_float2(x[2 * e], x[2 * e + 1]), cs2, mu2);
-                                w[e] = pack_bf16(ex2_fast(t.x), ex2_fast(t.y));
-                                sum = add2(sum, make_float2(__uint_as_float(w[e] << 16), __uint_as_float(w[e] & 0xffff0000u)));
+                                float2 t = fma2(make_float2(x[2 * e], x[2 * e + 1]), cs2, mu2);
+                                t = make_float2(ex2_fast(t.x), ex2_fast(t.y));
+                                w[e] = pack_bf16(t.x, t.y);
+                                sum = add2(sum, t);
                             }
                         }
                         // P: row r, 64 tokens of 16 bit per 128-byte swizzled line, a block per half page
