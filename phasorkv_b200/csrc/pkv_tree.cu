@@ -9,11 +9,15 @@
 // tile. Per page and tile:
 //   S  [128 rows x 128 tokens]  = Q' . C^T     block-scaled NVFP4 tcgen05.mma, the four residual terms of the query added up
 //                                              in tensor memory; a page is the B operand as it is stored
-//   P  = 2^(S - m)              one row per thread: maximum, sum and mask need no other thread
+//   P  = 2^(S - m)              a thread per row and half page: maximum, sum and mask need no other lane
 //   O^T[128 dims x rph] += V_g^T . P_g^T       bf16 tcgen05.mma, a kv head at a time, V as stored
-// With few drafted tokens the V pages bound it (HBM), with many the score MMAs and the softmax.
+// A tile of rows of several kv heads reads the latent page once for all of them, and one of 128 rows fills the M of the score MMA.
+// With few drafted tokens the V pages bound it: 131072 tokens, 8 drafts: 70 us, 4.1 TB/s; 16 x 32768 tokens, 16 drafts: 298 us, 3.9 TB/s,
+// where the GPU draws its 1000 W and the clock falls to 1.54 GHz. With many drafts a page and tile takes 2600 cycles (8 x 8192 tokens, 64
+// drafts: 130 us): 1536 of MMAs beside 1700 of exponentials, and 900 in which the warps hand over the page.
 //
-// Three launches: the operand (absorbed queries), the attention, the merge of what several CTAs did of one tile.
+// Three launches: the operand (absorbed queries), the attention, the merge of what several CTAs did of one tile. (A last CTA that
+// merges inside the attention launch waits for a counter and reads the others' partial results alone: slower than the third launch.)
 #include "pkv_common.cuh"
 #include "pkv_tcgen05.cuh"
 
@@ -80,8 +84,8 @@ struct Batch {
 //   Every sequence has as many tiles (the usual step: as many drafts): a page counts 1, a gang has a CTA per tile (up to 16, then there are
 //   passes), and the tiles of a sequence read a page at about the same time, from L2 all but the first.
 //   Otherwise every CTA is a gang of its own, a sequence has a pass per tile, and a page counts what it costs the tile: no CTA idles
-//   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts: 104 us; tiles of one shape, by the most
-//   drafts, and gangs of them: 130 us).
+//   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts, before later steps: 104 us; tiles of one
+//   shape, by the most drafts, and gangs of them: 130 us).
 struct List { int gang, gangs, U; };                 // gang: CTAs, or 0 for CTAs on their own
 constexpr int LIST_WORDS = 4;
 
@@ -234,8 +238,12 @@ struct AbsorbArgs {
 
 constexpr int AR = 16;                               // rows per CTA
 
-// CTA (16 rows of a tile, tile, sequence). Rows that
-// no drafted token has are not written: a row of garbage only reaches its own column of the result, which nobody reads.
+// CTA (16 rows of a tile, tile, sequence): a thread per column for the absorbed rows, then a thread per row and block of 16 columns for
+// the terms. Rows that no drafted token has are not written: a row of garbage only reaches its own column of the result, which nobody
+// reads. Latency with few drafts (6 us: lengths, queries and factors from cold memory), instruction issue with many (16384 rows of 256
+// columns: 15 us, 18 with the loads one after the other and the terms formed a value at a time).
+// The launch behind it is let go at once although its pages then compete with this one's loads: 74 us against 75 when the queries have
+// arrived and 78 at the end (131072 tokens, 8 drafts).
 template <int WP>
 __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const AbsorbArgs A) {
     constexpr int NB = WP / 16, NT = AR * NB, RB = WP / 2;
@@ -640,7 +648,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                     }
                     if constexpr (VQ) {
                         // The token scales of the page's kv heads. (Here and not with the tiles, behind which they would come when the
-                        // ring of tiles has moved on, a whole page late: 217 against 190 us for 16 x 16384 tokens, 12 drafts.)
+                        // ring of tiles has moved on, a whole page late: 16 x 16384 tokens, 12 drafts took 217 us instead of 190, now 163.)
                         const int g0 = s.z % s.t.groups * s.t.G, bytes = heads(s) * PKV_PAGE_TOKENS * 2;
                         if (k >= 2) ok = wait_or_abort(&X->sc_empty[k & 1], ((k >> 1) - 1) & 1, X, A.status, 22);
                         if (!ok) { ++k; break; }
@@ -1082,7 +1090,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
 // ------------------------------------------------------------------------------------------------ merge
 // O = sum 2^(m - M) o / sum 2^(m - M) l over the stretches of a tile that several gangs had. A warp has RW rows (a lane four dims of
 // each); WPR warps share the stretches of their rows. References, sums and outputs of DEEP stretches are asked for together: many
-// rows of few stretches, or few rows of many.
+// rows of few stretches, or few rows of many. Latency and the launch itself (one sequence in 74 stretches: 5 us).
 template <int WPR, int RW, int DEEP>
 __global__ void __launch_bounds__(256) pkv_tree_merge_kernel(const AttnArgs A) {
     __shared__ float4 acc_s[WPR > 1 ? 8 : 1][RW][32];
@@ -1244,10 +1252,12 @@ int launch(const pkv_cache_t* cache, const AbsorbArgs& ab, const AttnArgs& at, s
     PKV_CUDA_TRY(pkv_set_max_smem(pkv_tree_attn_kernel<WP, VQ, MANY>, C::SMEM, attr));
     PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_absorb_kernel<WP>, dim3(ROWS / AR + 1, X.Z, ab.B.batch), dim3(AR * WP / 16), 0, st, ab));
     PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_attn_kernel<WP, VQ, MANY>, dim3(N_SM), dim3(C::NTHREADS), C::SMEM, st, kmap, qmap, vmap, at));
-    // stretches of a tile, if all sequences have as many tiles and pages: the more, the more warps share a row's
+    // Stretches of a tile, if all sequences have as many tiles and pages: the more, the more warps share a row's. The three forms, all
+    // launches together: 3 stretches (16 x 32768 tokens, 16 drafts) 299, 304 and 345 us; 6 (7 x 20000, 16) 92, 95 and 121; 10 (4 x 4096,
+    // 32 kv heads, 8) 54, 49 and 61; 75 (131072, 8) 108, 79 and 69.
     const int parts = N_SM / (ab.B.batch * X.Z) + 1;
     const dim3 block(256);
-    if (parts <= 4) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1, 4, 2>, dim3(ROWS / 32, X.Z, ab.B.batch), block, 0, st, at));
+    if (parts <= 6) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<1, 4, 2>, dim3(ROWS / 32, X.Z, ab.B.batch), block, 0, st, at));
     else if (parts <= 16) PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<2, 1, 8>, dim3(ROWS / 4, X.Z, ab.B.batch), block, 0, st, at));
     else PKV_CUDA_TRY(pkv_launch_chained(pkv_tree_merge_kernel<8, 1, 10>, dim3(ROWS, X.Z, ab.B.batch), block, 0, st, at));
     return PKV_OK;
