@@ -455,3 +455,31 @@ def test_captured_graphs_share_a_workspace():
         outs[i].zero_()
         graphs[i].replay()
         (a, b)[i].check(outs[i])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,layout", [(64, 8, "freq1"), (64, 1, "freq2"), (64, 32, "freq1"), (48, 16, "band8")])
+@pytest.mark.parametrize("base,n", [([700, 5, 2100], [64, 64, 64]), ([700, 5, 2100], [64, 1, 33])])
+def test_more_tiles_than_a_gang_has_ctas(n_q, n_kv, layout, base, n):
+    """Several passes over a sequence's pages, all sequences alike and not."""
+    c = Case(layer(n_q, n_kv, layout), base, n)
+    c.check(c.run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v_bits", [0, 3])
+def test_a_reference_that_moves_on_every_page(v_bits):
+    """Cached rows that grow from page to page: every page's maximum passes the row's reference, sums and results are rescaled."""
+    c = Case(layer(32, 8), [1400, 600], [20, 3], v_bits=v_bits, q_dtype=torch.float32)
+    W, most = c.pk.cache_width, 0.0
+    for b, T in enumerate((1420, 603)):
+        s = c.slots(b, 0, T)
+        grow = (torch.arange(T, device="cuda") // PAGE + 1)[:, None] / (T // PAGE + 1.0)
+        g = torch.Generator(device="cuda").manual_seed(b)
+        c.cache.quantize_rows(torch.randn((T, W), generator=g, device="cuda") * grow * torch.linspace(2.5, 0.5, W, device="cuda"), s, c.pk.second)
+    c.q *= 8.0
+    out = c.run()
+    torch.cuda.synchronize()
+    for b, (lo, n) in enumerate(((0, 20), (20, 3))):                    # logits up to 300: as with peaked logits
+        O, A = c.formula(b, most=300)
+        assert ((out[lo:lo + n].double() - O).abs() <= (ELEM + 0.043) * A).all()
