@@ -13,8 +13,8 @@
 //   O^T[128 dims x rph] += V_g^T . P_g^T       bf16 tcgen05.mma, a kv head at a time, V as stored
 // A tile of rows of several kv heads reads the latent page once for all of them, and one of 128 rows fills the M of the score MMA.
 // With few drafted tokens the V pages bound it: 131072 tokens, 8 drafts: 70 us, 4.1 TB/s; 16 x 32768 tokens, 16 drafts: 298 us, 3.9 TB/s,
-// where the GPU draws its 1000 W and the clock falls to 1.54 GHz. With many drafts a page and tile takes 2600 cycles (8 x 8192 tokens, 64
-// drafts: 130 us): 1536 of MMAs beside 1700 of exponentials, and 900 in which the warps hand over the page.
+// where the GPU draws its 1000 W and the clock falls to 1.54 GHz. With many drafts a page and tile takes 2450 cycles (8 x 8192 tokens, 64
+// drafts: 122 to 137 us with the clock): 1536 of MMAs beside 1400 of exponentials and 1000 in which the warps hand over the page.
 //
 // Three launches: the operand (absorbed queries), the attention, the merge of what several CTAs did of one tile. (A last CTA that
 // merges inside the attention launch waits for a counter and reads the others' partial results alone: slower than the third launch.)
@@ -502,6 +502,18 @@ __device__ __forceinline__ float ex2_fast(float x) {     // 2 ulp, results below
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// The same for two numbers without the exponential unit, which the softmax keeps busy: n = rint(x), and 2^(x - n) by the cubic of least
+// relative error on -1/2 .. 1/2 (7.5e-5, a twenty-sixth of half a bf16 step; coefficients by linear programming on 4001 points). NaN stays NaN; below 2^-126 (-infinity too): 0.
+__device__ __forceinline__ float2 ex2_cubic(float2 x) {
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(x.x) : "f"(x.x), "f"(-127.0f));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(x.y) : "f"(x.y), "f"(-127.0f));
+    const float2 t = add2(x, make_float2(12582912.0f, 12582912.0f)), n = add2(t, make_float2(-12582912.0f, -12582912.0f));      // 1.5 x 2^23
+    const float2 f = fma2(n, make_float2(-1.0f, -1.0f), x);
+    float2 y = fma2(f, make_float2(0.055171670f, 0.055171670f), make_float2(0.242611125f, 0.242611125f));
+    y = fma2(f, y, make_float2(0.693260985f, 0.693260985f));
+    y = fma2(f, y, make_float2(0.999928073f, 0.999928073f));
+    return mul2(y, make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u), __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u)));
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -948,11 +960,14 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                             }
                         } else {
                             // rounded to bf16 for the tensor core (2^-8 of a weight at most, up as often as down); the sum takes the weights
-                            // themselves (over what was rounded it takes 3 % longer: 138 against 134 us for 64 drafts)
+                            // themselves (over what was rounded it takes 3 % longer: 138 against 134 us for 64 drafts). Five of 16 pairs
+                            // go to the multiply-add units: with none, 2, 4, 5 or 8 of them 131, 126, 128, 122 and 130 us for 64 drafts,
+                            // 123, 117, 118, 115 and 118 for 32. Tiles of several kv heads wait for values and for power (16 x 32768
+                            // tokens, 16 drafts: 289 us with none, 295 with 5): none.
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 float2 t = fma2(make_float2(x[2 * e], x[2 * e + 1]), cs2, mu2);
-                                t = make_float2(ex2_fast(t.x), ex2_fast(t.y));
+                                t = !MANY && e % 3 == 2 ? ex2_cubic(t) : make_float2(ex2_fast(t.x), ex2_fast(t.y));
                                 w[e] = pack_bf16(t.x, t.y);
                                 sum = add2(sum, t);
                             }
@@ -963,6 +978,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                         for (int u = 0; u < 4; ++u)
                             *reinterpret_cast<uint4*>(line + (((c * 4 + u) ^ (r & 7)) << 4)) = make_uint4(w[4 * u], w[4 * u + 1], w[4 * u + 2], w[4 * u + 3]);
                     }
+                    fence_proxy_async_smem();
                     if (!first_try) break;
                     top = mine ? top * cs : -INFINITY;                  // (a row that nobody has: whatever its column becomes, nobody reads it)
                     if (__builtin_expect(!opening && !softmax_any(top > m + RESCALE_THRESHOLD || !ok), true)) break;
@@ -1001,7 +1017,6 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                         tc_fence_before_sync();
                     }
                 }
-                fence_proxy_async_smem();
                 arrive_warp(&X->p_full[buf]);
                 if constexpr (!VQ) {
                     // Values behind the cached tokens: rows past the sequence become zero, and so does what is not finite in a
