@@ -64,7 +64,7 @@ class LayerDecodeState:
         self.seq = torch.arange(batch, dtype=torch.int32, device=pk.device)
         self.lengths = [0] * batch                          # tokens cached per sequence (host copy of cache.seqlens)
         self.calibrated = False
-        self.drafted = None                                 # plan and lengths before it, between verify() and accept()
+        self.drafted = None                                 # plan and parents, between verify() and accept()
         self.tree = {}                                      # drafts per sequence -> (plan, workspace, write scratch, counts)
 
     @property
@@ -137,6 +137,7 @@ class LayerDecodeState:
         pk, dev = self.pk, self.pk.device
         if B != self.batch or not 1 <= n <= TREE_MAX:
             raise ValueError(f"1 .. {TREE_MAX} drafted tokens for each of the {self.batch} sequences, not {n} for {B}")
+        host = torch.arange(-1, n - 1).repeat(B, 1)
         if parents is not None:
             host = parents.cpu()
             if host.shape != (B, n) or (host < -1).any() or (host >= torch.arange(n)).any():
@@ -156,7 +157,7 @@ class LayerDecodeState:
         self.cache.plan_step(plan, n_new, parents=parents)
         pk.write_paged(self.cache, x, plan.positions, plan.slots, v=v, scratch=scratch)
         out = pk.tree_step(self.cache, q, plan, ws)
-        self.drafted = (plan, n)
+        self.drafted = (plan, host.tolist())
         return out.view(B, n, pk.n_q, pk.head_dim)
 
     def accept(self, keep) -> None:
@@ -164,10 +165,11 @@ class LayerDecodeState:
         the next; none: all drafts of b are dropped). They become the sequence's next tokens."""
         if self.drafted is None:
             raise RuntimeError("accept() follows verify()")
-        plan, n = self.drafted
+        plan, parents = self.drafted
+        n = len(parents[0])
         keep = [[int(i) for i in rows] for rows in keep]
-        if len(keep) != self.batch or any(not 0 <= i < n for rows in keep for i in rows) or any(a >= b for rows in keep for a, b in zip(rows, rows[1:])):
-            raise ValueError(f"keep gives ascending rows 0 .. {n - 1} for each of the {self.batch} sequences")
+        if len(keep) != self.batch or any(not 0 <= i < n or parents[b][i] != up for b, rows in enumerate(keep) for up, i in zip([-1] + rows, rows)):
+            raise ValueError(f"keep gives a path of rows 0 .. {n - 1}, each the parent of the next, for each of the {self.batch} sequences")
         dev = self.pk.device
         rows = torch.tensor([r + [-1] * (n - len(r)) for r in keep], dtype=torch.int32).to(dev).reshape(-1)
         lengths = torch.empty(self.batch, dtype=torch.int32, device=dev)

@@ -128,7 +128,7 @@ def test_refusals_of_a_layer_state():
     st.verify(t(2, 4, D), t(2, 4, 32, 128), t(2, 4, 8, 128))
     with pytest.raises(RuntimeError):
         st.verify(t(2, 4, D), t(2, 4, 32, 128), t(2, 4, 8, 128))
-    for bad in ([[0]], [[0], [4]], [[1, 0], []], [[0, 0], []], [[-1], []]):
+    for bad in ([[0]], [[0], [4]], [[1, 0], []], [[0, 0], []], [[-1], []], [[1, 2], []], [[0, 2], []]):
         with pytest.raises(ValueError):
             st.accept(bad)
     st.accept([[0, 1], []])
