@@ -87,7 +87,7 @@ struct Batch {
 //   where a sequence has fewer tiles than another (24 ragged sequences of 0 .. 21 drafts, before later steps: 104 us; tiles of one
 //   shape, by the most drafts, and gangs of them: 130 us).
 struct List { int gang, gangs, U; };                 // gang: CTAs, or 0 for CTAs on their own
-constexpr int LIST_WORDS = 4;
+constexpr int LIST_WORDS = 5;
 
 __device__ __forceinline__ int passes_of(const Shape& t, int gang) { return gang == 0 ? t.Z : (t.Z + gang - 1) / gang; }
 __device__ __forceinline__ int cost_of(const Shape& t, int gang) { return gang == 0 ? t.cost : 1; }
@@ -96,7 +96,7 @@ __device__ __forceinline__ int cost_of(const Shape& t, int gang) { return gang =
 // (its only one, in batches of at most nt)
 __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid, int nt, int (*red)[LIST_WORDS], int2& last) {
     last = make_int2(0, 0);
-    int v[LIST_WORDS] = {0, 0, 0, 1 << 30};          // pages, pages x tiles x cost, most tiles, fewest tiles
+    int v[LIST_WORDS] = {0, 0, 0, 1 << 30, 1};       // pages, pages x tiles x cost, most tiles, fewest tiles, highest cost
 #pragma unroll 1
     for (int b = tid; b < B.batch; b += nt) {
         int lo, n, T;
@@ -106,10 +106,10 @@ __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid,
         const Shape t = X.of(n);
         const int Z = t.Z;
         v[0] += pages; v[1] += pages * Z * t.cost;
-        v[2] = max(v[2], Z); v[3] = min(v[3], Z);
+        v[2] = max(v[2], Z); v[3] = min(v[3], Z); v[4] = max(v[4], t.cost);
     }
     v[0] = __reduce_add_sync(0xffffffffu, v[0]); v[1] = __reduce_add_sync(0xffffffffu, v[1]);
-    v[2] = __reduce_max_sync(0xffffffffu, v[2]); v[3] = __reduce_min_sync(0xffffffffu, v[3]);
+    v[2] = __reduce_max_sync(0xffffffffu, v[2]); v[3] = __reduce_min_sync(0xffffffffu, v[3]); v[4] = __reduce_max_sync(0xffffffffu, v[4]);
     if ((tid & 31) == 0)
 #pragma unroll
         for (int i = 0; i < LIST_WORDS; ++i) red[tid >> 5][i] = v[i];
@@ -118,14 +118,15 @@ __device__ __forceinline__ List list_of(const Batch& B, const Tiles& X, int tid,
     for (int w = 0; w < min(nt, B.batch + 31) / 32; ++w) {     // (the other warps have none)
         if (w == (tid >> 5)) continue;
         v[0] += red[w][0]; v[1] += red[w][1];
-        v[2] = max(v[2], red[w][2]); v[3] = min(v[3], red[w][3]);
+        v[2] = max(v[2], red[w][2]); v[3] = min(v[3], red[w][3]); v[4] = max(v[4], red[w][4]);
     }
     List y;
     const int passes = (v[2] + 15) >> 4;
     y.gang = v[2] == v[3] ? (v[2] + passes - 1) / passes : 0;
     y.gangs = y.gang ? N_SM / y.gang : N_SM;
     y.U = v[2] == v[3] ? v[0] * passes : v[1];
-    y.gangs = min(y.gangs, y.gang ? y.U : max(y.U / COST_MOST, min(y.U, 1)));      // (a stretch that is not its tile's first or last has a page)
+    // (a stretch that is not its tile's first or last has a page: none is shorter than the dearest page)
+    y.gangs = min(y.gangs, y.gang ? y.U : max(y.U / v[4], min(y.U, 1)));
     return y;
 }
 
