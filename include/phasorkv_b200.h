@@ -442,7 +442,7 @@ typedef struct pkv_plan {
     int32_t* seq_dev;                /* [capacity] sequence of each token */
     int32_t* positions_dev;          /* [capacity] position: the place in the sequence, or in a tree length + depth */
     int32_t* slots_dev;              /* [capacity] page * 128 + row; -1 behind the last token (the writers skip it) */
-    int64_t* mask_dev;               /* [capacity] ancestors of a drafted token and itself, bit = row in its sequence; may be NULL without parents */
+    int64_t* mask_dev;               /* [capacity] ancestors of a token and itself, bit = row in its sequence (past 63: all bits); may be NULL without parents */
     uint32_t* ticket_dev;
     int32_t* status_dev;             /* optional int32[4] */
     int32_t  capacity;
@@ -451,7 +451,9 @@ typedef struct pkv_plan {
 /* Room for n_new_dev[b] >= 0 more tokens in every sequence: pages from the pool (in the order of the sequences), table
  * entries, slots and positions, and seqlens += n_new.  parents_dev (optional, [capacity], ragged like the rest): row of
  * each token's parent within its sequence, before the token itself, or -1 for a child of the last cached token; then
- * n_new <= PKV_TREE_MAX, and masks are filled too.  The other arrays behind the last token are left as they were.
+ * n_new <= PKV_TREE_MAX, and mask_dev is needed.  Without parents the tokens are a chain, and mask_dev, if given, gets a chain's
+ * words: a caller's own masks are written after this call.  Behind the last token slots are -1 and
+ * the other arrays are left as they were.
  * When a length, a parent or the pool does not allow the step, the call changes no table and no length, cu is all zero,
  * every slot is -1 and the status says why.  batch <= 4096.  n_new_dev and parents_dev are not the plan's own arrays. */
 int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev, const int32_t* parents_dev, const pkv_plan_t* plan,

@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(NT) pkv_plan_step_kernel(const PlanArgs A) {
                 }
                 pos[e] = L + depth;
                 A.plan.mask_dev[i] = (int64_t)word;
+            } else if (A.plan.mask_dev) {            // a chain: the step's tokens up to this one (words of an earlier tree must not stay)
+                A.plan.mask_dev[i] = (int64_t)(row >= PKV_TREE_MAX - 1 ? ~0ull : (2ull << row) - 1);
             }
         }
         if (wide && !refused && i0 + 4 <= total) {

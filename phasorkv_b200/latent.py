@@ -111,9 +111,10 @@ class PagedLatentCache:
 
     def plan_step(self, plan: "StepPlan", n_new: torch.Tensor, parents: Optional[torch.Tensor] = None) -> None:
         """Room for ``n_new[b]`` (int32 [batch], on the device) more tokens in every sequence: pages from the pool, `seqlens`,
-        and the tokens' sequence, position, slot and, with `parents` (int32 [capacity]), ancestor mask into `plan`.
-        ``parents[i]`` is the row of token i's parent among its sequence's new tokens, before i, or -1; positions are then
-        length + depth. A step that does not fit changes nothing: ``plan.cu`` is zero, every slot -1, ``plan.status`` says why."""
+        and the tokens' sequence, position, slot and, in a plan with masks, ancestor mask into `plan`.
+        ``parents[i]`` (int32 [capacity]) is the row of token i's parent among its sequence's new tokens, before i, or -1;
+        positions are then length + depth. Without `parents` the tokens are a chain, in the masks too (masks of the
+        caller's own are written after this call). A step that does not fit changes nothing: ``plan.cu`` is zero, every slot -1, ``plan.status`` says why."""
         _lib.need(n_new, torch.int32, (self.batch,), self.latent.device, "n_new")
         if parents is not None:
             _lib.need(parents, torch.int32, (plan.capacity,), self.latent.device, "parents")
@@ -223,8 +224,8 @@ class PagedLatentCache:
 
 class StepPlan:
     """What `PagedLatentCache.plan_step` fills, for the step's other calls: ``cu`` [batch + 1] first row of every sequence,
-    and for each of up to `capacity` tokens its sequence ``seq``, ``positions``, ``slots`` (-1 behind the last token) and, in
-    a tree, the 64-bit word ``mask`` of the drafted tokens it attends to (its ancestors and itself)."""
+    and for each of up to `capacity` tokens its sequence ``seq``, ``positions``, ``slots`` (-1 behind the last token) and, with
+    ``tree=True``, the 64-bit word ``mask`` of the drafted tokens it attends to (its ancestors and itself; in a chain those before it and itself)."""
 
     def __init__(self, batch: int, capacity: int, tree: bool, device):
         if capacity < 0:

@@ -347,3 +347,17 @@ def test_c_entries_refuse_an_array_given_twice(lib):
     one = (ctypes.c_void_p * 1)(ctypes.addressof(cache))
     for out in (1024, 2048, 5120, 8192):
         assert lib.pkv_keep_rows(one, 1, ctypes.byref(pg), 1024, 4, 2048, 5120, out, None, None) == -1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[5, 0, 64], [1, 1, 1], [700, 63, 900]])
+def test_a_plan_with_masks_has_a_chains_without_parents(new):
+    """Nothing of an earlier tree stays in the words: each token sees itself and the step's tokens before it."""
+    cache = PagedLatentCache(128, 1, 128, 3, 2000, "cuda", with_v=False)
+    cap = sum(new) + 4
+    plan = cache.step_plan(cap, tree=True)
+    plan.mask.fill_(0x5a5a)
+    cache.plan_step(plan, i32(new))
+    words = [(1 << min(i + 1, 64)) - 1 for m in new for i in range(m)]
+    assert plan.mask.tolist() == [w - (1 << 64) if w >> 63 else w for w in words] + [0x5a5a] * 4
+    assert plan.positions[:sum(new)].tolist() == [i for m in new for i in range(m)] and int(plan.status[0]) == 0

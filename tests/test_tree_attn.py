@@ -483,3 +483,17 @@ def test_a_reference_that_moves_on_every_page(v_bits):
     for b, (lo, n) in enumerate(((0, 20), (20, 3))):                    # logits up to 300: as with peaked logits
         O, A = c.formula(b, most=300)
         assert ((out[lo:lo + n].double() - O).abs() <= (ELEM + 0.043) * A).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("v_bits", [0, 3])
+def test_a_chain_planned_where_a_tree_was(v_bits):
+    """One plan with masks serves a step of a tree and, planned again without parents, a chain."""
+    base, n = [300, 64, 127], [9, 5, 12]
+    c = Case(layer(32, 8), base, n, mask="any", v_bits=v_bits)
+    c.check(c.run())
+    c.cache.seqlens.copy_(torch.tensor(base, dtype=torch.int32))
+    c.cache.plan_step(c.plan, torch.tensor(n, dtype=torch.int32, device="cuda"))
+    c.words = [tree_words(random.Random(0), m, "chain") for m in n]
+    c.positions = [[b + i for i in range(m)] for b, m in zip(base, n)]
+    c.check(c.run())
