@@ -137,6 +137,10 @@ class LayerDecodeState:
         pk, dev = self.pk, self.pk.device
         if B != self.batch or not 1 <= n <= TREE_MAX:
             raise ValueError(f"1 .. {TREE_MAX} drafted tokens for each of the {self.batch} sequences, not {n} for {B}")
+        for name, t, shape in (("x", x, (B, n, pk.d_model)), ("q", q, (B, n, pk.n_q, pk.head_dim)), ("v", v, (B, n, pk.n_kv, pk.head_dim))):
+            # the kernels would read past its end, or from another device's memory (x is moved by its writer)
+            if t.shape != shape or (t is not x and t.device != self.cache.latent.device):
+                raise ValueError(f"{name} must be of shape {shape} on {self.cache.latent.device}, got {tuple(t.shape)} on {t.device}")
         host = torch.arange(-1, n - 1).repeat(B, 1)
         if parents is not None:
             host = parents.cpu()

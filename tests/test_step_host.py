@@ -1,0 +1,64 @@
+"""What the step's Python calls refuse or arrange before anything reaches a GPU: with stand-ins for the layer and its cache, on the CPU."""
+import contextlib
+import types
+
+import pytest
+import torch
+
+from phasorkv_b200 import build
+from phasorkv_b200.patch import LayerDecodeState
+
+
+@pytest.fixture(scope="module", autouse=True)
+def lib():
+    build.build()
+
+
+# ------------------------------------------------------------------------------------------------ verify
+D, N_Q, N_KV = 32, 4, 2
+
+
+class Recorder:
+    """A layer and its cache that only note what is called, on which device."""
+
+    def __init__(self, batch=2):
+        self.calls, self.inside = [], None
+        note = lambda name: lambda *a, **k: self.calls.append((name, self.inside))
+        self.pk = types.SimpleNamespace(device=torch.device("cpu"), d_model=D, n_q=N_Q, n_kv=N_KV, head_dim=128, cache_width=64, write_paged=note("write"),
+                                        write_scratch=lambda n: None, tree_workspace=lambda *a, **k: types.SimpleNamespace(status=None),
+                                        tree_step=lambda cache, q, plan, ws, **k: (self.calls.append(("attend", self.inside)), torch.zeros(q.shape))[1])
+        plan = types.SimpleNamespace(positions=None, slots=None)
+        self.cache = types.SimpleNamespace(latent=torch.zeros(1), step_plan=lambda *a, **k: plan, plan_step=note("plan"), truncate=note("truncate"),
+                                           keep_rows=note("keep"))
+        st = self.state = object.__new__(LayerDecodeState)
+        st.pk, st.cache, st.batch, st.max_tokens, st.lengths, st.drafted, st.tree = self.pk, self.cache, batch, 256, [5, 9], None, {}
+
+    @contextlib.contextmanager
+    def on_device(self, device):
+        self.inside = device
+        yield 0
+        self.inside = None
+
+
+def tensors(B=2, n=3, **shapes):
+    z = lambda name, *s: torch.zeros(shapes.get(name, s))
+    return z("x", B, n, D), z("q", B, n, N_Q, 128), z("v", B, n, N_KV, 128)
+
+
+@pytest.mark.parametrize("shapes", [dict(x=(2, 3, D // 2)), dict(x=(2, 3, 2 * D)), dict(q=(2, 3, N_Q // 2, 128)), dict(q=(2, 6, N_Q, 64)), dict(q=(3, 2, N_Q, 128)),
+                                    dict(v=(2, 3, 2 * N_KV, 64)), dict(v=(3, 2, N_KV, 128)), dict(v=(2, 4, N_KV, 128))])
+def test_verify_refuses_tensors_of_another_shape(shapes):
+    """The write kernel reads d_model columns of every row: a narrower x would be read past its end."""
+    r = Recorder()
+    with pytest.raises(ValueError):
+        r.state.verify(*tensors(**shapes))
+    assert r.calls == [] and r.state.drafted is None
+
+
+@pytest.mark.parametrize("which", [1, 2])
+def test_verify_refuses_tensors_of_another_device(which):
+    r, t = Recorder(), list(tensors())
+    t[which] = t[which].to("meta")
+    with pytest.raises(ValueError):
+        r.state.verify(*t)
+    assert r.calls == []
