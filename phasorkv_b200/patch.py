@@ -43,7 +43,7 @@ from typing import Optional
 
 import torch
 
-from ._lib import TREE_MAX
+from ._lib import TREE_MAX, on_device
 from .latent import PAGE_TOKENS, PhasorKey
 
 NVFP4_BITS = 4.5          # E2M1 code + one E4M3 scale per 16 codes (phasorkv/quant.py:9)
@@ -148,19 +148,20 @@ class LayerDecodeState:
                 raise ValueError("parents [batch, drafts] name a row before the token's own, or -1")
         for b in range(B):
             self._need(b, n)
-        if n not in self.tree:
-            self.tree[n] = (self.cache.step_plan(B * n, tree=True), pk.tree_workspace(B, B * n, n, self.max_tokens), pk.write_scratch(B * n),
-                            torch.full((B,), n, dtype=torch.int32, device=dev),
-                            torch.arange(-1, n - 1, dtype=torch.int32, device=dev).repeat(B))
-        plan, ws, scratch, n_new, chain = self.tree[n]
-        parents = chain if parents is None else parents.to(device=dev, dtype=torch.int32).reshape(B * n).contiguous()
-        x, v = x.reshape(B * n, -1).contiguous(), v.reshape(B * n, pk.n_kv, pk.head_dim).contiguous()
-        q = q.reshape(B * n, pk.n_q, pk.head_dim).contiguous()
-        if q.dtype not in (torch.bfloat16, torch.float32):
-            q = q.float()
-        self.cache.plan_step(plan, n_new, parents=parents)
-        pk.write_paged(self.cache, x, plan.positions, plan.slots, v=v, scratch=scratch)
-        out = pk.tree_step(self.cache, q, plan, ws)
+        with on_device(self.cache.latent.device):              # the writer's launches go to the current device
+            if n not in self.tree:
+                self.tree[n] = (self.cache.step_plan(B * n, tree=True), pk.tree_workspace(B, B * n, n, self.max_tokens), pk.write_scratch(B * n),
+                                torch.full((B,), n, dtype=torch.int32, device=dev),
+                                torch.arange(-1, n - 1, dtype=torch.int32, device=dev).repeat(B))
+            plan, ws, scratch, n_new, chain = self.tree[n]
+            parents = chain if parents is None else parents.to(device=dev, dtype=torch.int32).reshape(B * n).contiguous()
+            x, v = x.reshape(B * n, -1).contiguous(), v.reshape(B * n, pk.n_kv, pk.head_dim).contiguous()
+            q = q.reshape(B * n, pk.n_q, pk.head_dim).contiguous()
+            if q.dtype not in (torch.bfloat16, torch.float32):
+                q = q.float()
+            self.cache.plan_step(plan, n_new, parents=parents)
+            pk.write_paged(self.cache, x, plan.positions, plan.slots, v=v, scratch=scratch)
+            out = pk.tree_step(self.cache, q, plan, ws)
         self.drafted = (plan, host.tolist())
         return out.view(B, n, pk.n_q, pk.head_dim)
 
@@ -174,11 +175,12 @@ class LayerDecodeState:
         keep = [[int(i) for i in rows] for rows in keep]
         if len(keep) != self.batch or any(not 0 <= i < n or parents[b][i] != up for b, rows in enumerate(keep) for up, i in zip([-1] + rows, rows)):
             raise ValueError(f"keep gives a path of rows 0 .. {n - 1}, each the parent of the next, for each of the {self.batch} sequences")
-        dev = self.pk.device
-        rows = torch.tensor([r + [-1] * (n - len(r)) for r in keep], dtype=torch.int32).to(dev).reshape(-1)
-        lengths = torch.empty(self.batch, dtype=torch.int32, device=dev)
-        self.cache.keep_rows(plan, rows, torch.tensor([len(r) for r in keep], dtype=torch.int32).to(dev), lengths)
-        self.cache.truncate(lengths)
+        with on_device(self.cache.latent.device):
+            dev = self.pk.device
+            rows = torch.tensor([r + [-1] * (n - len(r)) for r in keep], dtype=torch.int32).to(dev).reshape(-1)
+            lengths = torch.empty(self.batch, dtype=torch.int32, device=dev)
+            self.cache.keep_rows(plan, rows, torch.tensor([len(r) for r in keep], dtype=torch.int32).to(dev), lengths)
+            self.cache.truncate(lengths)
         self.lengths = [a + len(r) for a, r in zip(self.lengths, keep)]
         self.drafted = None
 

@@ -5,7 +5,7 @@ import types
 import pytest
 import torch
 
-from phasorkv_b200 import build
+from phasorkv_b200 import build, patch
 from phasorkv_b200.patch import LayerDecodeState
 
 
@@ -62,3 +62,13 @@ def test_verify_refuses_tensors_of_another_device(which):
     with pytest.raises(ValueError):
         r.state.verify(*t)
     assert r.calls == []
+
+
+def test_verify_runs_on_the_device_of_its_cache(monkeypatch):
+    """The writer's launches go to the current device: inside verify and accept that is the cache's, whatever the caller's is."""
+    r = Recorder()
+    monkeypatch.setattr(patch, "on_device", r.on_device, raising=False)
+    r.state.verify(*tensors())
+    r.state.accept([[0], [0, 1]])
+    assert [c[0] for c in r.calls] == ["plan", "write", "attend", "keep", "truncate"]
+    assert all(where == torch.device("cpu") for _, where in r.calls), r.calls
