@@ -160,8 +160,13 @@ class LayerDecodeState:
             if q.dtype not in (torch.bfloat16, torch.float32):
                 q = q.float()
             self.cache.plan_step(plan, n_new, parents=parents)
-            pk.write_paged(self.cache, x, plan.positions, plan.slots, v=v, scratch=scratch)
-            out = pk.tree_step(self.cache, q, plan, ws)
+            try:
+                pk.write_paged(self.cache, x, plan.positions, plan.slots, v=v, scratch=scratch)
+                out = pk.tree_step(self.cache, q, plan, ws)
+            except BaseException:
+                # nothing is pending, so the planned rows must not count as cached tokens
+                self.cache.truncate(torch.tensor(self.lengths, dtype=torch.int32).to(dev))
+                raise
         self.drafted = (plan, host.tolist())
         return out.view(B, n, pk.n_q, pk.head_dim)
 

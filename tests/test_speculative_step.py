@@ -133,3 +133,25 @@ def test_refusals_of_a_layer_state():
             st.accept(bad)
     st.accept([[0, 1], []])
     assert st.lengths == [502, 500] and st.cache.seqlens.tolist() == [502, 500]
+
+
+@pytest.mark.parametrize("fails", ["write_paged", "tree_step"])
+def test_a_verification_that_fails_leaves_the_layer_as_it_was(fails, monkeypatch):
+    """An error behind the plan: the drafts are no cached tokens, and the next verification gives what it would have given."""
+    pk = PhasorKey.from_spec(synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0))
+    g = torch.Generator(device="cuda").manual_seed(3)
+    t = lambda *s: torch.randn(s, generator=g, device="cuda")
+    x0, v0 = t(2, 126, D), t(2, 126, 8, 128)
+    x, q, v = t(2, 5, D), t(2, 5, 32, 128), t(2, 5, 8, 128)
+    st, other = state(pk, 2, 0, x0, v0), state(pk, 2, 0, x0, v0)
+
+    def error(*a, **k):
+        raise RuntimeError("out of memory")
+    with monkeypatch.context() as m:
+        m.setattr(pk, fails, error)
+        with pytest.raises(RuntimeError, match="out of memory"):
+            st.verify(x, q, v)
+    assert st.cache.seqlens.tolist() == st.lengths == [126, 126] and st.drafted is None
+    assert torch.equal(st.verify(x, q, v), other.verify(x, q, v))
+    st.accept([[0], []])
+    assert st.cache.seqlens.tolist() == st.lengths == [127, 126]
