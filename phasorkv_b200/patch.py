@@ -173,13 +173,9 @@ class LayerDecodeState:
     def accept(self, keep) -> None:
         """Keep a path of the drafts that ``verify`` wrote: ``keep[b]`` lists their rows, from the root on (each the parent of
         the next; none: all drafts of b are dropped). They become the sequence's next tokens."""
-        if self.drafted is None:
-            raise RuntimeError("accept() follows verify()")
+        keep = self._paths(keep)
         plan, parents = self.drafted
         n = len(parents[0])
-        keep = [[int(i) for i in rows] for rows in keep]
-        if len(keep) != self.batch or any(not 0 <= i < n or parents[b][i] != up for b, rows in enumerate(keep) for up, i in zip([-1] + rows, rows)):
-            raise ValueError(f"keep gives a path of rows 0 .. {n - 1}, each the parent of the next, for each of the {self.batch} sequences")
         with on_device(self.cache.latent.device):
             dev = self.pk.device
             rows = torch.tensor([r + [-1] * (n - len(r)) for r in keep], dtype=torch.int32).to(dev).reshape(-1)
@@ -188,6 +184,17 @@ class LayerDecodeState:
             self.cache.truncate(lengths)
         self.lengths = [a + len(r) for a, r in zip(self.lengths, keep)]
         self.drafted = None
+
+    def _paths(self, keep) -> list:
+        """`keep` as lists of ints; refuses what is no path of the drafted trees."""
+        if self.drafted is None:
+            raise RuntimeError("accept() follows verify()")
+        parents = self.drafted[1]
+        n = len(parents[0])
+        keep = [[int(i) for i in rows] for rows in keep]
+        if len(keep) != self.batch or any(not 0 <= i < n or parents[b][i] != up for b, rows in enumerate(keep) for up, i in zip([-1] + rows, rows)):
+            raise ValueError(f"keep gives a path of rows 0 .. {n - 1}, each the parent of the next, for each of the {self.batch} sequences")
+        return keep
 
 
 def _patched_forward(attn, state_of, original):
@@ -232,8 +239,13 @@ class PhasorKeyPatch:
             st.reset()
 
     def accept(self, keep) -> None:
-        """``LayerDecodeState.accept`` in every patched layer, after a verification pass of the model."""
-        for st in self.states.values():
+        """``LayerDecodeState.accept`` in every patched layer, after a verification pass of the model; a path that one layer refuses
+        changes none. Dropping all drafts (only empty paths) also ends a pass that failed on its way through the layers."""
+        keep = [[int(i) for i in rows] for rows in keep]
+        drafted = [st for st in self.states.values() if st.drafted is not None]
+        for st in drafted if drafted and not any(keep) else self.states.values():
+            st._paths(keep)
+        for st in drafted:
             st.accept(keep)
 
     @property

@@ -72,3 +72,48 @@ def test_verify_runs_on_the_device_of_its_cache(monkeypatch):
     r.state.accept([[0], [0, 1]])
     assert [c[0] for c in r.calls] == ["plan", "write", "attend", "keep", "truncate"]
     assert all(where == torch.device("cpu") for _, where in r.calls), r.calls
+
+
+# ------------------------------------------------------------------------------------------------ accept in all layers
+def two_layers(drafted):
+    """A patch of two layers, of which those in `drafted` wait for accept."""
+    p, rec = patch.PhasorKeyPatch(), [Recorder(), Recorder()]
+    for i, r in enumerate(rec):
+        if i in drafted:
+            r.state.drafted = (types.SimpleNamespace(), [[-1, 0, 0], [-1, 0, 1]])
+        p.states[i] = r.state
+    return p, rec
+
+
+@pytest.mark.parametrize("drafted,keep,error", [((0,), [[0], [0]], RuntimeError), ((0, 1), [[0], [1]], ValueError), ((0, 1), [[0]], ValueError)])
+def test_accept_refuses_in_all_layers_or_none(drafted, keep, error):
+    p, rec = two_layers(drafted)
+    with pytest.raises(error):
+        p.accept(keep)
+    assert all(r.calls == [] and r.state.lengths == [5, 9] for r in rec)
+    assert [r.state.drafted is not None for r in rec] == [i in drafted for i in range(2)]
+
+
+def test_accept_refuses_a_path_that_one_layer_did_not_draft():
+    p, rec = two_layers((0, 1))
+    rec[1].state.drafted = (types.SimpleNamespace(), [[-1, -1, 0], [-1, 0, 1]])
+    with pytest.raises(ValueError):
+        p.accept([[0, 1], [0]])
+    assert all(r.calls == [] and r.state.drafted is not None for r in rec)
+
+
+def test_accept_takes_the_paths_from_an_iterator_once(monkeypatch):
+    p, rec = two_layers((0, 1))
+    monkeypatch.setattr(patch, "on_device", rec[0].on_device, raising=False)
+    p.accept(iter(rows) for rows in ([0, 2], []))
+    assert all([c[0] for c in r.calls] == ["keep", "truncate"] and r.state.lengths == [7, 9] and r.state.drafted is None for r in rec)
+
+
+def test_dropping_all_drafts_ends_a_pass_that_failed_halfway(monkeypatch):
+    p, rec = two_layers((0,))
+    monkeypatch.setattr(patch, "on_device", rec[0].on_device, raising=False)
+    p.accept([[], []])
+    assert [[c[0] for c in r.calls] for r in rec] == [["keep", "truncate"], []]
+    assert all(r.state.lengths == [5, 9] and r.state.drafted is None for r in rec)
+    with pytest.raises(RuntimeError):
+        p.accept([[], []])
