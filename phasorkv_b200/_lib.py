@@ -16,6 +16,7 @@ MAX_WIDTH = 256
 QUERY_TERMS = 4
 NOALLOC_MAX_PARTS = 320
 TREE_MAX = 64
+SMALL_WRITE_TOKENS = 64
 F32, BF16, F64 = 0, 1, 2
 ATTN_SCORES_ONLY, ATTN_SIMT, ATTN_PACKED_OUT, ATTN_EARLY_STREAM, ATTN_TAIL_WRITTEN, ATTN_QUERY_READY = 1, 2, 4, 8, 16, 32
 EXCHANGE_PUSH, EXCHANGE_MERGE = 1, 2

@@ -271,7 +271,7 @@ class TreeWorkspace:
     """Scratch of `PhasorKey.tree_step` (the absorbed queries in operand form, partial results), reused by every layer of
     one shape and every step; ``status`` holds the kernels' status words."""
 
-    def __init__(self, pk: "PhasorKey", batch: int, capacity: int, max_draft: int, max_tokens: int):
+    def __init__(self, pk: "PhasorKey", batch: int, capacity: int, max_draft: int, max_tokens: int, own: bool = True):
         if not 1 <= max_draft <= _lib.TREE_MAX:
             raise ValueError(f"a tree has 1 .. {_lib.TREE_MAX} drafted tokens per sequence, not {max_draft}")
         if batch < 0 or capacity < 0 or max_tokens <= 0:
@@ -281,9 +281,17 @@ class TreeWorkspace:
         n = int(_lib.load().pkv_tree_workspace_bytes(ctypes.byref(pk._layer()), batch, max_draft, self.max_pages))
         if n < 0:
             _lib.check(n, "pkv_tree_workspace_bytes")
-        self.buffer = _aligned_bytes(n, pk.device)
         self.status = torch.zeros(4, dtype=torch.int32, device=pk.device)
-        self.at, self.bytes, self.status_at = self.buffer.data_ptr(), n, self.status.data_ptr()
+        self.bytes, self.status_at = n, self.status.data_ptr()
+        if own:
+            self.use(_aligned_bytes(n, pk.device))
+
+    def use(self, buffer: torch.Tensor) -> None:
+        """Work in `buffer`, a uint8 tensor of ``bytes`` or more at a multiple of 1024. Workspaces may share one if their calls run one after
+        the other."""
+        if buffer.dtype is not torch.uint8 or not buffer.is_contiguous() or buffer.numel() < self.bytes or buffer.data_ptr() % 1024:
+            raise ValueError(f"a workspace needs {self.bytes} contiguous bytes at a multiple of 1024")
+        self.buffer, self.at = buffer, buffer.data_ptr()
 
 
 class PhasorKey:
@@ -685,10 +693,11 @@ class PhasorKey:
         self.attend_step(cache, ws, simt=simt, scores_only=scores_only, out=ws.out, after_absorb=True)
         return ws.out
 
-    def tree_workspace(self, batch: int, capacity: int, max_draft: int, max_tokens: int) -> TreeWorkspace:
+    def tree_workspace(self, batch: int, capacity: int, max_draft: int, max_tokens: int, own: bool = True) -> TreeWorkspace:
         """Scratch of `tree_step` for up to `capacity` drafted tokens, `max_draft` (<= 64) a sequence, on caches of up to
-        `max_tokens` tokens a sequence. Calls that may run at the same time need one each."""
-        return TreeWorkspace(self, int(batch), int(capacity), int(max_draft), int(max_tokens))
+        `max_tokens` tokens a sequence. Calls that may run at the same time need one each. ``own=False``: without memory, which
+        `TreeWorkspace.use` gives it."""
+        return TreeWorkspace(self, int(batch), int(capacity), int(max_draft), int(max_tokens), own)
 
     def tree_step(self, cache: PagedLatentCache, q: torch.Tensor, plan: StepPlan, ws: TreeWorkspace,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:

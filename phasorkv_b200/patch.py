@@ -43,10 +43,36 @@ from typing import Optional
 
 import torch
 
-from ._lib import TREE_MAX, on_device
-from .latent import PAGE_TOKENS, PhasorKey
+from ._lib import SMALL_WRITE_TOKENS, TREE_MAX, on_device
+from .latent import PAGE_TOKENS, PhasorKey, _aligned_bytes
 
 NVFP4_BITS = 4.5          # E2M1 code + one E4M3 scale per 16 codes (phasorkv/quant.py:9)
+
+
+class VerifyScratch:
+    """Scratch of `LayerDecodeState.verify` for layers that run one after the other: per device and stream one buffer, as large as the
+    largest step so far, under the workspaces of all layer shapes and draft counts, and one scratch of the write kernel per model width. It moves when it grows, so a graph that captured
+    `verify` must not outlive a larger step."""
+
+    def __init__(self):
+        self.places = {}                                    # (device, stream) -> [buffer, {shape: workspace}, {width: write scratch}]
+
+    def take(self, pk: PhasorKey, batch: int, n: int, max_tokens: int, device, stream: int):
+        """Workspace and write scratch of n drafted tokens a sequence."""
+        place = self.places.setdefault((device, stream), [None, {}, {}])
+        buffer, spaces, writes = place
+        key = pk._tree_key(), batch, n, max_tokens
+        if key not in spaces:
+            ws = pk.tree_workspace(batch, batch * n, n, max_tokens, own=False)
+            if buffer is None or buffer.numel() < ws.bytes:
+                place[0] = buffer = _aligned_bytes(ws.bytes, device)
+                for other in spaces.values():
+                    other.use(buffer)
+            ws.use(buffer)
+            spaces[key] = ws
+        if pk.d_model not in writes:
+            writes[pk.d_model] = pk.write_scratch(SMALL_WRITE_TOKENS)          # (larger writes do not touch it)
+        return spaces[key], writes[pk.d_model]
 
 
 class LayerDecodeState:
@@ -57,7 +83,8 @@ class LayerDecodeState:
     cached, the next token of b is written at position ``lengths[b]`` and attends to positions
     ``0 .. lengths[b]``."""
 
-    def __init__(self, pk: PhasorKey, batch: int, max_tokens: int, write_chunk: int = 4096, v_bits: int = 0):
+    def __init__(self, pk: PhasorKey, batch: int, max_tokens: int, write_chunk: int = 4096, v_bits: int = 0,
+                 scratch: Optional[VerifyScratch] = None):
         self.pk, self.batch, self.max_tokens, self.write_chunk = pk, batch, max_tokens, write_chunk
         self.cache = pk.new_cache(batch, max_tokens, v_bits=v_bits)     # v_bits 3 / 2: V as per-token low-bit codes
         self.ws = pk.workspace(batch, pk.default_splits(batch, max_tokens))
@@ -65,7 +92,8 @@ class LayerDecodeState:
         self.lengths = [0] * batch                          # tokens cached per sequence (host copy of cache.seqlens)
         self.calibrated = False
         self.drafted = None                                 # plan and parents, between verify() and accept()
-        self.tree = {}                                      # drafts per sequence -> (plan, workspace, write scratch, counts)
+        self.tree = {}                                      # drafts per sequence -> (plan, workspace, counts, a chain's parents)
+        self.scratch = VerifyScratch() if scratch is None else scratch
 
     @property
     def length(self) -> int:
@@ -148,12 +176,12 @@ class LayerDecodeState:
                 raise ValueError("parents [batch, drafts] name a row before the token's own, or -1")
         for b in range(B):
             self._need(b, n)
-        with on_device(self.cache.latent.device):              # the writer's launches go to the current device
+        with on_device(self.cache.latent.device) as stream:    # the writer's launches go to the current device
+            ws, scratch = self.scratch.take(pk, B, n, self.max_tokens, self.cache.latent.device, stream)
             if n not in self.tree:
-                self.tree[n] = (self.cache.step_plan(B * n, tree=True), pk.tree_workspace(B, B * n, n, self.max_tokens), pk.write_scratch(B * n),
-                                torch.full((B,), n, dtype=torch.int32, device=dev),
+                self.tree[n] = (self.cache.step_plan(B * n, tree=True), ws, torch.full((B,), n, dtype=torch.int32, device=dev),
                                 torch.arange(-1, n - 1, dtype=torch.int32, device=dev).repeat(B))
-            plan, ws, scratch, n_new, chain = self.tree[n]
+            plan, _, n_new, chain = self.tree[n]
             parents = chain if parents is None else parents.to(device=dev, dtype=torch.int32).reshape(B * n).contiguous()
             x, v = x.reshape(B * n, -1).contiguous(), v.reshape(B * n, pk.n_kv, pk.head_dim).contiguous()
             q = q.reshape(B * n, pk.n_q, pk.head_dim).contiguous()
@@ -232,6 +260,7 @@ class PhasorKeyPatch:
         self.layer_stats = {}
         self.keys = {}
         self.states = {}
+        self.scratch = VerifyScratch()    # of all layers: they run one after the other
 
     def reset(self) -> None:
         """Forget the cached tokens of every patched layer (a new prompt follows)."""
@@ -282,7 +311,7 @@ class PhasorKeyPatch:
             def state_of(batch, i=i, pk=pk):
                 st = self.states.get(i)
                 if st is None or st.batch != batch:
-                    st = self.states[i] = LayerDecodeState(pk, batch, max_tokens, v_bits=self.v_bits)
+                    st = self.states[i] = LayerDecodeState(pk, batch, max_tokens, v_bits=self.v_bits, scratch=self.scratch)
                 return st
             attn.forward = _patched_forward(attn, state_of, original)
 

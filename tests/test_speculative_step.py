@@ -155,3 +155,59 @@ def test_a_verification_that_fails_leaves_the_layer_as_it_was(fails, monkeypatch
     assert torch.equal(st.verify(x, q, v), other.verify(x, q, v))
     st.accept([[0], []])
     assert st.cache.seqlens.tolist() == st.lengths == [127, 126]
+
+
+def patched_layers(k):
+    """k attention layers with patched forwards -> (layers, their undo calls, the patch)"""
+    spec = synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0)
+    lin = lambda i, o: torch.nn.Linear(i, o, bias=False, device="cuda", dtype=torch.float32)
+
+    class Attn(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.head_dim = 128
+            self.q_proj, self.v_proj, self.o_proj = lin(D, 32 * 128), lin(D, 8 * 128), lin(32 * 128, D)
+
+        def forward(self, hidden_states, **kw):
+            return hidden_states, None
+    layers = [types.SimpleNamespace(self_attn=Attn()) for _ in range(k)]
+    patch = PhasorKeyPatch(install_forward=True, max_tokens=512)
+    return layers, [patch.patch(i, y, spec, 8, 128, 32, "cuda") for i, y in enumerate(layers)], patch
+
+
+def test_layers_and_draft_counts_share_their_scratch():
+    """The workspaces of verification are the larger part of its memory: one buffer for all layers of a patch, whatever their draft counts."""
+    layers, undo, patch = patched_layers(3)
+    g = torch.Generator(device="cuda").manual_seed(7)
+    h = lambda n: torch.randn((2, n, D), generator=g, device="cuda")
+    with torch.no_grad():
+        for y in layers:
+            y.self_attn(h(20))
+            y.self_attn.kv_tree = "chain"
+        before = torch.cuda.memory_allocated()
+        for n in (1, 2, 3, 5, 8, 13, 21, 34, 64, 7):
+            drafts = h(n)
+            for y in layers:
+                y.self_attn(drafts)
+            patch.accept([[], [0]])
+    spaces = [w[1] for st in patch.states.values() for w in st.tree.values()]
+    assert len(spaces) == 30 and len({w.buffer.data_ptr() for w in spaces}) == 1
+    largest = max(w.bytes for w in spaces)
+    assert torch.cuda.memory_allocated() - before < 1.5 * largest          # the rest: plans and results, a few hundred KB
+    for u in undo:
+        u()
+
+
+def test_a_shared_workspace_that_grew_still_serves_the_small_steps():
+    """Draft counts up and down over layers that share their scratch: the outputs are those of layers of their own."""
+    pk = PhasorKey.from_spec(synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0))
+    g = torch.Generator(device="cuda").manual_seed(8)
+    t = lambda *s: torch.randn(s, generator=g, device="cuda")
+    x0, v0 = t(2, 100, D), t(2, 100, 8, 128)
+    shared, own = [state(pk, 2, 0, x0, v0) for _ in range(2)], [state(pk, 2, 0, x0, v0) for _ in range(2)]
+    shared[1].scratch = shared[0].scratch
+    for n in (2, 40, 2, 64, 1, 40):
+        x, q, v = t(2, n, D), t(2, n, 32, 128), t(2, n, 8, 128)
+        for a, b in zip(shared, own):
+            assert torch.equal(a.verify(x, q, v), b.verify(x, q, v))
+            a.accept([[0], []]), b.accept([[0], []])

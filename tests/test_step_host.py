@@ -25,13 +25,14 @@ class Recorder:
         self.calls, self.inside = [], None
         note = lambda name: lambda *a, **k: self.calls.append((name, self.inside))
         self.pk = types.SimpleNamespace(device=torch.device("cpu"), d_model=D, n_q=N_Q, n_kv=N_KV, head_dim=128, cache_width=64, write_paged=note("write"),
-                                        write_scratch=lambda n: None, tree_workspace=lambda *a, **k: types.SimpleNamespace(status=None),
+                                        write_scratch=lambda n: None, _tree_key=lambda: 0, tree_workspace=lambda *a, **k: types.SimpleNamespace(bytes=4, use=lambda b: None),
                                         tree_step=lambda cache, q, plan, ws, **k: (self.calls.append(("attend", self.inside)), torch.zeros(q.shape))[1])
         plan = types.SimpleNamespace(positions=None, slots=None)
         self.cache = types.SimpleNamespace(latent=torch.zeros(1), step_plan=lambda *a, **k: plan, plan_step=note("plan"), truncate=note("truncate"),
                                            keep_rows=note("keep"))
         st = self.state = object.__new__(LayerDecodeState)
         st.pk, st.cache, st.batch, st.max_tokens, st.lengths, st.drafted, st.tree = self.pk, self.cache, batch, 256, [5, 9], None, {}
+        st.scratch = patch.VerifyScratch()
 
     @contextlib.contextmanager
     def on_device(self, device):
