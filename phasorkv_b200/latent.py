@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import weakref
 from typing import Optional, Sequence
 
 import torch
@@ -69,6 +70,7 @@ class PagedLatentCache:
         self.page_table = (pt % self.n_pages).to(self.device)
         self.seqlens = torch.zeros(batch, dtype=torch.int32, device=self.device)
         self.free = None                                    # page pool, see use_page_pool()
+        self.sharers = [weakref.ref(self)]                  # the caches that go by these tables, see share_pages()
         self.status = None                                  # status words of truncate / keep_rows, made with the first plan
         self.c = _lib.Cache(self.latent.data_ptr(), 0 if self.v is None else self.v.data_ptr(), self.n_pages, W,
                             n_kv, head_dim, 0 if self.vq is None else self.vq.data_ptr(), self.v_bits)
@@ -82,18 +84,29 @@ class PagedLatentCache:
     # ------------------------------------------------------------------ pages of a step
     def use_page_pool(self) -> None:
         """Pages are handed out by `plan_step` and come back with `truncate` from here on, instead of every sequence owning a
-        fixed row of them. Forgets what is cached. ``free[0]`` counts the free pages, ``free[free[0]]`` is the next."""
-        self.free = torch.cat([torch.tensor([self.n_pages], dtype=torch.int32),
-                               torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32)]).to(self.device)
+        fixed row of them. Forgets what is cached. ``free[0]`` counts the free pages, ``free[free[0]]`` is the next. Holds for
+        all caches that share the tables; a pool that is there already is filled again in place."""
+        pool = torch.cat([torch.tensor([self.n_pages], dtype=torch.int32), torch.arange(self.n_pages - 1, -1, -1, dtype=torch.int32)])
+        if self.free is not None:
+            self.free.copy_(pool)
+        else:
+            pool = pool.to(self.device)
+            for cache in filter(None, (ref() for ref in self.sharers)):
+                cache.free = pool
         self.page_table.fill_(-1)
         self.seqlens.zero_()
 
     def share_pages(self, owner: "PagedLatentCache") -> None:
-        """Address this layer's pools by `owner`'s page table, lengths and pool (one plan then serves all layers)."""
+        """Address this layer's pools by `owner`'s page table, lengths and pool (one plan then serves all layers), whether `owner`
+        has its page pool already or gets it later."""
         mine, theirs = ((c.batch, c.max_pages, c.n_pages, c.latent.device) for c in (self, owner))
         if mine != theirs:
             raise ValueError("caches that share pages have the same batch, pages per sequence, pool size and device")
         self.page_table, self.seqlens, self.free = owner.page_table, owner.seqlens, owner.free
+        if self.sharers is not owner.sharers:
+            self.sharers[:] = [ref for ref in self.sharers if ref() not in (None, self)]
+            self.sharers = owner.sharers
+            self.sharers.append(weakref.ref(self))
 
     def _pages(self) -> _lib.Pages:
         return _lib.Pages(self.page_table.data_ptr(), self.seqlens.data_ptr(), 0 if self.free is None else self.free.data_ptr(),

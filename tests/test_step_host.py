@@ -5,7 +5,7 @@ import types
 import pytest
 import torch
 
-from phasorkv_b200 import build, patch
+from phasorkv_b200 import PagedLatentCache, build, patch
 from phasorkv_b200.patch import LayerDecodeState
 
 
@@ -118,3 +118,41 @@ def test_dropping_all_drafts_ends_a_pass_that_failed_halfway(monkeypatch):
     assert all(r.state.lengths == [5, 9] and r.state.drafted is None for r in rec)
     with pytest.raises(RuntimeError):
         p.accept([[], []])
+
+
+# ------------------------------------------------------------------------------------------------ page pool and sharing
+def caches(k):
+    return [PagedLatentCache(256, 8, 128, 2, 512, "cpu") for _ in range(k)]
+
+
+@pytest.mark.parametrize("who", [0, 1, 2])
+def test_a_page_pool_made_after_sharing_is_everyones(who):
+    a, b, c = caches(3)
+    b.share_pages(a), c.share_pages(b)
+    (a, b, c)[who].use_page_pool()
+    assert a.free is b.free is c.free and a.free.tolist() == [8, 7, 6, 5, 4, 3, 2, 1, 0] and int(a.page_table.max()) == -1
+
+
+def test_a_page_pool_is_refilled_in_place():
+    """A captured step and the caches that share the pool go on with the same array."""
+    a, b = caches(2)
+    a.use_page_pool()
+    b.share_pages(a)
+    pool = a.free
+    pool[0] = 3
+    a.page_table[0, 0], a.seqlens[1] = 4, 77
+    b.use_page_pool()
+    assert a.free is pool and b.free is pool and pool.tolist() == [8, 7, 6, 5, 4, 3, 2, 1, 0]
+    assert int(a.page_table.max()) == -1 and a.seqlens.tolist() == [0, 0]
+
+
+def test_a_cache_that_shares_with_another_leaves_its_first_owner():
+    a, b, c = caches(3)
+    b.share_pages(a)
+    b.share_pages(c)
+    a.use_page_pool()
+    assert b.free is None and c.free is None and b.page_table is c.page_table
+    c.use_page_pool()
+    assert b.free is c.free and b.free is not a.free
+    c.share_pages(c)
+    assert c.free is b.free
