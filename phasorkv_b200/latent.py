@@ -730,8 +730,11 @@ class PhasorKey:
         plan._match(cache)
         if n > plan.capacity or n > ws.capacity or ws.batch != cache.batch or ws.max_pages < cache.max_pages or ws.key != self._tree_key():
             raise ValueError("q has more rows than the plan or the workspace, or the workspace was made for another layer shape or cache")
+        layer = self._layer()
+        if self._dev["Bw"].device != dev or ws.buffer.device != dev or ws.status.device != dev:
+            raise ValueError(f"the layer's factors, on {self._dev['Bw'].device}, and the workspace, on {ws.buffer.device}, must be on the cache's device {dev}")
         with _lib.on_device(dev) as stream:
-            st = _lib.load().pkv_tree_attn(ctypes.byref(self._layer()), ctypes.byref(cache.c), ctypes.byref(cache._pages()), q.data_ptr(),
+            st = _lib.load().pkv_tree_attn(ctypes.byref(layer), ctypes.byref(cache.c), ctypes.byref(cache._pages()), q.data_ptr(),
                                            self._xdt(q), plan.c.positions_dev, plan.c.mask_dev, plan.c.cu_dev, n, ws.max_draft, ws.at, ws.bytes,
                                            out.data_ptr(), ws.status_at, stream)
         if st:

@@ -5,7 +5,7 @@ import types
 import pytest
 import torch
 
-from phasorkv_b200 import PagedLatentCache, build, patch
+from phasorkv_b200 import PagedLatentCache, PhasorKey, TreeWorkspace, _lib, build, patch
 from phasorkv_b200.patch import LayerDecodeState
 
 
@@ -156,3 +156,18 @@ def test_a_cache_that_shares_with_another_leaves_its_first_owner():
     assert b.free is c.free and b.free is not a.free
     c.share_pages(c)
     assert c.free is b.free
+
+
+# ------------------------------------------------------------------------------------------------ devices of a tree step
+@pytest.mark.parametrize("wrong", ["workspace", "layer"])
+def test_tree_step_refuses_another_devices_workspace_or_layer(wrong):
+    cpu = torch.zeros(1)
+    pk = PhasorKey.from_factors(torch.zeros((8, 128), dtype=torch.complex64), torch.zeros((128, 16), dtype=torch.complex64), torch.arange(128) // 2, 32, 8, 128,
+                                torch.ones(64, dtype=torch.float64), device="cpu")
+    pk._dev = {"Bw": cpu.to("meta") if wrong == "layer" else cpu, "layer": _lib.Layer()}
+    cache = PagedLatentCache(256, 8, 128, 1, 128, "cpu")
+    ws = object.__new__(TreeWorkspace)
+    ws.buffer = ws.status = cpu.to("meta") if wrong == "workspace" else cpu
+    ws.batch, ws.capacity, ws.max_draft, ws.max_pages, ws.key, ws.at, ws.bytes, ws.status_at = 1, 4, 4, 1, pk._tree_key(), 0, 0, 0
+    with pytest.raises(ValueError, match="device"):
+        pk.tree_step(cache, torch.zeros((4, 32, 128)), cache.step_plan(4), ws)
