@@ -455,12 +455,14 @@ typedef struct pkv_plan {
  * words: a caller's own masks are written after this call.  Behind the last token slots are -1 and
  * the other arrays are left as they were.
  * When a length, a parent or the pool does not allow the step, the call changes no table and no length, cu is all zero,
- * every slot is -1 and the status says why.  batch <= 4096.  n_new_dev and parents_dev are not the plan's own arrays. */
+ * every slot is -1 and the status says why.  batch <= 4096.  n_new_dev, parents_dev and the tables share no memory with what the plan
+ * gets (PKV_ERR_INVALID). */
 int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev, const int32_t* parents_dev, const pkv_plan_t* plan,
                   void* stream);
 
 /* seqlens[b] = min(seqlens[b], lengths_dev[b]); pages that hold no token any more go back to the pool, their table entries
- * become -1.  A step that is planned and dropped leaves the pool as it was.  lengths_dev must not be seqlens_dev. */
+ * become -1.  A step that is planned and dropped leaves the pool as it was.  lengths_dev shares no memory with
+ * the tables or the status (PKV_ERR_INVALID). */
 int pkv_truncate(const pkv_pages_t* pages, const int32_t* lengths_dev, int32_t* status_dev, void* stream);
 
 /* Attention of drafted tokens: row i of sequence b's rows cu_dev[b] .. cu_dev[b+1]-1 attends to the sequence's cached tokens
@@ -484,7 +486,7 @@ int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache, const pkv_
  * rows count) names rows of the step's tokens in ascending order; row base + keep[j] moves to base + j, base = seqlens -
  * (cu[b+1] - cu[b]), in the latent and value pages of every layer (layers: host array of n_layers caches that are addressed
  * by the same table; no cache twice).  Only bytes move: a token keeps its rotation, so a kept path's positions must
- * be base, base + 1, ... (in a tree, depths 0, 1, ...).  lengths_out_dev (optional, [batch], none of the inputs): base + n_keep,
+ * be base, base + 1, ... (in a tree, depths 0, 1, ...).  lengths_out_dev (optional, [batch], no memory of the inputs): base + n_keep,
  * for pkv_truncate.  Lengths and tables stay as they are.  A sequence whose indices do not ascend or are out of range is
  * left alone (status 4, lengths_out = its length). */
 int pkv_keep_rows(const pkv_cache_t* const* layers, int32_t n_layers, const pkv_pages_t* pages, const int32_t* cu_dev,

@@ -344,17 +344,36 @@ int check_pages(const pkv_pages_t* p) {
     return PKV_OK;
 }
 
+// An array that a call only reads must not reach into one that it writes: other CTAs, or other threads, still read it then.
+struct Span { const void* p; int64_t words; };       // 32-bit words
+bool overlap(const Span& a, const Span& b) {
+    if (!a.p || !b.p || a.words <= 0 || b.words <= 0) return false;
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return x < y ? y - x < (uintptr_t)a.words * 4 : x - y < (uintptr_t)b.words * 4;
+}
+template <int N, int M>
+bool any_overlap(const Span (&a)[N], const Span (&b)[M]) {
+    for (const Span& x : a)
+        for (const Span& y : b)
+            if (overlap(x, y)) return true;
+    return false;
+}
+
 }  // namespace
 
 extern "C" int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev, const int32_t* parents_dev, const pkv_plan_t* plan,
                              void* stream) {
     int st = check_pages(pages);
     if (st) return st;
-    if (!n_new_dev || !plan || !plan->cu_dev || !plan->ticket_dev || plan->capacity < 0 || plan->cu_dev == pages->seqlens_dev) return PKV_ERR_INVALID;
+    if (!n_new_dev || !plan || !plan->cu_dev || !plan->ticket_dev || plan->capacity < 0) return PKV_ERR_INVALID;
     if (plan->capacity > 0x3fffffff) return PKV_ERR_UNSUPPORTED;
-    // several CTAs read what the caller gives while the first already writes
-    auto written = [&](const int32_t* p) { return p && (p == plan->cu_dev || p == plan->seq_dev || p == plan->positions_dev || p == plan->slots_dev); };
-    if (written(n_new_dev) || written(parents_dev)) return PKV_ERR_INVALID;
+    // several CTAs read what the caller gives, and the tables, while the first already writes
+    const int64_t cap = plan->capacity, B = pages->batch;
+    const Span read[] = {{n_new_dev, B}, {parents_dev, cap}, {pages->page_table_dev, B * pages->max_pages}, {pages->seqlens_dev, B},
+                         {pages->free_dev, (int64_t)pages->n_pages + 1}};
+    const Span written[] = {{plan->cu_dev, B + 1}, {plan->seq_dev, cap}, {plan->positions_dev, cap}, {plan->slots_dev, cap}, {plan->mask_dev, 2 * cap},
+                            {plan->ticket_dev, 1}, {plan->status_dev, 4}};
+    if (any_overlap(read, written)) return PKV_ERR_INVALID;
     if (plan->capacity > 0 && (!plan->seq_dev || !plan->positions_dev || !plan->slots_dev || (parents_dev && !plan->mask_dev))) return PKV_ERR_INVALID;
     if (pages->batch == 0) return PKV_OK;
     PlanArgs A{*pages, *plan, n_new_dev, parents_dev};
@@ -366,7 +385,11 @@ extern "C" int pkv_plan_step(const pkv_pages_t* pages, const int32_t* n_new_dev,
 extern "C" int pkv_truncate(const pkv_pages_t* pages, const int32_t* lengths_dev, int32_t* status_dev, void* stream) {
     int st = check_pages(pages);
     if (st) return st;
-    if (!lengths_dev || lengths_dev == pages->seqlens_dev) return PKV_ERR_INVALID;
+    if (!lengths_dev) return PKV_ERR_INVALID;
+    const Span read[] = {{lengths_dev, pages->batch}};
+    const Span written[] = {{pages->page_table_dev, (int64_t)pages->batch * pages->max_pages}, {pages->seqlens_dev, pages->batch},
+                            {pages->free_dev, (int64_t)pages->n_pages + 1}, {status_dev, 4}};
+    if (any_overlap(read, written)) return PKV_ERR_INVALID;
     if (pages->batch == 0) return PKV_OK;
     PKV_CUDA_TRY(pkv_launch_chained(pkv_truncate_kernel, dim3(1), dim3(NT), 0, (cudaStream_t)stream, *pages, lengths_dev, status_dev));
     return PKV_OK;
@@ -377,8 +400,11 @@ extern "C" int pkv_keep_rows(const pkv_cache_t* const* layers, int32_t n_layers,
                              int32_t* status_dev, void* stream) {
     int st = check_pages(pages);
     if (st) return st;
-    if (!layers || n_layers <= 0 || !cu_dev || (capacity > 0 && !keep_dev) || !n_keep_dev || capacity < 0 || lengths_out_dev == pages->seqlens_dev) return PKV_ERR_INVALID;
-    if (lengths_out_dev && (lengths_out_dev == n_keep_dev || lengths_out_dev == keep_dev || lengths_out_dev == cu_dev)) return PKV_ERR_INVALID;   // (read by other CTAs)
+    if (!layers || n_layers <= 0 || !cu_dev || (capacity > 0 && !keep_dev) || !n_keep_dev || capacity < 0) return PKV_ERR_INVALID;
+    const int64_t B = pages->batch;
+    const Span read[] = {{cu_dev, B + 1}, {keep_dev, capacity}, {n_keep_dev, B}, {pages->page_table_dev, B * pages->max_pages}, {pages->seqlens_dev, B}};
+    const Span written[] = {{lengths_out_dev, B}, {status_dev, 4}};
+    if (any_overlap(read, written)) return PKV_ERR_INVALID;
     for (int i = 0; i < n_layers; ++i) {
         const pkv_cache_t* c = layers[i];
         st = pkv_check_cache(c);

@@ -361,3 +361,28 @@ def test_a_plan_with_masks_has_a_chains_without_parents(new):
     words = [(1 << min(i + 1, 64)) - 1 for m in new for i in range(m)]
     assert plan.mask.tolist() == [w - (1 << 64) if w >> 63 else w for w in words] + [0x5a5a] * 4
     assert plan.positions[:sum(new)].tolist() == [i for m in new for i in range(m)] and int(plan.status[0]) == 0
+
+
+@pytest.mark.parametrize("out", ["cu", "seq", "positions", "slots", "mask", "ticket", "status"])
+@pytest.mark.parametrize("shift", [-4, 0, 4])
+def test_c_entries_refuse_arrays_that_overlap(lib, out, shift):
+    """An input that begins inside a result, or reaches into it, is written while other CTAs still read it."""
+    pg = _lib.Pages(4096, 8192, 0, 2, 4, 8)
+    at = dict(cu=(0x10000, 12), seq=(0x20000, 32), positions=(0x30000, 32), slots=(0x40000, 32), mask=(0x50000, 64), ticket=(0x60000, 4), status=(0x70000, 16))
+    plan = _lib.Plan(*[at[k][0] for k in ("cu", "seq", "positions", "slots", "mask", "ticket", "status")], 8)
+    begin, size = at[out]
+    inside = begin + size - 4 if shift > 0 else begin + shift                     # its last word; itself; an array that ends in its first word
+    assert lib.pkv_plan_step(ctypes.byref(pg), inside, None, ctypes.byref(plan), None) == -1
+    assert lib.pkv_plan_step(ctypes.byref(pg), 0x9000, inside, ctypes.byref(plan), None) == -1
+
+
+@pytest.mark.parametrize("shift", [-4, 0, 4])
+def test_c_entries_refuse_lengths_that_overlap(lib, shift):
+    pg, cache = _lib.Pages(0x10000, 0x20000, 0x30000, 2, 4, 8), _lib.Cache(4096, 4096, 8, 256, 8, 128)
+    one = (ctypes.c_void_p * 1)(ctypes.addressof(cache))
+    for begin, size in ((0x10000, 32), (0x20000, 8), (0x30000, 36)):              # table, lengths, pool
+        inside = begin + size - 4 if shift > 0 else begin + shift
+        assert lib.pkv_truncate(ctypes.byref(pg), inside, None, None) == -1
+    for begin, size in ((0x10000, 32), (0x20000, 8), (0x40000, 12), (0x50000, 16), (0x60000, 8)):          # .. cu, keep, n_keep
+        inside = begin + size - 4 if shift > 0 else begin + shift
+        assert lib.pkv_keep_rows(one, 1, ctypes.byref(pg), 0x40000, 4, 0x50000, 0x60000, inside, None, None) == -1
