@@ -425,7 +425,9 @@ int pkv_decode_attn_noalloc(const pkv_layer_t* layer, const pkv_cache_t* cache, 
  * decodes token by token and has no pages).  Ragged: the tokens of sequence b are the rows cu[b] .. cu[b+1]-1 of every
  * per-token array.  All lengths live on the device, so that a step can be captured in a CUDA graph and replayed.
  * status_dev words of these calls besides 1 and 2 above: 4 = a length, a parent or an index out of range (word 1: the
- * sequence), 5 = the page pool has too few pages (word 1: how many are missing) or would get back more than it has. */
+ * sequence, one of them if there are several; -1: all together), 5 = the page pool has too few pages (word 1: how many are
+ * missing) or would get back more than it has (-1).  Words 0 and 1 tell of the first problem since the caller set them to zero;
+ * a call without one leaves them as they are. */
 
 /* The page table of a batch.  free_dev: optional page pool, int32 [n_pages + 1]: the number of free pages, then the free
  * pages as a stack (the next page is free_dev[free_dev[0]]).  NULL: every table row is filled for good. */

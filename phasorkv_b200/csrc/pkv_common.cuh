@@ -69,6 +69,12 @@ inline cudaError_t pkv_launch_chained(void (*kern)(KArgs...), dim3 grid, dim3 bl
     return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
 }
 
+// Status words of a call whose CTAs (or launches) may run into different problems: the first since the caller cleared the words
+// stays, so that both words tell of the same one.
+__device__ __forceinline__ void pkv_report(int32_t* status, int code, int where) {
+    if (status && atomicCAS(&status[0], 0, code) == 0) atomicExch(&status[1], where);
+}
+
 // ------------------------------------------------------------------------------------------------
 // page layout (documented in include/phasorkv_b200.h)
 // ------------------------------------------------------------------------------------------------

@@ -19,10 +19,6 @@ constexpr int FILL = 4 * NT;                         // tokens per CTA before an
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + PKV_PAGE_TOKENS - 1) / PKV_PAGE_TOKENS; }
 
-__device__ __forceinline__ void refuse(int32_t* status, int code, int where) {
-    if (status) { atomicExch(&status[0], code); atomicExch(&status[1], where); }
-}
-
 // the last index s with sums[s] <= i, for ascending sums[0 .. n]; empty entries (equal neighbours) are skipped
 __device__ __forceinline__ int owner_of(const int* sums, int n, int i) {
     int lo = 0, hi = n;                              // sums[lo] <= i < sums[hi]
@@ -112,7 +108,7 @@ __global__ void __launch_bounds__(NT) pkv_plan_step_kernel(const PlanArgs A) {
         }
         refused = __syncthreads_or(bad) != 0;
     }
-    if (bad && blockIdx.x == 0) refuse(A.plan.status_dev, bad, where);
+    if (bad && blockIdx.x == 0) pkv_report(A.plan.status_dev, bad, where);
 
     // Four tokens per thread, stored as one vector each where the arrays allow it: mostly of one sequence and page, so one search,
     // one length and one page index serve them.
@@ -218,7 +214,7 @@ __global__ void __launch_bounds__(NT) pkv_truncate_kernel(const pkv_pages_t pg, 
     if (tid == 0) off_s[B] = (int)run[0];
     if (run[0] > pg.n_pages - count) { bad = 5; where = -1; }       // more pages than the pool ever held
     const bool refused = __syncthreads_or(bad) != 0;
-    if (bad) refuse(status, bad, where);
+    if (bad) pkv_report(status, bad, where);
     if (refused) return;
     const int K = (int)run[0];
     for (int k = tid; k < K; k += NT) {
@@ -283,7 +279,7 @@ __global__ void __launch_bounds__(KT) pkv_keep_rows_kernel(const KeepArgs A) {
     }
     const bool refused = __syncthreads_or(!ok) != 0;
     if (blockIdx.x == 0 && blockIdx.z == 0 && tid == 0) {
-        if (refused) refuse(A.status, 4, b);
+        if (refused) pkv_report(A.status, 4, b);
         if (A.lengths_out) A.lengths_out[b] = refused ? L : base + nk;
     }
     if (refused || n_moves == 0) return;

@@ -290,7 +290,7 @@ __global__ void __launch_bounds__(AR * WP / 16) pkv_tree_absorb_kernel(const Abs
     int lo, n, T;
     const int pages = A.B.pages(b, lo, n, T);
     if (pages == 0) {
-        if (n != 0 && A.status && tid == 0 && blockIdx.x == 0 && z == 0) { atomicExch(&A.status[0], 4); atomicExch(&A.status[1], b); }
+        if (n != 0 && tid == 0 && blockIdx.x == 0 && z == 0) pkv_report(A.status, 4, b);
         return;
     }
     const Shape t = A.X.of(n);
@@ -464,7 +464,7 @@ __device__ __noinline__ bool wait_longer(uint64_t* bar, uint32_t parity, Shared*
         if ((i & 1023u) == 1023u && X->abort_flag) return false;
     }
     X->abort_flag = 1;
-    if (status) { atomicExch(&status[0], 1); atomicExch(&status[1], where); }
+    pkv_report(status, 1, where);
     return false;
 }
 // bounded; false when it gave up, or another role did (out of line: it is in many places, and the code has to stay small)
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                     const int st = k % C::NK, page = A.page_table[(size_t)s.b * A.B.max_pages + p];
                     if (page < 0 || page >= A.n_pages) {               // never dereferenced
                         X->abort_flag = 1;
-                        if (A.status) { atomicExch(&A.status[0], 2); atomicExch(&A.status[1], p); }
+                        pkv_report(A.status, 2, p);
                         ok = false;
                         break;
                     }

@@ -127,7 +127,8 @@ class PagedLatentCache:
         and the tokens' sequence, position, slot and, in a plan with masks, ancestor mask into `plan`.
         ``parents[i]`` (int32 [capacity]) is the row of token i's parent among its sequence's new tokens, before i, or -1;
         positions are then length + depth. Without `parents` the tokens are a chain, in the masks too (masks of the
-        caller's own are written after this call). A step that does not fit changes nothing: ``plan.cu`` is zero, every slot -1, ``plan.status`` says why."""
+        caller's own are written after this call). A step that does not fit changes nothing: ``plan.cu`` is zero, every slot -1, ``plan.status`` says why
+        (like the status words of the other calls of a step: the first problem since the caller zeroed them)."""
         _lib.need(n_new, torch.int32, (self.batch,), self.latent.device, "n_new")
         if parents is not None:
             _lib.need(parents, torch.int32, (plan.capacity,), self.latent.device, "parents")

@@ -386,3 +386,21 @@ def test_c_entries_refuse_lengths_that_overlap(lib, shift):
     for begin, size in ((0x10000, 32), (0x20000, 8), (0x40000, 12), (0x50000, 16), (0x60000, 8)):          # .. cu, keep, n_keep
         inside = begin + size - 4 if shift > 0 else begin + shift
         assert lib.pkv_keep_rows(one, 1, ctypes.byref(pg), 0x40000, 4, 0x50000, 0x60000, inside, None, None) == -1
+
+
+@pytest.mark.gpu
+def test_the_first_problem_stays_until_it_is_cleared():
+    """Both status words tell of one problem, however many there are."""
+    cache = PagedLatentCache(128, 1, 128, 3, 512, "cuda", with_v=False, n_pages=4)
+    cache.use_page_pool()
+    plan = cache.step_plan(2000)
+    cache.plan_step(plan, i32([1, -1, 1]))
+    assert plan.status[:2].tolist() == [4, 1]
+    cache.plan_step(plan, i32([512, 512, 512]))                                   # eight pages missing
+    assert plan.status[:2].tolist() == [4, 1]
+    plan.status.zero_()
+    cache.plan_step(plan, i32([512, 512, 512]))
+    assert plan.status[:2].tolist() == [5, 8]
+    cache.truncate(i32([0, 0, -1]))
+    cache.truncate(i32([-1, 0, 0]))
+    assert cache.status[:2].tolist() == [4, 2]

@@ -497,3 +497,18 @@ def test_a_chain_planned_where_a_tree_was(v_bits):
     c.words = [tree_words(random.Random(0), m, "chain") for m in n]
     c.positions = [[b + i for i in range(m)] for b, m in zip(base, n)]
     c.check(c.run())
+
+
+@pytest.mark.gpu
+def test_the_status_words_of_a_tree_step_belong_together():
+    """A sequence that is left out (noticed by the operand launch) and a bad page (by the attention): one of the two, not a mixture."""
+    c = Case(layer(32, 8), [700, 400, 20], [3, 9, 2])
+    ws = c.pk.tree_workspace(3, c.cap, 8, c.cache.max_pages * PAGE)
+    c.cache.page_table[0, 2] = -1
+    for _ in range(20):
+        ws.status.zero_()
+        c.pk.tree_step(c.cache, c.q, c.plan, ws)
+        assert ws.status[:2].tolist() in ([4, 1], [2, 2])
+    ws.status.copy_(torch.tensor([4, 77, 0, 0], dtype=torch.int32))               # not cleared: the first problem stays
+    c.pk.tree_step(c.cache, c.q, c.plan, ws)
+    assert ws.status[:2].tolist() == [4, 77]
