@@ -13,6 +13,8 @@ import torch
 from phasorkv_b200 import PhasorKey, PhasorKeyPatch, synth
 from phasorkv_b200.patch import LayerDecodeState
 
+from test_tree_attn import Case
+
 pytestmark = pytest.mark.gpu
 NORM = 8e-3
 D = 256
@@ -211,3 +213,125 @@ def test_a_shared_workspace_that_grew_still_serves_the_small_steps():
         for a, b in zip(shared, own):
             assert torch.equal(a.verify(x, q, v), b.verify(x, q, v))
             a.accept([[0], []]), b.accept([[0], []])
+
+
+def test_paths_of_different_lengths():
+    """Sequences that accept different numbers of rows, none among them: what follows is what each alone would have given."""
+    pk = PhasorKey.from_spec(synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0))
+    B, T, n = 3, 121, 7
+    g, r = torch.Generator(device="cuda").manual_seed(6), random.Random(6)
+    t = lambda *s: torch.randn(s, generator=g, device="cuda")
+    x0, v0 = t(B, T, D), t(B, T, 8, 128).to(torch.bfloat16)
+    many, alone = state(pk, B, 0, x0, v0), []
+    for b in range(B):
+        st = LayerDecodeState(pk, 1, 512)
+        st.calibrated = True                                         # one scale for all: the batch's
+        st.prefill(x0[b:b + 1], v0[b:b + 1])
+        alone.append(st)
+    for round_ in range(4):
+        x, q, v = t(B, n, D), 20 * t(B, n, 32, 128), t(B, n, 8, 128).to(torch.bfloat16)      # logits of a few units
+        parents = [[r.randint(max(-1, i - 3), i - 1) for i in range(n)] for _ in range(B)]
+        out = many.verify(x, q, v, torch.tensor(parents))
+        paths = []
+        for b in range(B):
+            path = [r.randrange(n)]
+            while parents[b][path[0]] >= 0:
+                path.insert(0, parents[b][path[0]])
+            paths.append(path[:[0, 1, n][(b + round_) % 3]])
+        many.accept(paths)
+        for b, path in enumerate(paths):
+            for j in path:
+                want = alone[b].decode(x[b:b + 1, j], q[b:b + 1, j], v[b:b + 1, j])
+                assert rel(out[b, j], want[0]) < NORM, (round_, b, j)
+        assert many.lengths == [st.lengths[0] for st in alone] and many.cache.seqlens.tolist() == many.lengths
+    assert len(set(many.lengths)) == 3
+
+
+def test_ragged_trees_over_layers_that_share_a_page_pool():
+    """The operators together, as a server runs them: one plan a step for all layers, drafts written and attended to in each, one move of
+    the accepted rows, the pages behind them back. Outputs against the formula in 64 bits, the caches byte for byte against
+    what was accepted so far, and no page lost."""
+    specs = [(synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0), 0), (synth.make_layer("cfg3", 1, d_model=D, factor_gain=16.0), 3),
+             (synth.make_layer("cfg2", 2, d_model=D, factor_gain=16.0), 2)]
+    pks = [PhasorKey.from_spec(s) for s, _ in specs]
+    B, most, r = 5, 700, random.Random(12)
+    g = torch.Generator(device="cuda").manual_seed(12)
+    t = lambda *s: torch.randn(s, generator=g, device="cuda")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    caches = [pk.new_cache(B, most, v_bits=bits) for pk, (_, bits) in zip(pks, specs)]
+    lead = caches[0]
+    for c in caches[1:]:
+        c.share_pages(lead)
+    lead.use_page_pool()
+    for pk in pks:
+        pk.set_second(0.002)
+    cap = B * 20 + 7
+    plan, prompts, n_keep, lengths = lead.step_plan(cap, tree=True), lead.step_plan(B * 300), i32([0] * B), i32([0] * B)
+    spaces = [pk.tree_workspace(B, cap, 20, most) for pk in pks]
+    out = torch.zeros((cap, 32, 128), dtype=torch.bfloat16, device="cuda")
+
+    def write(p, n):                                                 # random inputs of n planned tokens, and of the rows behind them
+        for pk, c in zip(pks, caches):
+            pk.write_paged(c, t(p.capacity, D), p.positions, p.slots, v=t(p.capacity, 8, 128).to(torch.bfloat16))
+
+    def rows(c, slots):
+        codes, scales = c.read(slots, 0.002, rows=False)[1:]
+        return [codes, scales] + ([x.view(torch.int16) if x.dtype is torch.bfloat16 else x for x in c.read_vq(slots)[1:]] if c.v_bits else [c.v_rows(slots).view(torch.int16)])
+
+    def place(b, lo, hi):
+        return lead.slots(i32([b] * (hi - lo)), i32(list(range(lo, hi))))
+
+    base = [300, 0, 127, 128, 61]
+    lead.plan_step(prompts, i32(base))
+    write(prompts, sum(base))
+    kept = [[rows(c, place(b, 0, base[b])) for b in range(B)] for c in caches]
+    for round_ in range(6):
+        n = [r.choice([0, 1, 20, r.randint(0, 20)]) for _ in range(B)]
+        chain = round_ == 4                                          # planned without parents where trees were before
+        parents = [[i - 1 if chain else r.randint(max(-1, i - 4), i - 1) for i in range(m)] for m in n]
+        flat = sum(parents, [])
+        lead.plan_step(plan, i32(n), parents=None if chain else i32(flat + [-1] * (cap - len(flat))))
+        write(plan, sum(n))
+        words, positions = [], []
+        for b, m in enumerate(n):
+            w, d = [], []
+            for i, p in enumerate(parents[b]):
+                w.append((w[p] if p >= 0 else 0) | 1 << i)
+                d.append(d[p] + 1 if p >= 0 else 0)
+            words.append(w), positions.append([base[b] + k for k in d])
+        for pk, c, ws in zip(pks, caches, spaces):
+            q = 20 * t(cap, 32, 128)                                 # logits of a few units
+            out.fill_(7.0)
+            pk.tree_step(c, q, plan, ws, out=out)
+            case = object.__new__(Case)
+            case.pk, case.cache, case.q, case.ws, case.base, case.n, case.words, case.positions = pk, c, q, ws, base, n, words, positions
+            case.check(out)
+            assert (out[sum(n):] == 7).all()
+        paths = []
+        for b, m in enumerate(n):
+            path = [r.randrange(m)] if m and r.random() < 0.8 else []
+            while path and parents[b][path[0]] >= 0:
+                path.insert(0, parents[b][path[0]])
+            paths.append(path)
+        cu = plan.cu.tolist()
+        for l, c in enumerate(caches):
+            for b, path in enumerate(paths):
+                if path:
+                    new = rows(c, plan.slots[i32([cu[b] + i for i in path]).long()])
+                    kept[l][b] = [torch.cat([x, y]) for x, y in zip(kept[l][b], new)] if base[b] else new
+        keep = [-1] * cap
+        for b, path in enumerate(paths):
+            keep[cu[b]:cu[b] + len(path)] = path
+        n_keep.copy_(i32([len(p) for p in paths]))
+        lead.keep_rows(plan, i32(keep), n_keep, lengths, layers=caches)
+        lead.truncate(lengths)
+        base = [b + len(p) for b, p in zip(base, paths)]
+        assert lead.seqlens.tolist() == base == lengths.tolist()
+        for l, c in enumerate(caches):
+            for b in range(B):
+                if base[b]:
+                    assert all(torch.equal(x, y) for x, y in zip(rows(c, place(b, 0, base[b])), kept[l][b])), (round_, l, b)
+        used = [p for b in range(B) for p in lead.page_table[b, :-(-base[b] // 128)].tolist()]
+        free = lead.free[1:1 + int(lead.free[0])].tolist()
+        assert sorted(used + free) == list(range(lead.n_pages))
+    assert all(int(s.abs().sum()) == 0 for s in (plan.status, prompts.status, lead.status, *[w.status for w in spaces]))
