@@ -512,3 +512,79 @@ def test_the_status_words_of_a_tree_step_belong_together():
     ws.status.copy_(torch.tensor([4, 77, 0, 0], dtype=torch.int32))               # not cleared: the first problem stays
     c.pk.tree_step(c.cache, c.q, c.plan, ws)
     assert ws.status[:2].tolist() == [4, 77]
+
+
+# The kernel's own roundings, counted one by one (the limits above leave room for one more that it no longer has): a weight is rounded to
+# bf16 once, in the numerator alone (2^-8 A), the result once (2^-8 |O|); the sum takes the weights themselves. The cubic that forms a part of
+# the weights is off by 7.5e-5 of them, in numerator and denominator. An NVFP4 term leaves 0.092 to 0.095 of what it is formed from
+# (2-norm, of normal columns; E2M1 with a scale per 16 of them): 7.8e-4 after three terms, 7.2e-5 after four, here 0.096^4; a logit is off by TERMS s, s = (sum q'_k^2 c_k^2 / d)^1/2,
+# in the 2-norm over many of them, since the residuals' signs are independent of the row. A single one stays below five times that.
+# Uniform over a half step, a rounding is 2^-8 / 3^1/2 of the value in the 2-norm.
+TERMS, ONE = 8.5e-5, 2.0 ** -8 / 3 ** 0.5
+
+
+def spread(c, b, see):
+    """(P, s, V) of sequence b: weights [n, H, T] and logit scales in doubles, values of each query head [H, T, d]."""
+    pk, n, base = c.pk, c.n[b], c.base[b]
+    lo, rep, dev = sum(c.n[:b]), pk.n_q // pk.n_kv, "cuda"
+    slots = c.slots(b, 0, base + n)
+    C, V = c.cache.read(slots, pk.second, codes=False)[0].double(), c.cache.v_rows(slots).double()
+    q = c.q[lo:lo + n].double()
+    ang = torch.tensor(c.positions[b], dtype=torch.float64, device=dev)[:, None] * pk.inv_freq.to(dev)
+    z = (torch.complex(q[..., :64], q[..., 64:]) * torch.polar(torch.ones_like(ang), ang)[:, None])[..., pk.freq.to(dev)]
+    z = pk.A.to(torch.complex128).to(dev).conj().repeat_interleave(rep, 0)[None] * z
+    qa = torch.cat([z.real, z.imag], -1)
+    S = torch.where(see[:, None], qa @ C.T * 128 ** -0.5, -torch.inf)
+    return torch.softmax(S, -1), (qa ** 2 @ C.T ** 2 / 128).sqrt(), V.permute(1, 0, 2).repeat_interleave(rep, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,layout,v_bits,n", [(32, 8, "freq2", 0, 16), (32, 8, "freq2", 0, 64), (32, 32, "freq1", 0, 8), (32, 8, "freq2", 3, 12)])
+def test_no_more_roundings_than_counted(n_q, n_kv, layout, v_bits, n):
+    c = Case(layer(n_q, n_kv, layout), [1900], [n], mask="chain", v_bits=v_bits, q_dtype=torch.float32)
+    out = c.run().double()
+    see = torch.ones((n, 1900 + n), dtype=torch.bool, device="cuda").tril(1900)
+    P, s, V = spread(c, 0, see)
+    O, A = c.formula(0)
+    Q2 = torch.einsum("nht,htd->nhd", P ** 2, V ** 2)                             # what independent errors of the weights add up to, squared
+    L2 = torch.einsum("nht,htd->nhd", (P * s) ** 2, V ** 2) + torch.einsum("nht,nhd->nhd", (P * s) ** 2, O ** 2)
+    most = 5 * TERMS * torch.where(see[:, None], s, 0.0).amax()
+    assert ((out - O).abs() <= 2.0 ** -8 * O.abs() + (2.0 ** -8 + 4 * 7.5e-5 + 2 * most) * A).all()
+    limit = (ONE ** 2 * (Q2.sum() + (O ** 2).sum()) + TERMS ** 2 * L2.sum()).sqrt() + 2 * 7.5e-5 * O.norm()
+    assert float((out - O).norm()) <= float(limit), (float((out - O).norm() / O.norm()), float(limit / O.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,layout", [(32, 8, "freq2"), (32, 32, "freq1")])
+def test_all_four_terms_of_the_query_count(n_q, n_kv, layout):
+    """Rows that see two drafted tokens of nearly the same large logit: the difference of the logits' errors decides, and three terms would leave
+    ten times as much. Queries 60 times as large; for each row the pair of head 0 whose logits are closest."""
+    n = 64
+    c = Case(layer(n_q, n_kv, layout), [0], [n], mask="chain", q_dtype=torch.float32)
+    c.q *= 60.0
+    everything = torch.ones((n, n), dtype=torch.bool, device="cuda")
+    pk = c.pk
+    q = c.q.double()
+    ang = torch.tensor(c.positions[0], dtype=torch.float64, device="cuda")[:, None] * pk.inv_freq.to("cuda")
+    z = (torch.complex(q[:, 0, :64], q[:, 0, 64:]) * torch.polar(torch.ones_like(ang), ang))[:, pk.freq.to("cuda")] * pk.A[0].to(torch.complex128).to("cuda").conj()
+    S = torch.cat([z.real, z.imag], -1) @ c.cache.read(c.slots(0, 0, n), pk.second, codes=False)[0].double().T * 128 ** -0.5
+    value, order = S.sort(-1)
+    near = (value[:, 1:] - value[:, :-1]).argmin(-1)
+    pairs = torch.stack([order.gather(1, near[:, None]), order.gather(1, near[:, None] + 1)], -1)[:, 0].tolist()
+    words = [1 << j | 1 << k for j, k in pairs]
+    c.words = [[w - (1 << 64) if w >> 63 else w for w in words]]
+    c.plan.mask[:n] = torch.tensor(c.words[0], dtype=torch.int64)
+    out = c.run().double()[:, 0]
+    see = torch.zeros_like(everything)
+    for i, (j, k) in enumerate(pairs):
+        see[i, j] = see[i, k] = True
+    P, s, V = spread(c, 0, see)
+    P, s, V = P[:, 0], s[:, 0], V[0]
+    O = P @ V
+    two = torch.tensor(pairs, device="cuda")
+    p, sv, v = P.gather(1, two), s.gather(1, two), V[two]                         # [n, 2], [n, 2], [n, 2, d]
+    delta = (p[:, 0] * p[:, 1]) ** 2 * (sv ** 2).sum(-1) * ((v[:, 0] - v[:, 1]) ** 2).sum(-1)       # squared, for one unit of TERMS
+    round2 = ONE ** 2 * ((p[..., None] * v) ** 2).sum() + ONE ** 2 * (O ** 2).sum()
+    limit = (round2 + (2 * TERMS) ** 2 * delta.sum()).sqrt() + 2 * 7.5e-5 * O.norm()                 # (64 samples: twice the expected 2-norm)
+    assert float(((7.8e-4 / 2) ** 2 * delta.sum()).sqrt()) > float(limit)         # half of what three terms would leave
+    assert float((out - O).norm()) <= float(limit), (float((out - O).norm() / O.norm()), float(limit / O.norm()))
