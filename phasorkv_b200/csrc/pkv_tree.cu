@@ -416,9 +416,9 @@ constexpr uint32_t TM_SFA = 384;      // 4 per (term, K step): scales of the que
 constexpr uint32_t TM_SFB = 448;      // 2 x 16: scales of the page
 constexpr uint32_t TM_COLS = 512;
 
-// MANY: tiles of two kv heads or more. Their values are most of what a page brings, and the page after next can wait: one latent page and
-// four stages of values instead of two and three (16 x 16384 tokens, 6 drafts, 4 kv heads per tile: 140 -> 123 us; 32 drafts of one kv
-// head per tile: 134 -> 150 us).
+// MANY: tiles of two kv heads or more, of bf16 values. Of wide rows, their values are most of what a page brings, and the page after next can
+// wait: one latent page and four stages of values instead of two and three (16 x 16384 tokens, 6 drafts, 4 kv heads per tile: 140 -> 123 us;
+// 32 drafts of one kv head per tile: 134 -> 150 us). The exponentials differ too, see there.
 template <int WP, bool VQ, bool MANY>
 struct Cfg {
     static constexpr int RB = WP / 2, KB = WP / 64, PAGE = page_bytes(WP), CODES = PKV_PAGE_TOKENS * RB;
@@ -438,7 +438,7 @@ struct Cfg {
     static constexpr int SMEM = X_OFF + 6144;
     static constexpr int NTHREADS = VQ ? 512 : 384;
     static constexpr uint64_t SWZ = RB == 128 ? SWZ_128B : SWZ_64B;
-    static_assert(!MANY || (WP == 256 && !VQ), "of wide rows and bf16 values alone");
+    static_assert(!MANY || !VQ, "of bf16 values alone");
     static_assert(SMEM <= 232448 && V_OFF % 1024 == 0 && P_OFF % 1024 == 0, "shared memory of a CTA");
 };
 
@@ -962,9 +962,10 @@ __global__ void __launch_bounds__(Cfg<WP, VQ, MANY>::NTHREADS, 1) pkv_tree_attn_
                         } else {
                             // rounded to bf16 for the tensor core (2^-8 of a weight at most, up as often as down); the sum takes the weights
                             // themselves (over what was rounded it takes 3 % longer: 138 against 134 us for 64 drafts). Five of 16 pairs
-                            // go to the multiply-add units: with none, 2, 4, 5 or 8 of them 131, 126, 128, 122 and 130 us for 64 drafts,
-                            // 123, 117, 118, 115 and 118 for 32. Tiles of several kv heads wait for values and for power (16 x 32768
-                            // tokens, 16 drafts: 289 us with none, 295 with 5): none.
+                            // go to the multiply-add units (2, 4 or 8: slower): 8 x 8192 tokens, 64 drafts take 125 us instead of 129 in
+                            // short runs, 135.6 instead of 137.1 in long ones at the power limit; 128 columns 110.6 instead of 114.2 and 114.4
+                            // instead of 115.3. Tiles of several kv heads wait for values and for power: none (16 x 16384 tokens, 16 drafts,
+                            // 128 columns: 119 and 134 us with none, 122 and 140 with five; 4 x 16384, 32 kv heads: 106.0 and 106.4).
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 float2 t = fma2(make_float2(x[2 * e], x[2 * e + 1]), cs2, mu2);
@@ -1332,7 +1333,7 @@ extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache,
     at.out = (__nv_bfloat16*)out_dev; at.status = status_dev;
     cudaStream_t s = (cudaStream_t)stream;
     if (cache->v_bits) return WP == 256 ? launch<256, true, false>(cache, ab, at, blob_rows, s) : launch<128, true, false>(cache, ab, at, blob_rows, s);
-    if (WP == 128) return launch<128, false, false>(cache, ab, at, blob_rows, s);
     const bool many = (X.shape[max_draft] >> 9 & 7u) > 0;         // kv heads of the largest tree's tiles
+    if (WP == 128) return many ? launch<128, false, true>(cache, ab, at, blob_rows, s) : launch<128, false, false>(cache, ab, at, blob_rows, s);
     return many ? launch<256, false, true>(cache, ab, at, blob_rows, s) : launch<256, false, false>(cache, ab, at, blob_rows, s);
 }

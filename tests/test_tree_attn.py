@@ -588,3 +588,19 @@ def test_all_four_terms_of_the_query_count(n_q, n_kv, layout):
     limit = (round2 + (2 * TERMS) ** 2 * delta.sum()).sqrt() + 2 * 7.5e-5 * O.norm()                 # (64 samples: twice the expected 2-norm)
     assert float(((7.8e-4 / 2) ** 2 * delta.sum()).sqrt()) > float(limit)         # half of what three terms would leave
     assert float((out - O).norm()) <= float(limit), (float((out - O).norm() / O.norm()), float(limit / O.norm()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,layout,n", [(32, 32, "freq1", 8), (32, 8, "freq1", 16), (32, 8, "freq2", 16), (16, 8, "band8", 3)])
+@pytest.mark.parametrize("base", [100, 5000])
+def test_equal_logits_give_the_exact_mean(n_q, n_kv, layout, n, base):
+    """Tiles of several kv heads take every exponential from the hardware, which gives 1 for 0: with queries of zero all weights are 1, sums and
+    result exact in 32 bits. Half of the values are 1, half 1 + 2^-7: the mean is a tie between two bf16 numbers and goes to the even one, 1;
+    any weight off by 1e-5 would decide it."""
+    c = Case(layer(n_q, n_kv, layout), [base], [n], mask="chain")
+    c.q.zero_()
+    s = c.slots(0, 0, base + n).long()
+    c.cache.v[s // PAGE, :, s % PAGE, :] = (1.0 + (torch.arange(base + n, device="cuda") % 2) * 2.0 ** -7).to(torch.bfloat16)[:, None, None]
+    out = c.run()
+    even = [i for i in range(n) if (base + i + 1) % 2 == 0]                       # rows that see as many of one as of the other
+    assert even and (out[even] == 1).all()
