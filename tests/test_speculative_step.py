@@ -335,3 +335,67 @@ def test_ragged_trees_over_layers_that_share_a_page_pool():
         free = lead.free[1:1 + int(lead.free[0])].tolist()
         assert sorted(used + free) == list(range(lead.n_pages))
     assert all(int(s.abs().sum()) == 0 for s in (plan.status, prompts.status, lead.status, *[w.status for w in spaces]))
+
+
+@pytest.mark.parametrize("v_bits,chain", [(0, False), (3, False), (0, True)])
+def test_a_whole_step_in_one_graph(v_bits, chain):
+    """plan, write, attend, keep and truncate captured together and replayed with other drafts, lengths and paths: tables, pages and outputs are
+    those of the calls made one by one."""
+    pk = PhasorKey.from_spec(synth.make_layer("cfg2", 0, d_model=D, factor_gain=16.0))
+    pk.set_second(0.002)
+    B, cap, r = 3, 40, random.Random(21)
+    g = torch.Generator(device="cuda").manual_seed(21)
+    t = lambda *s: torch.randn(s, generator=g, device="cuda")
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")
+    n_new, parents, keep, n_keep = i32([0] * B), i32([-1] * cap), i32([-1] * cap), i32([0] * B)
+    x, q, v = t(cap, D), 20 * t(cap, 32, 128), t(cap, 8, 128).to(torch.bfloat16)
+    x0, v0 = t(400, D), t(400, 8, 128).to(torch.bfloat16)
+
+    class One:
+        def __init__(self):
+            self.cache = pk.new_cache(B, 400, v_bits=v_bits)
+            self.cache.use_page_pool()
+            self.plan, self.ws = self.cache.step_plan(cap, tree=True), pk.tree_workspace(B, cap, 12, 400)
+            self.scratch, self.lengths = pk.write_scratch(cap), i32([0] * B)
+            self.out = torch.zeros((cap, 32, 128), dtype=torch.bfloat16, device="cuda")
+            prompt = self.cache.step_plan(400)
+            self.cache.plan_step(prompt, i32([130, 0, 250]))
+            pk.write_paged(self.cache, x0, prompt.positions, prompt.slots, v=v0)
+
+        def step(self):
+            self.cache.plan_step(self.plan, n_new, parents=None if chain else parents)
+            pk.write_paged(self.cache, x, self.plan.positions, self.plan.slots, v=v, scratch=self.scratch)
+            pk.tree_step(self.cache, q, self.plan, self.ws, out=self.out)
+            self.cache.keep_rows(self.plan, keep, n_keep, self.lengths)
+            self.cache.truncate(self.lengths)
+
+        def state(self):
+            c, p = self.cache, self.plan
+            return [c.page_table, c.seqlens, c.free, c.latent, c.vq if c.v_bits else c.v.view(torch.int16), p.cu, p.slots, p.mask, self.lengths, self.out]
+    one, graphed = One(), One()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        graphed.step()
+    for round_ in range(6):
+        n = [r.choice([0, 1, 12, r.randint(0, 12)]) for _ in range(B)]
+        ups = [[i - 1 if chain else r.randint(max(-1, i - 4), i - 1) for i in range(m)] for m in n]
+        paths = []
+        for up in ups:
+            path = [r.randrange(len(up))] if up else []
+            while path and up[path[0]] >= 0:
+                path.insert(0, up[path[0]])
+            paths.append(path)
+        flat = lambda lists, pad: sum((l + [pad] * (m - len(l)) for l, m in zip(lists, n)), [])
+        n_new.copy_(i32(n)), n_keep.copy_(i32([len(p) for p in paths]))
+        parents[:sum(n)], keep[:sum(n)] = i32(flat(ups, -1)), i32(flat(paths, -1))
+        for a in (x, v):
+            a.copy_(t(*a.shape))
+        q.copy_(20 * t(*q.shape))
+        graph.replay()
+        one.step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(one.state(), graphed.state())), round_
+    assert sum(one.cache.seqlens.tolist()) > 380
+    assert all(int(s.abs().sum()) == 0 for o in (one, graphed) for s in (o.plan.status, o.cache.status, o.ws.status))
