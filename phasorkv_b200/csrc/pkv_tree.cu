@@ -12,9 +12,10 @@
 //   P  = 2^(S - m)              a thread per row and half page: maximum, sum and mask need no other lane
 //   O^T[128 dims x rph] += V_g^T . P_g^T       bf16 tcgen05.mma, a kv head at a time, V as stored
 // A tile of rows of several kv heads reads the latent page once for all of them, and one of 128 rows fills the M of the score MMA.
-// With few drafted tokens the V pages bound it: 131072 tokens, 8 drafts: 70 us, 4.1 TB/s; 16 x 32768 tokens, 16 drafts: 298 us, 3.9 TB/s,
-// where the GPU draws its 1000 W and the clock falls to 1.54 GHz. With many drafts a page and tile takes 2450 cycles (8 x 8192 tokens, 64
-// drafts: 122 to 137 us with the clock): 1536 of MMAs beside 1400 of exponentials and 1000 in which the warps hand over the page.
+// With few drafted tokens a page's load, scores, softmax and P.V wait for one another with little slack between them: 131072 tokens, 8
+// drafts: 70 us, 4.1 TB/s; 16 x 32768 tokens, 16 drafts: 266 us and 4.3 TB/s in short runs, 305 us and 3.8 TB/s in long ones, where the GPU
+// draws its 1000 W and the clock falls to 1.54 GHz. With many drafts a page and tile takes 2450 cycles (8 x 8192 tokens, 64 drafts: 125 us in
+// short runs, 138 in long ones at 1.76 GHz): 1536 of MMAs beside 1400 of exponentials and 1000 in which the warps hand over the page.
 //
 // Three launches: the operand (absorbed queries), the attention, the merge of what several CTAs did of one tile. (A last CTA that
 // merges inside the attention launch waits for a counter and reads the others' partial results alone: slower than the third launch.)
@@ -1333,7 +1334,9 @@ extern "C" int pkv_tree_attn(const pkv_layer_t* layer, const pkv_cache_t* cache,
     at.out = (__nv_bfloat16*)out_dev; at.status = status_dev;
     cudaStream_t s = (cudaStream_t)stream;
     if (cache->v_bits) return WP == 256 ? launch<256, true, false>(cache, ab, at, blob_rows, s) : launch<128, true, false>(cache, ab, at, blob_rows, s);
-    const bool many = (X.shape[max_draft] >> 9 & 7u) > 0;         // kv heads of the largest tree's tiles
+    // kv heads of the largest tree's tiles: the call's own lengths are on the device (16 x 16384 tokens, 6 drafts: 121 us in a workspace for
+    // 6 or 16, 135 in one for 64)
+    const bool many = (X.shape[max_draft] >> 9 & 7u) > 0;
     if (WP == 128) return many ? launch<128, false, true>(cache, ab, at, blob_rows, s) : launch<128, false, false>(cache, ab, at, blob_rows, s);
     return many ? launch<256, false, true>(cache, ab, at, blob_rows, s) : launch<256, false, false>(cache, ab, at, blob_rows, s);
 }

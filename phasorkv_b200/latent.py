@@ -718,7 +718,9 @@ class PhasorKey:
         """Attention of the step's drafted tokens, which are written already: q [n, H, d] pre-RoPE (bf16 or fp32), ragged by
         ``plan.cu``, at ``plan.positions`` -> out [n, H, d] bf16. Row i attends to all tokens cached before the step and to the
         drafted tokens of its sequence named by ``plan.mask[i]`` (a plan without masks: to those up to itself). A row
-        that sees nothing gets zeros, rows behind ``plan.cu[-1]`` are left as they were."""
+        that sees nothing gets zeros, rows behind ``plan.cu[-1]`` are left as they were. A drafted value row with an infinity or NaN
+        makes every output that sees it NaN as a whole. Make the workspace for the draft counts in use: one for far larger
+        trees picks the kernel form of those."""
         self._need_inv_freq("tree_step")
         n, dev = q.shape[0], cache.latent.device
         if q.dtype not in (torch.bfloat16, torch.float32):
