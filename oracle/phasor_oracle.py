@@ -176,7 +176,9 @@ def nvfp4_dequantize(codes: torch.Tensor, scale_bytes: torch.Tensor, second) -> 
 
 def nv_static_second(var: torch.Tensor) -> torch.Tensor:
     """Static tensor scale: 32 sigma of the widest channel over (448 * 6) (quant.py:119-124)."""
-    return (32 * var.max().clamp_min(1e-30).sqrt() / (E4M3_MAX * E2M1_MAX)).reshape(1).float()
+    top = var.max().clamp_min(1e-30)
+    # (through fp64, which rounds an fp32 root correctly: some host libraries' fp32 roots are off by a bit)
+    return (32 * top.double().sqrt().to(top.dtype) / (E4M3_MAX * E2M1_MAX)).reshape(1).float()
 
 
 # ----------------------------------------------------------------------------------------------
