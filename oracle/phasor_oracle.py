@@ -53,6 +53,19 @@ def to_complex(x: torch.Tensor) -> torch.Tensor:
 # PhasorKey (phasorkv/latent.py)
 # ----------------------------------------------------------------------------------------------
 
+def _product(a: torch.Tensor, b: torch.Tensor) -> torch.Tensor:
+    """a @ b. Small fp32 products add up over the inner index, one fused multiply-add after the other, as the stored vectors were formed: host
+    libraries differ in their order, by a last bit. (A product of fp32 numbers is exact in fp64.) Larger ones, which are only
+    held to tolerances, are the host library's."""
+    if a.dtype != torch.float32 or b.dtype != torch.float32 or a.numel() * b.shape[-1] > 1 << 22:
+        return a @ b
+    c = torch.zeros((*a.shape[:-1], b.shape[-1]), dtype=torch.float32)
+    a, b = a.double(), b.double()
+    for k in range(a.shape[-1]):
+        c = (a[..., k:k + 1] * b[k] + c.double()).float()
+    return c
+
+
 class PhasorKeyOracle:
     """write / absorb / scores on injected factors (the attributes latent.py:47-54 builds)."""
 
@@ -82,12 +95,12 @@ class PhasorKeyOracle:
         """x [T, D], ph [T, h] -> rows [T, 2R + R_s] laid out [Re c_rot | Im c_rot | slow]."""
         rd = torch.float64 if x.dtype == torch.float64 else torch.float32
         xr = x.to(rd)
-        re = xr @ self.B.real.to(rd).T
-        im = xr @ self.B.imag.to(rd).T
+        re = _product(xr, self.B.real.to(rd).T)
+        im = _product(xr, self.B.imag.to(rd).T)
         c = torch.complex(re, im) * ph[:, self.freq].to(torch.complex128 if rd == torch.float64 else torch.complex64)
         out = [c.real, c.imag]
         if self.R_s:
-            out.append(xr @ self.B_s.to(rd).T)
+            out.append(_product(xr, self.B_s.to(rd).T))
         return torch.cat(out, dim=-1)
 
     def absorb(self, q: torch.Tensor, ph: torch.Tensor) -> torch.Tensor:
@@ -106,7 +119,7 @@ class PhasorKeyOracle:
     @staticmethod
     def scores(q_abs: torch.Tensor, cache: torch.Tensor) -> torch.Tensor:
         """Unscaled logits [H, Tq, Tk]."""
-        return q_abs @ cache.T.to(q_abs.dtype)
+        return _product(q_abs, cache.T.to(q_abs.dtype))
 
 
 # ----------------------------------------------------------------------------------------------
