@@ -604,3 +604,27 @@ def test_equal_logits_give_the_exact_mean(n_q, n_kv, layout, n, base):
     out = c.run()
     even = [i for i in range(n) if (base + i + 1) % 2 == 0]                       # rows that see as many of one as of the other
     assert even and (out[even] == 1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,layout,v_bits", [(32, 8, "freq2", 0), (32, 32, "freq1", 0), (32, 8, "band8", 0), (32, 8, "freq2", 3)])
+def test_one_token_a_sequence_is_decode_attention(n_q, n_kv, layout, v_bits):
+    """A batch of which nobody drafts: the decode kernel's outputs (within 2e-3 of the formula in the 2-norm) to two roundings to bf16. The same in a
+    workspace for the widest tree, which picks other tiles."""
+    c = Case(layer(n_q, n_kv, layout), [1, 127, 128, 900, 3000, 2], [1] * 6, mask="chain", v_bits=v_bits)
+    c.check(c.run())
+    ws = c.pk.workspace(6, c.pk.default_splits(6, 3001))
+    want = c.pk.decode(c.cache, c.q.float(), c.plan.positions, ws).double()
+    wide = c.pk.tree_workspace(6, c.cap, 64, c.cache.max_pages * PAGE)
+    for space in (c.ws, wide):
+        out = c.pk.tree_step(c.cache, c.q, c.plan, space).double()
+        assert float((out - want.view_as(out)).norm()) <= (2e-3 + NORM) * float(want.norm())
+        assert int(space.status.abs().sum()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n_q,n_kv,layout,v_bits", [(32, 8, "freq2", 0), (32, 32, "freq1", 0), (32, 8, "freq2", 2)])
+def test_small_trees_in_a_workspace_for_the_widest(n_q, n_kv, layout, v_bits):
+    c = Case(layer(n_q, n_kv, layout), [700, 0, 255, 1500], [6, 1, 0, 17], v_bits=v_bits)
+    c.ws = c.pk.tree_workspace(4, c.cap, 64, c.cache.max_pages * PAGE)
+    c.check(c.run())
