@@ -171,3 +171,15 @@ def test_tree_step_refuses_another_devices_workspace_or_layer(wrong):
     ws.batch, ws.capacity, ws.max_draft, ws.max_pages, ws.key, ws.at, ws.bytes, ws.status_at = 1, 4, 4, 1, pk._tree_key(), 0, 0, 0
     with pytest.raises(ValueError, match="device"):
         pk.tree_step(cache, torch.zeros((4, 32, 128)), cache.step_plan(4), ws)
+
+
+def test_a_workspace_refuses_a_buffer_that_does_not_hold_it():
+    ws = object.__new__(TreeWorkspace)
+    ws.bytes = 2048
+    room = torch.zeros(8192, dtype=torch.uint8)
+    at = -room.data_ptr() % 1024
+    for bad in (room[at:at + 2047], room[at + 16:at + 4096], room[at:at + 4096].view(torch.int32), room[at:at + 4096 + 2048:2]):
+        with pytest.raises(ValueError):
+            ws.use(bad)
+    ws.use(room[at:at + 2048])
+    assert ws.at == room.data_ptr() + at
